@@ -313,6 +313,94 @@ int ts_mse_pieces_fwd_bwd(const void* const* s_pieces, const void* const* t_piec
                           int accumulate, void* workspace, float* loss_out, int dtype,
                           ts_stream_t stream);
 
+/* ------------------------------------------------------------------------ */
+/* Losses on rows of vocabulary logits that the reference does not have:     */
+/* sparse teachers and post-training objectives.  Shared conventions:        */
+/*   s: logits, n_seq sequences of seq_len tokens; the row of token t of      */
+/*     sequence q starts at s + q * ld_seq + t * ld_tok elements (any          */
+/*     strides, slices included); V contiguous elements a row, V < 2^31 - 64;   */
+/*     n_seq * seq_len < 2^22 rows (else TS_ERR_RANGE);                         */
+/*   grad: dense [n_seq, seq_len, V], every element written, may be NULL (loss  */
+/*     only) where the function also returns a loss;                            */
+/*   labels: int64 per row; a row counts when its label differs from             */
+/*     ignore_index, lies in [0, V) and row_mask (a byte per row, may be NULL)    */
+/*     is not 0.  Rows that do not count are not read; their outputs and gradients */
+/*     are 0;                                                                      */
+/*   temperature T in [1e-30, 1e30]; fp32 arrays are 4-byte, workspaces 16-byte     */
+/*     aligned.  Per-row sums are fp32, sums over rows 64-bit in a fixed order.      */
+/* ------------------------------------------------------------------------ */
+
+/* logp[r] = ln softmax(s_r / T)[labels[r]], 0 for rows that do not count.
+ * stats (2 floats per row, 8-byte aligned, may be NULL): the row's maximum and
+ * sum, what the backward pass takes. */
+int ts_token_logp_fwd(const void* s, int64_t n_seq, int64_t seq_len, int64_t V, int64_t ld_seq,
+                      int64_t ld_tok, const int64_t* labels, const uint8_t* row_mask,
+                      int64_t ignore_index, double temperature, float* logp, float* stats, int dtype,
+                      ts_stream_t stream);
+
+/* grad = grad_logp[r] / T * (onehot(labels[r]) - softmax(s_r / T)). */
+int ts_token_logp_bwd(const void* s, int64_t n_seq, int64_t seq_len, int64_t V, int64_t ld_seq,
+                      int64_t ld_tok, const int64_t* labels, const uint8_t* row_mask,
+                      int64_t ignore_index, double temperature, const float* stats,
+                      const float* grad_logp, void* grad, int dtype, ts_stream_t stream);
+
+/* Workspace of the two losses below. */
+size_t ts_token_loss_workspace_bytes(int64_t n_seq, int64_t seq_len);
+
+/* Preference loss over pairs: sequence 2i is preferred to sequence 2i + 1.
+ *   R_q = sum (average != 0: mean) over the rows that count of logp - ref,
+ *   h_i = R_2i - R_2i+1,  loss = weight * mean_i f(h_i)
+ *   kind 0: f = -(1 - smoothing) ln sigmoid(beta h) - smoothing ln sigmoid(-beta h)
+ *   kind 1: f = max(0, 1 - beta h);  kind 2: f = (h - 1 / (2 beta))^2
+ * ref_logp: per row (ref_per_token != 0) or, already summed (or averaged), per
+ * sequence.  rewards (may be NULL): beta * R_q.  n_seq even; no pairs: NaN. */
+int ts_preference_fwd_bwd(const void* s, int64_t n_seq, int64_t seq_len, int64_t V, int64_t ld_seq,
+                          int64_t ld_tok, const int64_t* labels, const uint8_t* row_mask,
+                          int64_t ignore_index, const float* ref_logp, int ref_per_token,
+                          double beta, int kind, double smoothing, int average, double weight,
+                          void* workspace, float* loss_out, float* rewards, void* grad, int dtype,
+                          ts_stream_t stream);
+
+/* Clipped policy loss with a KL term.  Per row that counts, r = e^(logp - old):
+ *   term = -min(r A, clip(r, clip_lo, clip_hi) A) + kl_weight (e^d - d - 1),  d = ref - logp
+ * loss = weight * mean of the terms over all rows that count or, with per_seq,
+ * the mean over the sequences that have such rows of each one's mean.
+ * advantages: per row or (adv_per_seq) per sequence; ref_logp may be NULL when
+ * kl_weight is 0.  logp (may be NULL): as ts_token_logp_fwd gives it.  No row
+ * counts: NaN. */
+int ts_policy_fwd_bwd(const void* s, int64_t n_seq, int64_t seq_len, int64_t V, int64_t ld_seq,
+                      int64_t ld_tok, const int64_t* labels, const uint8_t* row_mask,
+                      int64_t ignore_index, double temperature, const float* old_logp,
+                      const float* ref_logp, const float* advantages, int adv_per_seq,
+                      double kl_weight, double clip_lo, double clip_hi, int per_seq, double weight,
+                      void* workspace, float* loss_out, float* logp, void* grad, int dtype,
+                      ts_stream_t stream);
+
+/* The k largest logits of each row, largest first, equal ones by their place
+ * (NaN counts as largest): values [rows, k] in the logits' type, indices
+ * [rows, k]; logsumexp (may be NULL): ln sum e^(s / T) per row.
+ * 1 <= k <= min(V, 256) (more than 256: TS_ERR_RANGE). */
+int ts_top_logits(const void* s, int64_t n_seq, int64_t seq_len, int64_t V, int64_t ld_seq,
+                  int64_t ld_tok, int k, double temperature, void* values, int32_t* indices,
+                  float* logsumexp, int dtype, ts_stream_t stream);
+
+/* Distillation from such rows.  Entries whose index lies outside [0, V) are
+ * absent, those of value -inf weigh nothing.  q = softmax(s / T);
+ *   t_logsumexp NULL: p = softmax over the row's entries, term = sum p (ln p - ln q)
+ *   else: p = e^(value / T - t_logsumexp), and the tokens without an entry form one
+ *     more outcome of probability 1 - sum p on one side, their q's sum on the other
+ * loss = weight * T^2 * mean of the terms over the rows of row_mask (NULL: all).
+ * t_dtype: type of t_values [rows, k]; k <= 256; with t_logsumexp V <= 2^20
+ * (else TS_ERR_RANGE). */
+size_t ts_top_distil_workspace_bytes(int64_t n_rows);
+
+int ts_top_distil_fwd_bwd(const void* s, int64_t n_seq, int64_t seq_len, int64_t V, int64_t ld_seq,
+                          int64_t ld_tok, const void* t_values, int t_dtype,
+                          const int32_t* t_indices, const float* t_logsumexp, int k,
+                          const uint8_t* row_mask, double temperature, double weight,
+                          void* workspace, float* loss_out, void* grad, int dtype,
+                          ts_stream_t stream);
+
 /* Cosine embedding loss with target +1, forward and backward: the hidden-state
  * term of DistilBERT's loss (benchmarks/distilbert/distiller.py:756-770,
  * nn.CosineEmbeddingLoss(reduction="mean") on the rows the attention mask keeps):

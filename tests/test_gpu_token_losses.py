@@ -1,0 +1,504 @@
+"""GPU parity of the token losses (log probabilities, preference, clipped
+policy) against 64-bit statements on the CPU.
+
+Tolerances.  A row's sum z of 2^((x - m) k) has terms off by the exponent's
+two roundings, relative |x - m| k ln2 2^-23 (the shares of terms with
+|x - m| / T above 16 vanish, so 16 * 2^-23 = 1.9e-6), and v_exp_f32's unit in
+the last place; adding them up in fp32, a few hundred to a thread at most,
+stays below 2e-6.  So a log probability is off by at most 4e-6 besides the
+rounding of the fp32 result, a probability q by 1e-5 q, and a gradient
+c (onehot - q) by 1e-5 |c| q, the half step of its storage type and the
+rounding of 1 - q at 2^-24 |c|.
+"""
+import pytest
+import torch
+
+import token_oracle as ref64
+import tspipe_amd as ta
+from helpers import bits_equal, seeded
+
+pytestmark = pytest.mark.gpu
+DTYPES = [torch.float32, torch.bfloat16, torch.float16]
+LOGP_ABS = 4e-6
+
+
+def check_logp(got, want, extra=0.0):
+    got, want = got.detach().cpu().double(), want.detach().double()
+    assert got.shape == want.shape
+    err = (got - want).abs()
+    assert (err <= LOGP_ABS + extra + 2.0 ** -24 * want.abs()).all(), err.max().item()
+
+
+def check_grad(got, want, dtype, coef=None):
+    """`coef`: largest |c| of the rows, [...] against gradients [..., V]."""
+    assert got.dtype == dtype and got.shape == want.shape
+    g, w = got.detach().cpu().double(), want.double()
+    fi = torch.finfo(dtype)
+    c = w.abs().amax(-1, keepdim=True) if coef is None else coef
+    # half a step of fp16's subnormals is felt; those of the wider types may be flushed
+    least = fi.smallest_normal * fi.eps if dtype == torch.float16 else fi.smallest_normal
+    # (the coefficient itself comes from sums of log probabilities: 1e-5 relative covers it)
+    tol = (fi.eps / 2 * 1.001 + 2e-5) * w.abs() + 2.0 ** -22 * c + least
+    bad = (g - w).abs() > tol
+    assert not bad.any(), ((g - w).abs() / tol).max().item()
+
+
+def make(shape, dtype, seed, std=2.5):
+    g = seeded(seed)
+    x = (torch.randn(*shape, generator=g) * std).to(dtype)
+    labels = torch.randint(0, shape[-1], shape[:-1], generator=g)
+    lift = torch.rand(*shape[:-1], 1, generator=g) * 8
+    x.scatter_(-1, labels[..., None], lift.to(dtype))
+    return x, labels, g
+
+
+SIZES = [(1, 1, 1), (1, 1, 2), (2, 3, 7), (2, 5, 100), (3, 4, 255), (2, 2, 1000), (2, 3, 2049), (2, 7, 4099), (2, 2, 8193),
+         (2, 3, 30522), (2, 2, 32001), (2, 2, 50257), (2, 1, 65537), (2, 1, 131072), (2, 1, 140003)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,L,V", SIZES)
+def test_log_probs(device, n, L, V, dtype):
+    x, labels, g = make((n, L, V), dtype, 10 + V)
+    if n * L > 2:
+        labels[0, 0] = -100
+        labels[-1, -1] = V  # outside: does not count either
+    T = 0.9 if V % 2 else 1.0
+    x64 = x.double().requires_grad_()
+    want, live = ref64.log_probs(x64, labels, T)
+    go = torch.randn(n, L, generator=g)
+    want.backward(go.double())
+    xd = x.to(device).requires_grad_()
+    got = ta.token_log_probs(xd, labels.to(device), T)
+    assert got.dtype == torch.float32
+    check_logp(got, want)
+    got.backward(go.to(device))
+    check_grad(xd.grad, x64.grad, dtype, coef=(go.abs() / T)[..., None])
+    assert (xd.grad.cpu()[~live] == 0).all()
+    with torch.no_grad():
+        again = ta.token_log_probs(xd, labels.to(device), T)
+    assert not again.requires_grad and bits_equal(again, got)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("V,cut", [(37, 1), (1000, 1), (4099, 2), (30522, 1)])
+def test_log_probs_of_slices_and_shifted_bases(device, V, cut, dtype):
+    # the logits without each sequence's last positions, a transposed batch, and rows off a 16-byte
+    # boundary are read where they lie; where the rows start at the same distances from such a boundary
+    # as a dense copy's (V a multiple of 8), the sums run in the same order and give the same bits
+    x, labels, g = make((3, 6, V), dtype, 77 + V)
+    go = torch.randn(3, 6 - cut, generator=g)
+    lab = labels[:, cut:].contiguous()
+    x64 = x[:, :-cut].double().requires_grad_()
+    want, _ = ref64.log_probs(x64, lab)
+    want.backward(go.double())
+    xd, labd, god = x.to(device), lab.to(device), go.to(device)
+    dense = xd[:, :-cut].contiguous().requires_grad_()
+    plain = ta.token_log_probs(dense, labd)
+    plain.backward(god)
+    pad = torch.zeros(3 * 6 * V + 3, dtype=dtype, device=device)
+    pad[3:] = xd.reshape(-1)
+    views = {
+        "slice": xd.clone(),
+        "token major": xd.permute(1, 0, 2).contiguous().permute(1, 0, 2),
+        "shifted": pad[3:].view(3, 6, V),
+        "last dimension not dense": xd.transpose(1, 2).contiguous().transpose(1, 2),
+    }
+    for name, v in views.items():
+        leaf = v.detach().requires_grad_()
+        out = ta.token_log_probs(leaf[:, :-cut], labd)
+        out.backward(god)
+        check_logp(out, want)
+        check_grad(leaf.grad[:, :-cut], x64.grad, dtype, coef=go.abs()[..., None])
+        assert (leaf.grad[:, -cut:] == 0).all()
+        if V % 8 == 0 and name != "shifted":
+            assert bits_equal(out, plain) and bits_equal(leaf.grad[:, :-cut], dense.grad), name
+
+
+def test_log_probs_row_mask_and_label_types(device):
+    x, labels, g = make((4, 5, 501), torch.float32, 3)
+    mask = torch.rand(4, 5, generator=g) < 0.5
+    want, _ = ref64.log_probs(x.double(), labels.masked_fill(~mask, -100))
+    for m in (mask, mask.to(torch.int32) * 3, mask.float()):
+        for lab in (labels, labels.to(torch.int32)):
+            check_logp(ta.token_log_probs(x.to(device), lab.to(device), row_mask=m.to(device)), want)
+    odd = labels.clone()
+    odd[0] = 7
+    check_logp(ta.token_log_probs(x.to(device), odd.to(device), ignore_index=7),
+               ref64.log_probs(x.double(), odd.masked_fill(odd == 7, -100))[0])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_log_probs_extreme_logits(device, dtype):
+    V = 3001
+    x, labels, g = make((1, 8, V), dtype, 5)
+    fi = torch.finfo(dtype)
+    labels[:] = 0
+    x[0, 0, 5:] = float("-inf")              # a masked vocabulary
+    x[0, 1, 5:] = fi.min                     # masked by the type's lowest value
+    x[0, 2, :] = fi.min                      # all of it: equal logits
+    x[0, 3, :] = 0                           # equal logits
+    x[0, 4, 1:] = float("-inf")              # one class left
+    x[0, 5, 7] = 80.0                        # far from the label
+    x[0, 6, 0], x[0, 6, 1] = 60.0, 59.5      # large, close
+    x[0, 7, 9] = float("-inf")
+    x64 = x.double().requires_grad_()
+    want, _ = ref64.log_probs(x64, labels)
+    go = torch.randn(1, 8, generator=g)
+    want.backward(go.double())
+    xd = x.to(device).requires_grad_()
+    got = ta.token_log_probs(xd, labels.to(device))
+    check_logp(got, want)
+    got.backward(go.to(device))
+    check_grad(xd.grad, x64.grad, dtype, coef=go.abs()[..., None])
+
+
+def test_log_probs_nan_and_infinities(device):
+    x, labels, _ = make((1, 6, 700), torch.float32, 6)
+    x[0, 0, 13] = float("nan")
+    x[0, 1, 13] = float("inf")
+    x[0, 2, :] = float("-inf")
+    x[0, 3, labels[0, 3]] = float("-inf")
+    x[0, 4, :] = float("nan")
+    labels[0, 4] = -100  # not read
+    got = ta.token_log_probs(x.to(device), labels.to(device)).cpu()[0]
+    assert torch.isnan(got[:3]).all() and got[3] == float("-inf") and got[4] == 0 and torch.isfinite(got[5])
+    xd = x.to(device).requires_grad_()
+    ta.token_log_probs(xd, labels.to(device)).sum().backward()
+    assert (xd.grad[0, 4] == 0).all() and torch.isfinite(xd.grad[0, 5]).all()
+
+
+def test_log_probs_empty(device):
+    for shape in [(0, 4, 10), (3, 0, 10), (0, 10)]:
+        x = torch.zeros(shape, device=device, requires_grad=True)
+        out = ta.token_log_probs(x, torch.zeros(shape[:-1], dtype=torch.int64, device=device))
+        assert out.shape == shape[:-1]
+        out.sum().backward()
+        assert x.grad.shape == shape
+    x = torch.randn(10, device=device)
+    out = ta.token_log_probs(x, torch.tensor(3, device=device))
+    check_logp(out, x.cpu().double().log_softmax(-1)[3])
+
+
+def test_log_probs_against_differences(device):
+    x, labels, g = make((2, 4, 777), torch.float32, 8, std=1.0)
+    d = torch.randn(x.shape, generator=g).to(device)
+    go = torch.randn(2, 4, generator=g).to(device)
+    xd = x.to(device).requires_grad_()
+    lab = labels.to(device)
+    ta.token_log_probs(xd, lab).backward(go)
+    h = 1e-2
+    up, down = (ta.token_log_probs((xd + s * h * d).detach(), lab) for s in (1, -1))
+    numeric = ((up.double() - down.double()) * go).sum() / (2 * h)
+    # eight log probabilities off by 4e-6 each over 2 h, and h^2 / 6 times third cumulants of order one
+    tol = 8 * LOGP_ABS / h * go.abs().max().item() + 8 * h * h
+    assert abs(numeric.item() - (xd.grad.double() * d).sum().item()) < tol
+
+
+# ---- preference ------------------------------------------------------------------------
+
+def ragged(labels, g, empty=()):
+    L = labels.shape[1]
+    for i in range(labels.shape[0]):
+        a, b = sorted(torch.randint(0, L + 1, (2,), generator=g).tolist())
+        labels[i, :a] = -100
+        labels[i, max(b, a + 1):] = -100
+        if i in empty:
+            labels[i] = -100
+    return labels
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("kind,smoothing,average", [("sigmoid", 0.0, False), ("sigmoid", 0.2, True), ("hinge", 0.0, False),
+                                                    ("ipo", 0.0, True), ("ipo", 0.0, False)])
+@pytest.mark.parametrize("pairs,L,V", [(1, 1, 5), (1, 9, 4099), (3, 17, 1000), (5, 6, 30522), (2, 300, 131)])
+def test_preference(device, pairs, L, V, kind, smoothing, average, dtype):
+    x, labels, g = make((2 * pairs, L, V), dtype, 1000 + V + L)
+    if L > 1:
+        labels = ragged(labels, g, empty=(1,) if pairs > 1 else ())
+    ref = ref64.log_probs(x.double(), labels)[0].float() + torch.randn(2 * pairs, L, generator=g) * 0.2
+    beta, weight = 0.3, 64.0
+    x64 = x.double().requires_grad_()
+    want, rewards = ref64.preference(x64, labels, ref.double(), beta, kind, smoothing, average, weight)
+    want.backward()
+    xd = x.to(device).requires_grad_()
+    loss, got_r = ta.preference_loss(xd, labels.to(device), ref.to(device), beta, kind, smoothing, average, weight,
+                                     return_rewards=True)
+    loss.backward()
+    # an answer's sum is off by 4e-6 a token; its reward by beta times that, the loss by weight * |f'| times two
+    n_tok = 1 if average else L
+    slope = {"sigmoid": beta, "hinge": beta, "ipo": 2 * (rewards.abs().max().item() * 2 / beta + 1 / (2 * beta))}[kind]
+    assert ((got_r.cpu().double() - rewards).abs() <= beta * n_tok * LOGP_ABS + 2.0 ** -24 * rewards.abs()).all()
+    assert abs(loss.item() - want.item()) <= weight * slope * 2 * n_tok * LOGP_ABS + 2.0 ** -23 * abs(want.item())
+    assert not got_r.requires_grad and loss.dtype == torch.float32
+    # the factor c inherits the sums' error through f''
+    curve = {"sigmoid": beta * beta / 4, "hinge": 0.0, "ipo": 2.0}[kind] * weight / pairs * 2 * n_tok * LOGP_ABS
+    check_grad(xd.grad, x64.grad, dtype, coef=x64.grad.abs().amax(-1, keepdim=True) + curve * 2 ** 22)
+    # loss alone, and a reference summed per answer
+    with torch.no_grad():
+        assert bits_equal(ta.preference_loss(xd, labels.to(device), ref.to(device), beta, kind, smoothing, average, weight),
+                          loss.detach())
+    live = labels >= 0
+    per = torch.where(live, ref, torch.zeros_like(ref)).double().sum(-1)
+    if average:
+        per = per / live.sum(-1).clamp_min(1)
+    per = per.float()
+    want2, r2 = ref64.preference(x.double(), labels, per.double(), beta, kind, smoothing, average, weight)
+    loss2, got2 = ta.preference_loss(xd, labels.to(device), per.to(device), beta, kind, smoothing, average, weight,
+                                     return_rewards=True)
+    assert ((got2.cpu().double() - r2).abs() <= beta * n_tok * LOGP_ABS + 2.0 ** -24 * r2.abs()).all()
+    slope2 = slope if kind != "ipo" else 2 * (r2.abs().max().item() * 2 / beta + 1 / (2 * beta))
+    assert abs(loss2.item() - want2.item()) <= weight * slope2 * 2 * n_tok * LOGP_ABS + 2.0 ** -23 * abs(want2.item())
+
+
+def test_preference_empty_and_extreme(device):
+    x = torch.zeros(0, 4, 10, device=device, requires_grad=True)
+    loss = ta.preference_loss(x, torch.zeros(0, 4, dtype=torch.int64, device=device), torch.zeros(0, 4, device=device))
+    assert torch.isnan(loss)
+    loss.backward()
+    x = torch.zeros(2, 0, 10, device=device, requires_grad=True)
+    loss = ta.preference_loss(x, torch.zeros(2, 0, dtype=torch.int64, device=device), torch.zeros(2, device=device))
+    assert abs(loss.item() - 0.6931471805599453) < 1e-6
+    loss.backward()
+    # far apart: neither side overflows
+    x, labels, g = make((2, 40, 300), torch.float32, 12)
+    for sign in (1.0, -1.0):
+        shift = torch.tensor([5000.0, -5000.0]) * sign
+        want, _ = ref64.preference(x.double(), labels, shift.double(), 1.0)
+        xd = x.to(device).requires_grad_()
+        loss = ta.preference_loss(xd, labels.to(device), shift.to(device), 1.0)
+        loss.backward()
+        assert abs(loss.item() - want.item()) <= 1e-6 * abs(want.item()) + 1e-6
+        assert torch.isfinite(xd.grad).all()
+    # NaN logits in a row that does not count, and in one that does
+    x[0, 3] = float("nan")
+    labels[0, 3] = -100
+    xd = x.to(device).requires_grad_()
+    loss = ta.preference_loss(xd, labels.to(device), torch.zeros(2, device=device))
+    loss.backward()
+    assert torch.isfinite(loss) and torch.isfinite(xd.grad).all() and (xd.grad[0, 3] == 0).all()
+    labels[0, 3] = 5
+    assert torch.isnan(ta.preference_loss(xd, labels.to(device), torch.zeros(2, device=device)))
+
+
+# ---- clipped policy loss -------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("reduction", ["token", "sequence"])
+@pytest.mark.parametrize("per_answer", [True, False])
+@pytest.mark.parametrize("n,L,V,kl,T", [(1, 1, 3, 0.0, 1.0), (3, 7, 1000, 0.1, 0.7), (4, 9, 4099, 0.0, 1.0),
+                                        (3, 5, 30522, 0.05, 1.0), (2, 3, 70001, 0.1, 1.5), (5, 200, 127, 0.3, 1.0)])
+def test_policy(device, n, L, V, kl, T, per_answer, reduction, dtype):
+    x, labels, g = make((n, L, V), dtype, 2000 + V + L)
+    if L > 1:
+        labels = ragged(labels, g, empty=(1,))
+    base = ref64.log_probs(x.double(), labels, T)[0].float()
+    drift = torch.randn(n, L, generator=g) * 0.25
+    # ratios within 1e-4 of an end of the clipping range are moved: there the last bits decide
+    ends = torch.minimum((torch.exp(-drift) - 0.9).abs(), (torch.exp(-drift) - 1.3).abs()) < 1e-4
+    old = base + drift.masked_fill(ends, 0.0)
+    rlp = base + torch.randn(n, L, generator=g) * 0.3
+    adv = torch.randn(n, generator=g) if per_answer else torch.randn(n, L, generator=g)
+    weight = 32.0 * n * L
+    x64 = x.double().requires_grad_()
+    want, lp = ref64.policy(x64, labels, old.double(), adv.double(), rlp.double(), kl, 0.1, 0.3, T, reduction, weight)
+    want.backward()
+    xd = x.to(device).requires_grad_()
+    loss, got_lp = ta.clipped_policy_loss(xd, labels.to(device), old.to(device), adv.to(device),
+                                          rlp.to(device) if kl else None, kl, 0.1, 0.3, T, reduction, weight,
+                                          return_log_probs=True)
+    loss.backward()
+    check_logp(got_lp, lp)
+    # a term moves by |A| r + kl e^d times its log probability's error
+    steep = adv.abs().max().item() * 2 + 2 * kl
+    assert abs(loss.item() - want.item()) <= weight * steep * LOGP_ABS + 2.0 ** -23 * abs(want.item())
+    per_row = weight / (1 if reduction == "sequence" else max(1, int((labels >= 0).sum())))
+    check_grad(xd.grad, x64.grad, dtype,
+               coef=x64.grad.abs().amax(-1, keepdim=True) + per_row / T * (kl + steep) * LOGP_ABS * 2 ** 22)
+    with torch.no_grad():
+        assert bits_equal(ta.clipped_policy_loss(xd, labels.to(device), old.to(device), adv.to(device),
+                                                 rlp.to(device) if kl else None, kl, 0.1, 0.3, T, reduction, weight),
+                          loss.detach())
+
+
+def test_policy_empty_and_nothing_counts(device):
+    for n, L in [(0, 3), (2, 0), (2, 3)]:
+        for reduction in ("token", "sequence"):
+            x = torch.randn(n, L, 50, device=device).requires_grad_()
+            labels = torch.full((n, L), -100, device=device)
+            z = torch.zeros(n, L, device=device)
+            loss = ta.clipped_policy_loss(x, labels, z, z, reduction=reduction)
+            assert torch.isnan(loss)
+            loss.backward()
+            assert (x.grad == 0).all()
+
+
+def test_policy_gradient_stops_at_the_clip(device):
+    x, labels, g = make((1, 4, 64), torch.float32, 31)
+    lp = ref64.log_probs(x.double(), labels)[0].float()
+    old = lp - torch.tensor([[0.5, 0.5, -0.5, -0.5]])     # ratios e^.5, e^.5, e^-.5, e^-.5
+    adv = torch.tensor([[1.0, -1.0, 1.0, -1.0]])
+    xd = x.to(device).requires_grad_()
+    ta.clipped_policy_loss(xd, labels.to(device), old.to(device), adv.to(device)).backward()
+    moved = xd.grad.abs().amax(-1).cpu()[0] > 0
+    assert moved.tolist() == [False, True, True, False]
+
+
+@pytest.mark.parametrize("which", ["preference", "policy"])
+def test_losses_against_differences(device, which):
+    x, labels, g = make((2, 5, 400), torch.float32, 41, std=1.0)
+    base = ref64.log_probs(x.double(), labels)[0].float()
+    rlp = (base + 0.3 * torch.randn(2, 5, generator=g)).to(device)
+    old = (base + 0.05 * torch.randn(2, 5, generator=g)).to(device)
+    adv = torch.randn(2, 5, generator=g).to(device)
+    lab = labels.to(device)
+
+    def f(t):
+        if which == "preference":
+            return ta.preference_loss(t, lab, rlp, 0.5)
+        return ta.clipped_policy_loss(t, lab, old, adv, rlp, 0.2, clip_low=10.0, clip_high=10.0)
+
+    d = torch.randn(x.shape, generator=g).to(device) * 0.3
+    xd = x.to(device).requires_grad_()
+    f(xd).backward()
+    h = 1e-2
+    with torch.no_grad():
+        numeric = (f(xd + h * d).double() - f(xd - h * d).double()).item() / (2 * h)
+    # losses of order one off by 1e-5 over 2 h, and h^2 / 6 times a third derivative of order ten along d
+    assert abs(numeric - (xd.grad.double() * d).sum().item()) < 1e-5 / h + 20 * h * h
+
+
+def test_scaled_backward_runs_once(device):
+    x, labels, g = make((2, 4, 600), torch.float32, 51)
+    ref = torch.zeros(2, 4, device=device)
+    a, b = (x.to(device).requires_grad_() for _ in range(2))
+    la = ta.preference_loss(a, labels.to(device), ref)
+    la.backward()
+    lb = ta.preference_loss(b, labels.to(device), ref)
+    (lb * 3.0).backward()
+    assert torch.allclose(b.grad, 3.0 * a.grad, rtol=1e-6, atol=0)
+    with pytest.raises(RuntimeError):
+        la.backward()
+    # log probabilities keep their inputs and may go backward again
+    c = x.to(device).requires_grad_()
+    out = ta.token_log_probs(c, labels.to(device)).sum()
+    g1, = torch.autograd.grad(out, c, retain_graph=True)
+    g2, = torch.autograd.grad(out, c)
+    assert bits_equal(g1, g2)
+
+
+def test_other_stream_and_repeatability(device):
+    x, labels, g = make((4, 50, 2000), torch.bfloat16, 61)
+    lab, ref, adv = labels.to(device), torch.randn(4, 50, generator=g).to(device) - 8, torch.randn(4, generator=g).to(device)
+
+    def step(xd):
+        l1, r = ta.preference_loss(xd, lab, ref, return_rewards=True)
+        l2, lp = ta.clipped_policy_loss(xd, lab, ref, adv, ref, 0.1, return_log_probs=True)
+        return [l1.detach(), r, l2.detach(), lp, *torch.autograd.grad(l1 + l2, xd)]
+
+    xd = x.to(device).requires_grad_()
+    want = [t.clone() for t in step(xd)]
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = step(xd)
+    side.synchronize()
+    for a, b in zip(want, got):
+        assert bits_equal(a, b)
+
+
+def test_graph_capture_replays(device):
+    x, labels, g = make((2, 20, 3000), torch.bfloat16, 71)
+    lab, ref, adv = labels.to(device), torch.randn(2, 20, generator=g).to(device) - 8, torch.randn(2, generator=g).to(device)
+    static = x.to(device).requires_grad_()
+
+    def step(xd):
+        lp = ta.token_log_probs(xd, lab)
+        l1 = ta.preference_loss(xd, lab, ref)
+        l2 = ta.clipped_policy_loss(xd, lab, ref, adv, ref, 0.1)
+        return [lp.detach(), l1.detach(), l2.detach(), torch.autograd.grad(lp, xd, torch.ones_like(lp))[0],
+                torch.autograd.grad(l1, xd)[0], torch.autograd.grad(l2, xd)[0]]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(static)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step(static)
+    for trial in range(4):
+        fresh = (x.float() * (1 + 0.1 * trial)).to(torch.bfloat16).to(device)
+        with torch.no_grad():
+            static.copy_(fresh)
+        graph.replay()
+        torch.cuda.synchronize()
+        want = step(fresh.requires_grad_())
+        for a, b in zip(outs, want):
+            assert bits_equal(a, b), trial
+
+
+# ---- used together ----------------------------------------------------------------------------
+
+class _Params:
+    beta, kl_weight, clip_low, clip_high = 0.2, 0.1, 0.2, 0.25
+
+
+def test_plug_ins(device):
+    g = seeded(81)
+    n, L, V = 4, 12, 900
+    s, t = (torch.randn(n, L, V, generator=g) * 2 for _ in range(2))
+    tokens = torch.randint(0, V, (n, L), generator=g)
+    mask = torch.rand(n, L, generator=g) < 0.6
+    nxt = torch.full_like(tokens, -100)
+    nxt[:, :-1] = tokens[:, 1:].masked_fill(~mask[:, 1:], -100)
+    ref = ref64.log_probs(t.double(), nxt)[0]
+    s64 = s.double().requires_grad_()
+    want, _ = ref64.preference(s64, nxt, ref, _Params.beta)
+    want.backward()
+    sd = s.to(device).requires_grad_()
+    loss = ta.preference_loss_fn({"logits": sd}, {"logits": t.to(device)}, (tokens.to(device), mask.to(device)), None,
+                                 _Params(), 0)
+    loss.backward()
+    assert abs(loss.item() - want.item()) < 4 * L * LOGP_ABS + 1e-6
+    check_grad(sd.grad, s64.grad, torch.float32, coef=1.0)
+    old = ref64.log_probs(s.double(), nxt)[0].float() + 0.01
+    adv = torch.randn(n, generator=g)
+    s64 = s.double().requires_grad_()
+    want, _ = ref64.policy(s64, nxt, old.double(), adv.double(), ref, 0.1, 0.2, 0.25)
+    want.backward()
+    sd = s.to(device).requires_grad_()
+    loss = ta.policy_loss_fn({"logits": sd}, {"logits": t.to(device)},
+                             (tokens.to(device), mask.to(device), old.to(device), adv.to(device)), None, _Params(), 0)
+    loss.backward()
+    # ref - log p reaches several units here, and its exponential multiplies the error
+    big = (ref - ref64.log_probs(s.double(), nxt)[0]).abs().max().exp().item()
+    assert abs(loss.item() - want.item()) < (3 + big) * LOGP_ABS * 2 + 1e-6 * abs(want.item())
+    check_grad(sd.grad, s64.grad, torch.float32, coef=1.0 + 0.1 * big * 2 * LOGP_ABS * 2 ** 22)
+
+
+def test_training_steps_with_the_plug_in(device):
+    # a few optimizer steps of a linear head under the preference plug-in follow the same steps in 64 bits
+    g = seeded(91)
+    n, L, D, V = 4, 8, 16, 300
+    h = torch.randn(n, L, D, generator=g)
+    w0 = torch.randn(V, D, generator=g) * 0.3
+    tokens = torch.randint(0, V, (n, L), generator=g)
+    mask = torch.ones(n, L, dtype=torch.bool)
+    nxt = torch.full_like(tokens, -100)
+    nxt[:, :-1] = tokens[:, 1:]
+    t = h @ w0.t()
+    ref = ref64.log_probs(t.double(), nxt)[0]
+    w64, wd = w0.double(), w0.to(device)
+    for _ in range(3):
+        w64 = w64.detach().requires_grad_()
+        l64, _ = ref64.preference(h.double() @ w64.t(), nxt, ref, 0.2)
+        l64.backward()
+        wd = wd.detach().requires_grad_()
+        loss = ta.preference_loss_fn({"logits": h.to(device) @ wd.t()}, {"logits": t.to(device)},
+                                     (tokens.to(device), mask.to(device)), None, _Params(), 0)
+        loss.backward()
+        assert abs(loss.item() - l64.item()) < 1e-4
+        assert (wd.grad.cpu().double() - w64.grad).abs().max() < 1e-4 * w64.grad.abs().max() + 1e-5
+        w64, wd = w64.detach() - 0.5 * w64.grad, wd.detach() - 0.5 * wd.grad

@@ -14,6 +14,9 @@ from .losses import (Logits, SoftTarget, byol_contrastive_loss, byol_contrastive
                      moco_contrastive_loss_pieces, set_infonce_fp32_arithmetic, set_infonce_workgroup_target,
                      soft_target_tspipe_loss)
 from .model_wrapper import TSPipeModelOutput, TSPipeModelWrapper
+from .token_losses import (clipped_policy_loss, policy_loss_fn, preference_loss, preference_loss_fn,
+                           token_log_probs)
+from .top_logits import TopLogits, top_distil_loss_fn, top_logits, top_logits_distil_loss
 from .utils import generic_object_gather, generic_object_scatter, traverse_tensor_map
 
 __version__ = "0.1.0"

@@ -47,6 +47,23 @@ SIGNATURES = {
                                 c_float, c_float, c_float, c_void_p, c_void_p, c_void_p, c_int64, c_int, c_void_p]),
     "ts_kdce_pieces_fwd_bwd": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int64, c_int64,
                                        c_float, c_float, c_float, c_void_p, c_void_p, c_int, c_void_p]),
+    "ts_token_logp_fwd": (c_int, [c_void_p, c_int64, c_int64, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_int64,
+                                  c_double, c_void_p, c_void_p, c_int, c_void_p]),
+    "ts_token_logp_bwd": (c_int, [c_void_p, c_int64, c_int64, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_int64,
+                                  c_double, c_void_p, c_void_p, c_void_p, c_int, c_void_p]),
+    "ts_token_loss_workspace_bytes": (c_size_t, [c_int64, c_int64]),
+    "ts_preference_fwd_bwd": (c_int, [c_void_p, c_int64, c_int64, c_int64, c_int64, c_int64, c_void_p, c_void_p,
+                                      c_int64, c_void_p, c_int, c_double, c_int, c_double, c_int, c_double, c_void_p,
+                                      c_void_p, c_void_p, c_void_p, c_int, c_void_p]),
+    "ts_policy_fwd_bwd": (c_int, [c_void_p, c_int64, c_int64, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_int64,
+                                  c_double, c_void_p, c_void_p, c_void_p, c_int, c_double, c_double, c_double, c_int,
+                                  c_double, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p]),
+    "ts_top_logits": (c_int, [c_void_p, c_int64, c_int64, c_int64, c_int64, c_int64, c_int, c_double, c_void_p,
+                              c_void_p, c_void_p, c_int, c_void_p]),
+    "ts_top_distil_workspace_bytes": (c_size_t, [c_int64]),
+    "ts_top_distil_fwd_bwd": (c_int, [c_void_p, c_int64, c_int64, c_int64, c_int64, c_int64, c_void_p, c_int, c_void_p,
+                                      c_void_p, c_int, c_void_p, c_double, c_double, c_void_p, c_void_p, c_void_p,
+                                      c_int, c_void_p]),
     "ts_cosine_workspace_bytes": (c_size_t, [c_int64]),
     "ts_cosine_fwd_bwd": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_float, c_void_p, c_void_p,
                                   c_void_p, c_int, c_void_p]),

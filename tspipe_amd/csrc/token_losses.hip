@@ -1,0 +1,454 @@
+// Losses on the log probabilities of sampled tokens, forward and backward:
+//   token log probability   ln softmax(s / T)[label] per row, and its gradient,
+//   preference loss         paired log ratios against a reference model,
+//   clipped policy loss     probability ratios against the sampling policy,
+//                           clipped, with a KL term against a reference model.
+// All three come down to d loss / d s = c (onehot(label) - softmax(s / T)) / T
+// with one factor c per row; they differ in where c comes from: the caller, the
+// sums over both sequences of a pair, or the row itself.
+#include "vocab_rows.h"
+
+namespace ts {
+
+constexpr int kTokBlock = 256;
+
+// Which rows count, and for which token.
+struct TokenRows {
+  VocabRows r;
+  const int64_t* labels;
+  const uint8_t* mask;  // may be null (all rows)
+  int64_t ignore_index;
+};
+
+__device__ __forceinline__ bool token_live(const TokenRows& a, int64_t row, int64_t* label) {
+  const int64_t l = a.labels[row];
+  *label = l;
+  return l != a.ignore_index && l >= 0 && l < a.r.V && (!a.mask || a.mask[row] != 0);
+}
+
+// d loss / d s of one row from its maximum, its sum and the factor c / T.
+template <typename T>
+__device__ __forceinline__ void token_grad_row(const VocabRows& r, const T* row, T* grow, float m, float z, float c,
+                                               int label) {
+  const float cz = c / z, k = r.k;
+  vocab_map_walk<T, kTokBlock>(row, grow, r.V, [=](float x, int j) {
+    const float q = fast_exp2((x - m) * k);
+    return j == label ? fmaf(-cz, q, c) : -cz * q;
+  });
+}
+
+// ---- token log probabilities ------------------------------------------------
+
+// log_ratio (optional): the log probability minus ref[row] in 64 bits, for the
+// sums over whole sequences.
+template <typename T>
+__global__ __launch_bounds__(kTokBlock) void token_stat_kernel(const TokenRows a, const float* __restrict__ ref,
+                                                               float* __restrict__ logp, double* __restrict__ log_ratio,
+                                                               float2* __restrict__ stats) {
+  __shared__ VocabStat lds[kTokBlock / kWave];
+  const int64_t row = blockIdx.x;
+  int64_t label;
+  if (!token_live(a, row, &label)) {
+    if (threadIdx.x == 0) {
+      if (logp) logp[row] = 0.f;
+      if (log_ratio) log_ratio[row] = 0.0;
+      if (stats) stats[row] = make_float2(0.f, 1.f);
+    }
+    return;
+  }
+  const T* srow = vocab_row<T>(a.r, row);
+  const VocabStat s =
+      vstat_block<kTokBlock / kWave>(vocab_stat_walk<T, kTokBlock>(srow, a.r.V, a.r.k), a.r.k, lds);
+  if (threadIdx.x == 0) {
+    const double lp = vstat_log_prob(a.r, s, to_f32(srow[label]));
+    if (logp) logp[row] = (float)lp;
+    if (log_ratio) log_ratio[row] = ref ? lp - (double)ref[row] : lp;
+    if (stats) stats[row] = make_float2(s.m, s.z);
+  }
+}
+
+// The factor c of a row is coef[row] or, with per_seq, coef[row / seq_len].
+template <typename T>
+__global__ __launch_bounds__(kTokBlock) void token_grad_kernel(const TokenRows a, const float2* __restrict__ stats,
+                                                               const float* __restrict__ coef, int per_seq,
+                                                               T* __restrict__ grad) {
+  const int64_t row = blockIdx.x;
+  T* grow = grad + row * a.r.V;
+  int64_t label;
+  if (!token_live(a, row, &label)) {
+    vocab_zero_row<T, kTokBlock>(grow, a.r.V);
+    return;
+  }
+  const float c = coef[per_seq ? row / a.r.seq_len : row] * (float)a.r.inv_T;
+  const float2 st = stats[row];
+  token_grad_row<T>(a.r, vocab_row<T>(a.r, row), grow, st.x, st.y, c, (int)label);
+}
+
+// ---- preference loss ---------------------------------------------------------
+
+enum { kPrefSigmoid = 0, kPrefHinge = 1, kPrefIpo = 2 };
+
+struct PrefArgs {
+  const double* log_ratio;  // per row, the per-token reference already taken off
+  const float* ref_seq;     // per sequence, or null
+  double beta, smoothing, weight;
+  int kind, average;
+  float* rewards;       // per sequence, may be null
+  float* coef;          // per sequence
+  double* pair_loss;    // per pair
+};
+
+__device__ __forceinline__ double softplus_f64(double x) { return fmax(x, 0.0) + log1p(exp(-fabs(x))); }
+
+// One workgroup per pair: both sequences' sums, the pair's loss and the factors
+// c of its two sequences.
+__global__ __launch_bounds__(kTokBlock) void pref_join_kernel(const TokenRows a, const PrefArgs p, int64_t pairs) {
+  __shared__ double lds[kTokBlock / kWave];
+  const int64_t pair = blockIdx.x, L = a.r.seq_len;
+  double R[2], n[2];
+  for (int side = 0; side < 2; ++side) {
+    const int64_t row0 = (2 * pair + side) * L;
+    double s = 0.0, c = 0.0;
+    for (int64_t i = threadIdx.x; i < L; i += kTokBlock) {
+      s += p.log_ratio[row0 + i];
+      if (p.average) {
+        int64_t label;
+        c += token_live(a, row0 + i, &label) ? 1.0 : 0.0;
+      }
+    }
+    R[side] = block_sum_f64<kTokBlock / kWave>(s, lds);
+    n[side] = p.average ? fmax(block_sum_f64<kTokBlock / kWave>(c, lds), 1.0) : 1.0;
+    R[side] = R[side] / n[side] - (p.ref_seq ? (double)p.ref_seq[2 * pair + side] : 0.0);
+  }
+  if (threadIdx.x != 0) return;
+  const double h = R[0] - R[1], bh = p.beta * h;
+  double loss, slope;  // slope = d loss / d h
+  if (p.kind == kPrefSigmoid) {
+    loss = (1.0 - p.smoothing) * softplus_f64(-bh) + p.smoothing * softplus_f64(bh);
+    slope = p.beta * (p.smoothing - 1.0 / (1.0 + exp(bh)));
+  } else if (p.kind == kPrefHinge) {
+    loss = bh < 1.0 ? 1.0 - bh : (bh >= 1.0 ? 0.0 : bh);  // (a NaN stays one)
+    slope = bh < 1.0 ? -p.beta : 0.0;
+  } else {
+    const double e = h - 0.5 / p.beta;
+    loss = e * e;
+    slope = 2.0 * e;
+  }
+  p.pair_loss[pair] = loss;
+  const double c = slope * p.weight / (double)pairs;
+  for (int side = 0; side < 2; ++side) {
+    p.coef[2 * pair + side] = (float)((side ? -c : c) / n[side]);
+    if (p.rewards) p.rewards[2 * pair + side] = (float)(p.beta * R[side]);
+  }
+}
+
+// out = scale * sum(v) / denom; NaN when there is nothing to average.
+__global__ __launch_bounds__(1024) void sum_f64_kernel(const double* __restrict__ v, int64_t n, double scale,
+                                                       const int* __restrict__ live, float* __restrict__ out) {
+  __shared__ double lds[1024 / kWave];
+  double s = 0.0;
+  for (int64_t i = threadIdx.x; i < n; i += 1024) s += v[i];
+  s = block_sum_f64<1024 / kWave>(s, lds);
+  if (threadIdx.x == 0) *out = (live ? *live != 0 : n != 0) ? (float)(s * scale) : __builtin_nanf("");
+}
+
+// ---- clipped policy loss ------------------------------------------------------
+
+struct PolicyArgs {
+  const float* old_logp;
+  const float* ref_logp;  // may be null when kl_weight is 0
+  const float* adv;
+  int adv_per_seq;
+  double kl_weight, clip_lo, clip_hi;
+  const float* seq_weight;  // weight of a sequence's tokens
+  float* logp;              // per row, may be null
+  double* row_loss;
+  void* grad;  // may be null
+};
+
+// Weight of every sequence's tokens: weight / (live rows), or with per_seq
+// weight / (sequences with a live row) / (live rows of this one).
+// counts[0] = live rows.
+__global__ __launch_bounds__(1024) void policy_weight_kernel(const TokenRows a, int64_t n_seq, int per_seq, float weight,
+                                                             float* __restrict__ seq_weight, int* __restrict__ counts) {
+  __shared__ int total, full;
+  const int lane = threadIdx.x % kWave, w = threadIdx.x / kWave;
+  if (threadIdx.x == 0) total = full = 0;
+  __syncthreads();
+  const int64_t L = a.r.seq_len;
+  for (int64_t q = w; q < n_seq; q += 1024 / kWave) {
+    int c = 0;
+    for (int64_t i = lane; i < L; i += kWave) {
+      int64_t label;
+      c += token_live(a, q * L + i, &label);
+    }
+#pragma unroll
+    for (int off = kWave / 2; off > 0; off >>= 1) c += __shfl_xor(c, off, kWave);
+    if (lane == 0) {
+      seq_weight[q] = (float)c;  // exact: fewer than 2^24 rows
+      atomicAdd(&total, c);
+      if (c) atomicAdd(&full, 1);
+    }
+  }
+  __syncthreads();
+  for (int64_t q = w; q < n_seq; q += 1024 / kWave) {
+    if (lane == 0) {
+      const float c = seq_weight[q];
+      seq_weight[q] = per_seq ? weight / ((float)full * fmaxf(c, 1.f)) : weight / (float)total;
+    }
+  }
+  if (threadIdx.x == 0) counts[0] = total;
+}
+
+// loss term and d loss / d logp of one token
+__device__ __forceinline__ void policy_term(const PolicyArgs& p, double lp, float old_lp, float ref_lp, float A,
+                                            double* term, double* slope) {
+  const double r = exp(lp - (double)old_lp);
+  const double held = r < p.clip_lo ? p.clip_lo : (r > p.clip_hi ? p.clip_hi : r);
+  const double f = r * (double)A, h = held * (double)A;
+  // min(f, h): the gradient flows where the ratio itself decides
+  *term = f <= h ? -f : (h < f ? -h : f + h);
+  *slope = f <= h ? -f : 0.0;
+  if (p.kl_weight != 0.0) {
+    const double d = (double)ref_lp - lp;
+    const double em1 = expm1(d);
+    *term += p.kl_weight * (em1 - d);
+    *slope -= p.kl_weight * em1;
+  }
+}
+
+template <typename T>
+__global__ __launch_bounds__(kTokBlock) void policy_rows_kernel(const TokenRows a, const PolicyArgs p) {
+  __shared__ VocabStat lds[kTokBlock / kWave];
+  const int64_t row = blockIdx.x, seq = row / a.r.seq_len;
+  T* grow = p.grad ? reinterpret_cast<T*>(p.grad) + row * a.r.V : nullptr;
+  int64_t label;
+  if (!token_live(a, row, &label)) {
+    if (threadIdx.x == 0) {
+      if (p.logp) p.logp[row] = 0.f;
+      p.row_loss[row] = 0.0;
+    }
+    if (grow) vocab_zero_row<T, kTokBlock>(grow, a.r.V);
+    return;
+  }
+  const T* srow = vocab_row<T>(a.r, row);
+  const VocabStat s =
+      vstat_block<kTokBlock / kWave>(vocab_stat_walk<T, kTokBlock>(srow, a.r.V, a.r.k), a.r.k, lds);
+  const double lp = vstat_log_prob(a.r, s, to_f32(srow[label]));
+  double term, slope;
+  policy_term(p, lp, p.old_logp[row], p.ref_logp ? p.ref_logp[row] : 0.f, p.adv[p.adv_per_seq ? seq : row], &term,
+              &slope);
+  const double w = (double)p.seq_weight[seq];
+  if (threadIdx.x == 0) {
+    if (p.logp) p.logp[row] = (float)lp;
+    p.row_loss[row] = w * term;
+  }
+  if (grow) token_grad_row<T>(a.r, srow, grow, s.m, s.z, (float)(w * slope * a.r.inv_T), (int)label);
+}
+
+// ---- host side ------------------------------------------------------------------
+
+inline size_t pad16(size_t b) { return (b + 15) / 16 * 16; }
+
+struct TokenWs {
+  double* row;     // n_rows: log ratios or loss terms
+  float2* stats;   // n_rows
+  double* pair;    // n_seq / 2
+  float* seq;      // n_seq: factors or weights
+  int* counts;     // 4
+};
+
+inline size_t token_ws_bytes(int64_t n_rows, int64_t n_seq) {
+  return 16 + pad16((size_t)n_rows * 8) * 2 + pad16((size_t)(n_seq / 2) * 8) + pad16((size_t)n_seq * 4);
+}
+
+inline TokenWs token_carve(void* ws, int64_t n_rows, int64_t n_seq) {
+  char* b = reinterpret_cast<char*>(ws);
+  TokenWs w;
+  w.counts = reinterpret_cast<int*>(b);
+  b += 16;
+  w.row = reinterpret_cast<double*>(b);
+  b += pad16((size_t)n_rows * 8);
+  w.stats = reinterpret_cast<float2*>(b);
+  b += pad16((size_t)n_rows * 8);
+  w.pair = reinterpret_cast<double*>(b);
+  b += pad16((size_t)(n_seq / 2) * 8);
+  w.seq = reinterpret_cast<float*>(b);
+  return w;
+}
+
+template <typename T>
+int launch_token_stat(const TokenRows& a, const float* ref, float* logp, double* log_ratio, float2* stats,
+                      hipStream_t st) {
+  hipLaunchKernelGGL((token_stat_kernel<T>), dim3((unsigned)a.r.n_rows), dim3(kTokBlock), 0, st, a, ref, logp,
+                     log_ratio, stats);
+  return check_launch();
+}
+
+template <typename T>
+int launch_token_grad(const TokenRows& a, const float2* stats, const float* coef, int per_seq, void* grad,
+                      hipStream_t st) {
+  hipLaunchKernelGGL((token_grad_kernel<T>), dim3((unsigned)a.r.n_rows), dim3(kTokBlock), 0, st, a, stats, coef, per_seq,
+                     reinterpret_cast<T*>(grad));
+  return check_launch();
+}
+
+template <typename T>
+int launch_preference(const TokenRows& a, const float* ref_tok, PrefArgs p, const TokenWs& w, int64_t n_seq,
+                      float* loss_out, void* grad, hipStream_t st) {
+  const int64_t pairs = n_seq / 2;
+  int rc = TS_OK;
+  if (a.r.n_rows > 0) {
+    rc = launch_token_stat<T>(a, ref_tok, nullptr, w.row, w.stats, st);
+    if (rc) return rc;
+  }
+  if (pairs > 0) {
+    hipLaunchKernelGGL(pref_join_kernel, dim3((unsigned)pairs), dim3(kTokBlock), 0, st, a, p, pairs);
+    rc = check_launch();
+    if (rc) return rc;
+  }
+  hipLaunchKernelGGL(sum_f64_kernel, dim3(1), dim3(1024), 0, st, w.pair, pairs, pairs ? p.weight / (double)pairs : 0.0,
+                     (const int*)nullptr, loss_out);
+  rc = check_launch();
+  if (rc || !grad || a.r.n_rows == 0) return rc;
+  return launch_token_grad<T>(a, w.stats, w.seq, 1, grad, st);
+}
+
+template <typename T>
+int launch_policy(const TokenRows& a, const PolicyArgs& p, const TokenWs& w, int64_t n_seq, int per_seq, float weight,
+                  float* loss_out, hipStream_t st) {
+  hipLaunchKernelGGL(policy_weight_kernel, dim3(1), dim3(1024), 0, st, a, a.r.seq_len ? n_seq : 0, per_seq, weight,
+                     w.seq, w.counts);
+  int rc = check_launch();
+  if (rc) return rc;
+  if (a.r.n_rows > 0) {
+    hipLaunchKernelGGL((policy_rows_kernel<T>), dim3((unsigned)a.r.n_rows), dim3(kTokBlock), 0, st, a, p);
+    rc = check_launch();
+    if (rc) return rc;
+  }
+  hipLaunchKernelGGL(sum_f64_kernel, dim3(1), dim3(1024), 0, st, w.row, a.r.n_rows, 1.0, (const int*)w.counts, loss_out);
+  return check_launch();
+}
+
+// Checks shared by the entry points; `grad` and `f32s` may be null.
+inline int token_status(const void* s, int64_t n_seq, int64_t seq_len, int64_t V, int64_t ld_seq, int64_t ld_tok,
+                        const int64_t* labels, double temperature, const void* grad, int dtype) {
+  const int rc = vocab_rows_status(s, n_seq, seq_len, V, ld_seq, ld_tok, temperature, dtype);
+  if (rc) return rc;
+  if (n_seq * seq_len > 0 && !labels) return TS_ERR_ARG;
+  if ((uintptr_t)labels & 7u) return TS_ERR_ALIGN;
+  if ((uintptr_t)grad & (dtype == TS_F32 ? 3u : 1u)) return TS_ERR_ALIGN;
+  return TS_OK;
+}
+
+inline TokenRows token_rows(const void* s, int64_t n_seq, int64_t seq_len, int64_t V, int64_t ld_seq, int64_t ld_tok,
+                            const int64_t* labels, const uint8_t* mask, int64_t ignore_index, double temperature) {
+  TokenRows a;
+  a.r = vocab_rows(s, n_seq * seq_len, seq_len, V, ld_seq, ld_tok, temperature);
+  a.labels = labels;
+  a.mask = mask;
+  a.ignore_index = ignore_index;
+  return a;
+}
+
+}  // namespace ts
+
+extern "C" {
+
+int ts_token_logp_fwd(const void* s, int64_t n_seq, int64_t seq_len, int64_t V, int64_t ld_seq, int64_t ld_tok,
+                      const int64_t* labels, const uint8_t* row_mask, int64_t ignore_index, double temperature,
+                      float* logp, float* stats, int dtype, ts_stream_t stream) {
+  const int rc = ts::token_status(s, n_seq, seq_len, V, ld_seq, ld_tok, labels, temperature, nullptr, dtype);
+  if (rc) return rc;
+  if (n_seq * seq_len == 0) return TS_OK;
+  if (!logp) return TS_ERR_ARG;
+  if (((uintptr_t)logp & 3u) || ((uintptr_t)stats & 7u)) return TS_ERR_ALIGN;
+  const ts::TokenRows a =
+      ts::token_rows(s, n_seq, seq_len, V, ld_seq, ld_tok, labels, row_mask, ignore_index, temperature);
+  hipStream_t st = (hipStream_t)stream;
+  TS_BY_DTYPE(dtype, (ts::launch_token_stat<T>(a, nullptr, logp, nullptr, (float2*)stats, st)))
+}
+
+int ts_token_logp_bwd(const void* s, int64_t n_seq, int64_t seq_len, int64_t V, int64_t ld_seq, int64_t ld_tok,
+                      const int64_t* labels, const uint8_t* row_mask, int64_t ignore_index, double temperature,
+                      const float* stats, const float* grad_logp, void* grad, int dtype, ts_stream_t stream) {
+  const int rc = ts::token_status(s, n_seq, seq_len, V, ld_seq, ld_tok, labels, temperature, grad, dtype);
+  if (rc) return rc;
+  if (n_seq * seq_len == 0) return TS_OK;
+  if (!stats || !grad_logp || !grad) return TS_ERR_ARG;
+  if (((uintptr_t)grad_logp & 3u) || ((uintptr_t)stats & 7u)) return TS_ERR_ALIGN;
+  const ts::TokenRows a =
+      ts::token_rows(s, n_seq, seq_len, V, ld_seq, ld_tok, labels, row_mask, ignore_index, temperature);
+  hipStream_t st = (hipStream_t)stream;
+  TS_BY_DTYPE(dtype, (ts::launch_token_grad<T>(a, (const float2*)stats, grad_logp, 0, grad, st)))
+}
+
+size_t ts_token_loss_workspace_bytes(int64_t n_seq, int64_t seq_len) {
+  if (n_seq < 0 || seq_len < 0) return 0;
+  return ts::token_ws_bytes(n_seq * seq_len, n_seq);
+}
+
+int ts_preference_fwd_bwd(const void* s, int64_t n_seq, int64_t seq_len, int64_t V, int64_t ld_seq, int64_t ld_tok,
+                          const int64_t* labels, const uint8_t* row_mask, int64_t ignore_index, const float* ref_logp,
+                          int ref_per_token, double beta, int kind, double smoothing, int average, double weight,
+                          void* workspace, float* loss_out, float* rewards, void* grad, int dtype,
+                          ts_stream_t stream) {
+  const int rc = ts::token_status(s, n_seq, seq_len, V, ld_seq, ld_tok, labels, 1.0, grad, dtype);
+  if (rc) return rc;
+  if (n_seq % 2 || !workspace || !loss_out) return TS_ERR_ARG;
+  if (!(beta > 0.0) || !(smoothing >= 0.0 && smoothing <= 1.0)) return TS_ERR_ARG;
+  if (kind != ts::kPrefSigmoid && kind != ts::kPrefHinge && kind != ts::kPrefIpo) return TS_ERR_ARG;
+  if (smoothing != 0.0 && kind != ts::kPrefSigmoid) return TS_ERR_ARG;
+  if (n_seq * (ref_per_token ? seq_len : 1) > 0 && !ref_logp) return TS_ERR_ARG;
+  if (((uintptr_t)workspace & 15u) || (((uintptr_t)ref_logp | (uintptr_t)loss_out | (uintptr_t)rewards) & 3u))
+    return TS_ERR_ALIGN;
+  const ts::TokenRows a = ts::token_rows(s, n_seq, seq_len, V, ld_seq, ld_tok, labels, row_mask, ignore_index, 1.0);
+  const ts::TokenWs w = ts::token_carve(workspace, a.r.n_rows, n_seq);
+  ts::PrefArgs p;
+  p.log_ratio = w.row;
+  p.ref_seq = ref_per_token ? nullptr : ref_logp;
+  p.beta = beta;
+  p.smoothing = smoothing;
+  p.weight = weight;
+  p.kind = kind;
+  p.average = average;
+  p.rewards = rewards;
+  p.coef = w.seq;
+  p.pair_loss = w.pair;
+  const float* ref_tok = ref_per_token ? ref_logp : nullptr;
+  hipStream_t st = (hipStream_t)stream;
+  TS_BY_DTYPE(dtype, (ts::launch_preference<T>(a, ref_tok, p, w, n_seq, loss_out, grad, st)))
+}
+
+int ts_policy_fwd_bwd(const void* s, int64_t n_seq, int64_t seq_len, int64_t V, int64_t ld_seq, int64_t ld_tok,
+                      const int64_t* labels, const uint8_t* row_mask, int64_t ignore_index, double temperature,
+                      const float* old_logp, const float* ref_logp, const float* advantages, int adv_per_seq,
+                      double kl_weight, double clip_lo, double clip_hi, int per_seq, double weight, void* workspace,
+                      float* loss_out, float* logp, void* grad, int dtype, ts_stream_t stream) {
+  const int rc = ts::token_status(s, n_seq, seq_len, V, ld_seq, ld_tok, labels, temperature, grad, dtype);
+  if (rc) return rc;
+  if (!workspace || !loss_out || !(clip_lo <= clip_hi)) return TS_ERR_ARG;
+  if (n_seq * seq_len > 0 && (!old_logp || !advantages || (!ref_logp && kl_weight != 0.0))) return TS_ERR_ARG;
+  if (((uintptr_t)workspace & 15u) || (((uintptr_t)old_logp | (uintptr_t)ref_logp | (uintptr_t)advantages |
+                                        (uintptr_t)loss_out | (uintptr_t)logp) & 3u))
+    return TS_ERR_ALIGN;
+  const ts::TokenRows a =
+      ts::token_rows(s, n_seq, seq_len, V, ld_seq, ld_tok, labels, row_mask, ignore_index, temperature);
+  const ts::TokenWs w = ts::token_carve(workspace, a.r.n_rows, n_seq);
+  ts::PolicyArgs p;
+  p.old_logp = old_logp;
+  p.ref_logp = ref_logp;
+  p.adv = advantages;
+  p.adv_per_seq = adv_per_seq;
+  p.kl_weight = kl_weight;
+  p.clip_lo = clip_lo;
+  p.clip_hi = clip_hi;
+  p.seq_weight = w.seq;
+  p.logp = logp;
+  p.row_loss = w.row;
+  p.grad = grad;
+  hipStream_t st = (hipStream_t)stream;
+  TS_BY_DTYPE(dtype, (ts::launch_policy<T>(a, p, w, n_seq, per_seq, (float)weight, loss_out, st)))
+}
+
+}  // extern "C"
