@@ -18,18 +18,29 @@ __global__ __launch_bounds__(1024) void sum_scale_kernel(const float* __restrict
   }
 }
 
-// grad[r, :] *= *g, skipped entirely when *g == 1.
+// grad[r, :] *= *g, skipped entirely when *g == 1.  The grid is bounded and
+// strides over the row, because the usual call does nothing: a workgroup per
+// 2048 elements took 62 us to start and end them all over 8192 x 65536 elements.
+constexpr int kScaleMaxGrid = 2048;
+
 template <typename T>
 __global__ __launch_bounds__(256) void scale_rows_kernel(T* __restrict__ grad, int64_t V, int64_t ld,
                                                          const float* __restrict__ g_dev) {
+  constexpr int VEC = Vec16<T>::N;
   const float g = *g_dev;
   if (g == 1.0f) return;
   T* row = grad + (int64_t)blockIdx.y * ld;
-  const int64_t i0 = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8;
+  const int64_t first = (int64_t)blockIdx.x * 256 + threadIdx.x, step = (int64_t)gridDim.x * 256;
+  int64_t head = (int64_t)(((16u - (uint32_t)((uintptr_t)row & 15u)) & 15u) / sizeof(T));
+  if (head > V) head = V;
+  const int64_t nvec = (V - head) / VEC, tail0 = head + nvec * VEC;
+  if (first < head) row[first] = from_f32<T>(to_f32(row[first]) * g);
+  if (tail0 + first < V) row[tail0 + first] = from_f32<T>(to_f32(row[tail0 + first]) * g);
+  for (int64_t v = first; v < nvec; v += step) {
+    Vec16<T> x = load16(row + head + v * VEC);
 #pragma unroll
-  for (int k = 0; k < 8; ++k) {
-    const int64_t i = i0 + k;
-    if (i < V) row[i] = from_f32<T>(to_f32(row[i]) * g);
+    for (int i = 0; i < VEC; ++i) x.v[i] = from_f32<T>(to_f32(x.v[i]) * g);
+    store16(row + head + v * VEC, x);
   }
 }
 
@@ -728,8 +739,7 @@ int ts_scale_rows(void* grad, int64_t n_rows, int64_t V, int64_t ld_g, const flo
   }
   if (n_rows > 65535) return TS_ERR_RANGE;
   const int64_t bx = (V + 2047) / 2048;
-  if (bx > 0x7fffffffLL) return TS_ERR_RANGE;
-  dim3 grid((unsigned)bx, (unsigned)n_rows);
+  dim3 grid((unsigned)(bx < ts::kScaleMaxGrid ? bx : ts::kScaleMaxGrid), (unsigned)n_rows);
   hipStream_t st = (hipStream_t)stream;
   switch (dtype) {
     case TS_F32:
