@@ -26,27 +26,39 @@ __device__ __forceinline__ bool token_live(const TokenRows& a, int64_t row, int6
   return l != a.ignore_index && l >= 0 && l < a.r.V && (!a.mask || a.mask[row] != 0);
 }
 
-// d loss / d s of one row from its maximum, its sum and the factor c / T.
-template <typename T>
-__device__ __forceinline__ void token_grad_row(const VocabRows& r, const T* row, T* grow, float m, float z, float c,
-                                               int label) {
-  const float cz = c / z, k = r.k;
-  vocab_map_walk<T, kTokBlock>(row, grow, r.V, [=](float x, int j) {
-    const float q = fast_exp2((x - m) * k);
-    return j == label ? fmaf(-cz, q, c) : -cz * q;
-  });
-}
-
 // ---- token log probabilities ------------------------------------------------
+// stats[row] = (c, z): the row's sum z of 2^(x k + c), or (m, -z) with z the sum
+// of 2^((x - m) k) where that sum over- or underflows.
+
+// d loss / d x from a row's stats and its factor c / T.
+struct TokenGrad {
+  float k, off, cz, c;
+  bool by_max;
+  __device__ __forceinline__ TokenGrad(float k_, float2 st, float c_) {
+    k = k_;
+    off = st.x;
+    by_max = !(st.y > 0.f);
+    cz = c_ / fabsf(st.y);
+    c = c_;
+  }
+  __device__ __forceinline__ float prob_c(float x) const {  // c * probability
+    return cz * fast_exp2(by_max ? (x - off) * k : fmaf(x, k, off));
+  }
+  __device__ __forceinline__ float other(float x) const { return -prob_c(x); }
+  __device__ __forceinline__ float label(float x) const { return c - prob_c(x); }
+};
 
 // log_ratio (optional): the log probability minus ref[row] in 64 bits, for the
-// sums over whole sequences.
-template <typename T>
-__global__ __launch_bounds__(kTokBlock) void token_stat_kernel(const TokenRows a, const float* __restrict__ ref,
-                                                               float* __restrict__ logp, double* __restrict__ log_ratio,
-                                                               float2* __restrict__ stats) {
-  __shared__ VocabStat lds[kTokBlock / kWave];
-  const int64_t row = blockIdx.x;
+// sums over whole sequences.  Rows longer than NT * KREG vectors are walked in
+// pieces of that size.
+template <typename T, int NT, int KREG>
+__global__ __launch_bounds__(NT) void token_stat_kernel(const TokenRows a, int64_t row0, const float* __restrict__ ref,
+                                                        float* __restrict__ logp, double* __restrict__ log_ratio,
+                                                        float2* __restrict__ stats) {
+  constexpr int VEC = Vec16<T>::N;
+  __shared__ RowSum lds[NT / kWave];
+  __shared__ VocabStat lds_v[NT / kWave];
+  const int64_t row = row0 + blockIdx.x;
   int64_t label;
   if (!token_live(a, row, &label)) {
     if (threadIdx.x == 0) {
@@ -57,31 +69,128 @@ __global__ __launch_bounds__(kTokBlock) void token_stat_kernel(const TokenRows a
     return;
   }
   const T* srow = vocab_row<T>(a.r, row);
-  const VocabStat s =
-      vstat_block<kTokBlock / kWave>(vocab_stat_walk<T, kTokBlock>(srow, a.r.V, a.r.k), a.r.k, lds);
-  if (threadIdx.x == 0) {
-    const double lp = vstat_log_prob(a.r, s, to_f32(srow[label]));
-    if (logp) logp[row] = (float)lp;
-    if (log_ratio) log_ratio[row] = ref ? lp - (double)ref[row] : lp;
-    if (stats) stats[row] = make_float2(s.m, s.z);
+  const int64_t V = a.r.V;
+  const float k = a.r.k;
+  const VocabGeom g = vocab_geom(srow, V);
+  RowRegs<T, NT, KREG> r;
+  regs_load(r, srow, V, g);
+  const float c = regs_anchor(r, g, k);
+  float z = 0.f, s_a = 0.f;
+  auto add = [&](float x) {
+    const float d = fmaf(x, k, c), e = fast_exp2(d);
+    z += e;
+    s_a = fmaf(e, fmaxf(d, -1e30f), s_a);
+  };
+  if (threadIdx.x < kWave) {
+    add(r.h);
+    add(r.t);
   }
+  regs_each(r, g, add);
+  for (int64_t v0 = NT * KREG; v0 < g.nvec; v0 += NT * KREG) {
+#pragma unroll
+    for (int j = 0; j < KREG; ++j) {
+      const int64_t v = v0 + threadIdx.x + j * NT;
+      if (v < g.nvec) r.v[j] = load16_stream(srow + g.head + v * VEC);
+    }
+#pragma unroll
+    for (int j = 0; j < KREG; ++j) {
+      if (v0 + threadIdx.x + j * NT < g.nvec) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) add(to_f32(r.v[j].v[i]));
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+  const RowSum s = rowsum_block<NT / kWave, true>(c, z, s_a, lds);
+  Float2x lp;
+  float2 st;
+  if (s.ok) {
+    if (threadIdx.x != 0) return;
+    lp = rowsum_log_prob<true>(a.r, s, to_f32(srow[label]));
+    st = make_float2(s.c, s.z);
+  } else {
+    const VocabStat sv = vstat_block<NT / kWave>(vocab_stat_walk<T, NT>(srow, V, k), k, lds_v);
+    if (threadIdx.x != 0) return;
+    const double l = vstat_log_prob(a.r, sv, to_f32(srow[label]));
+    lp = Float2x{(float)l, isfinite(l) ? (float)(l - (double)(float)l) : 0.f};
+    st = make_float2(sv.m, -sv.z);
+  }
+  if (logp) logp[row] = lp.hi;
+  if (log_ratio) log_ratio[row] = ((double)lp.hi - (ref ? (double)ref[row] : 0.0)) + (double)lp.lo;
+  if (stats) stats[row] = st;
 }
 
-// The factor c of a row is coef[row] or, with per_seq, coef[row / seq_len].
+// One workgroup per part of a row: every element depends on its row's two
+// numbers only, so this is a copy with an exponential.  The factor c of a row
+// is coef[row] or, with per_seq, coef[row / seq_len].
+constexpr int kGradVecs = 8;                           // 16-byte vectors per thread, all loads in flight at once
+constexpr int kGradPart = kTokBlock * kGradVecs;       // vectors per workgroup
+
 template <typename T>
-__global__ __launch_bounds__(kTokBlock) void token_grad_kernel(const TokenRows a, const float2* __restrict__ stats,
+__global__ __launch_bounds__(kTokBlock) void token_grad_kernel(const TokenRows a, int64_t row0, int parts,
+                                                               const float2* __restrict__ stats,
                                                                const float* __restrict__ coef, int per_seq,
                                                                T* __restrict__ grad) {
-  const int64_t row = blockIdx.x;
-  T* grow = grad + row * a.r.V;
+  constexpr int VEC = Vec16<T>::N;
+  const int64_t local = blockIdx.x / (unsigned)parts, row = row0 + local;
+  const int part = (int)(blockIdx.x - (unsigned)local * (unsigned)parts);
+  const int64_t V = a.r.V, v0 = (int64_t)part * kGradPart;
+  const int tid = threadIdx.x;
+  T* grow = grad + row * V;
   int64_t label;
   if (!token_live(a, row, &label)) {
-    vocab_zero_row<T, kTokBlock>(grow, a.r.V);
+    const VocabGeom g = vocab_geom(grow, V);
+    const T zero = from_f32<T>(0.f);
+    if (part == 0 && tid < g.head) grow[tid] = zero;
+    if (part == parts - 1 && g.tail0 + tid < V) grow[g.tail0 + tid] = zero;
+    Vec16<T> z;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) z.v[i] = zero;
+#pragma unroll
+    for (int j = 0; j < kGradVecs; ++j) {
+      const int64_t v = v0 + tid + j * kTokBlock;
+      if (v < g.nvec) store16(grow + g.head + v * VEC, z);
+    }
     return;
   }
-  const float c = coef[per_seq ? row / a.r.seq_len : row] * (float)a.r.inv_T;
-  const float2 st = stats[row];
-  token_grad_row<T>(a.r, vocab_row<T>(a.r, row), grow, st.x, st.y, c, (int)label);
+  const T* srow = vocab_row<T>(a.r, row);
+  const VocabGeom g = vocab_geom(srow, V);
+  Vec16<T> x[kGradVecs];
+#pragma unroll
+  for (int j = 0; j < kGradVecs; ++j) {
+    const int64_t v = v0 + tid + j * kTokBlock;
+    if (v < g.nvec) x[j] = load16_stream(srow + g.head + v * VEC);
+  }
+  const TokenGrad f(a.r.k, stats[row], coef[per_seq ? row / a.r.seq_len : row] * (float)a.r.inv_T);
+  auto one = [&](float xv, int64_t j) { return from_f32<T>(j == label ? f.label(xv) : f.other(xv)); };
+  if (part == 0 && tid < g.head) grow[tid] = one(to_f32(srow[tid]), tid);
+  if (part == parts - 1 && g.tail0 + tid < V) grow[g.tail0 + tid] = one(to_f32(srow[g.tail0 + tid]), g.tail0 + tid);
+  const bool gvec = (((uintptr_t)grow ^ (uintptr_t)srow) & 15u) == 0;
+  const int64_t lv = label >= g.head ? (label - g.head) / VEC : -1;
+  const int li = (int)(label - g.head - lv * VEC);
+#pragma unroll
+  for (int j = 0; j < kGradVecs; ++j) {
+    const int64_t v = v0 + tid + j * kTokBlock;
+    if (v < g.nvec) {
+      forget(x[j]);
+      Vec16<T> o;
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) o.v[i] = from_f32<T>(f.other(to_f32(x[j].v[i])));
+      if (v == lv) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i)
+          if (i == li) o.v[i] = from_f32<T>(f.label(to_f32(x[j].v[i])));
+      }
+      T* p = grow + g.head + v * VEC;
+      if (gvec) {
+        store16_stream(p, o);
+      } else {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) p[i] = o.v[i];
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  }
 }
 
 // ---- preference loss ---------------------------------------------------------
@@ -159,7 +268,7 @@ struct PolicyArgs {
   const float* ref_logp;  // may be null when kl_weight is 0
   const float* adv;
   int adv_per_seq;
-  double kl_weight, clip_lo, clip_hi;
+  float kl_weight, clip_lo, clip_hi;
   const float* seq_weight;  // weight of a sequence's tokens
   float* logp;              // per row, may be null
   double* row_loss;
@@ -201,49 +310,90 @@ __global__ __launch_bounds__(1024) void policy_weight_kernel(const TokenRows a, 
 }
 
 // loss term and d loss / d logp of one token
-__device__ __forceinline__ void policy_term(const PolicyArgs& p, double lp, float old_lp, float ref_lp, float A,
-                                            double* term, double* slope) {
-  const double r = exp(lp - (double)old_lp);
-  const double held = r < p.clip_lo ? p.clip_lo : (r > p.clip_hi ? p.clip_hi : r);
-  const double f = r * (double)A, h = held * (double)A;
+__device__ __forceinline__ void policy_term(const PolicyArgs& p, Float2x lp, float old_lp, float ref_lp, float A,
+                                            float* term, float* slope) {
+  const float r = expf((lp.hi - old_lp) + lp.lo);
+  const float held = r < p.clip_lo ? p.clip_lo : (r > p.clip_hi ? p.clip_hi : r);
+  const float f = r * A, h = held * A;
   // min(f, h): the gradient flows where the ratio itself decides
   *term = f <= h ? -f : (h < f ? -h : f + h);
-  *slope = f <= h ? -f : 0.0;
-  if (p.kl_weight != 0.0) {
-    const double d = (double)ref_lp - lp;
-    const double em1 = expm1(d);
-    *term += p.kl_weight * (em1 - d);
-    *slope -= p.kl_weight * em1;
+  *slope = f <= h ? -f : 0.f;
+  if (p.kl_weight != 0.f) {
+    const float d = (ref_lp - lp.hi) - lp.lo;
+    const float em1 = expm1f(d);
+    // e^d - 1 - d: its leading terms where the difference would cancel
+    const float kl = fabsf(d) < 0.03f ? d * d * (0.5f + d * (1.f / 6.f + d * (1.f / 24.f + d * (1.f / 120.f)))) : em1 - d;
+    *term = fmaf(p.kl_weight, kl, *term);
+    *slope = fmaf(-p.kl_weight, em1, *slope);
   }
 }
 
-template <typename T>
-__global__ __launch_bounds__(kTokBlock) void policy_rows_kernel(const TokenRows a, const PolicyArgs p) {
-  __shared__ VocabStat lds[kTokBlock / kWave];
-  const int64_t row = blockIdx.x, seq = row / a.r.seq_len;
-  T* grow = p.grad ? reinterpret_cast<T*>(p.grad) + row * a.r.V : nullptr;
+// What one thread of a row's workgroup does with the row's log probability:
+// outputs, and the factor of its gradient.
+__device__ __forceinline__ float policy_finish(const TokenRows& a, const PolicyArgs& p, int64_t row, Float2x lp) {
+  const int64_t seq = row / a.r.seq_len;
+  float term, slope;
+  policy_term(p, lp, p.old_logp[row], p.ref_logp ? p.ref_logp[row] : 0.f, p.adv[p.adv_per_seq ? seq : row], &term,
+              &slope);
+  const float w = p.seq_weight[seq];
+  if (p.logp) p.logp[row] = lp.hi;
+  p.row_loss[row] = (double)w * (double)term;
+  return w * slope * (float)a.r.inv_T;
+}
+
+// Rows whose sum needs the true maximum, and rows too long for registers: two
+// walks over the row.
+template <typename T, int NT>
+__device__ __forceinline__ void policy_row_walked(const TokenRows& a, const PolicyArgs& p, int64_t row, const T* srow,
+                                                  T* grow, int64_t label) {
+  __shared__ VocabStat lds[NT / kWave];
+  __shared__ float coef;
+  const float k = a.r.k;
+  const VocabStat s = vstat_block<NT / kWave>(vocab_stat_walk<T, NT>(srow, a.r.V, k), k, lds);
+  if (threadIdx.x == 0) {
+    const double l = vstat_log_prob(a.r, s, to_f32(srow[label]));
+    coef = policy_finish(a, p, row, Float2x{(float)l, isfinite(l) ? (float)(l - (double)(float)l) : 0.f});
+  }
+  if (!grow) return;
+  __syncthreads();
+  const TokenGrad f(k, make_float2(s.m, -s.z), coef);
+  vocab_map_walk<T, NT>(srow, grow, a.r.V, [&](float x, int j) { return j == (int)label ? f.label(x) : f.other(x); });
+}
+
+// A row's factor c follows from the row itself, so the row stays in registers
+// between its sum and its gradient and is read once.  KREG = 0: the row is
+// walked twice.
+template <typename T, int NT, int KREG>
+__global__ __launch_bounds__(NT) void policy_rows_kernel(const TokenRows a, const PolicyArgs p) {
+  __shared__ RowSum lds[NT / kWave];
+  __shared__ float coef;
+  const int64_t row = blockIdx.x, V = a.r.V;
+  T* grow = p.grad ? reinterpret_cast<T*>(p.grad) + row * V : nullptr;
   int64_t label;
   if (!token_live(a, row, &label)) {
     if (threadIdx.x == 0) {
       if (p.logp) p.logp[row] = 0.f;
       p.row_loss[row] = 0.0;
     }
-    if (grow) vocab_zero_row<T, kTokBlock>(grow, a.r.V);
+    if (grow) vocab_zero_row<T, NT>(grow, V);
     return;
   }
   const T* srow = vocab_row<T>(a.r, row);
-  const VocabStat s =
-      vstat_block<kTokBlock / kWave>(vocab_stat_walk<T, kTokBlock>(srow, a.r.V, a.r.k), a.r.k, lds);
-  const double lp = vstat_log_prob(a.r, s, to_f32(srow[label]));
-  double term, slope;
-  policy_term(p, lp, p.old_logp[row], p.ref_logp ? p.ref_logp[row] : 0.f, p.adv[p.adv_per_seq ? seq : row], &term,
-              &slope);
-  const double w = (double)p.seq_weight[seq];
-  if (threadIdx.x == 0) {
-    if (p.logp) p.logp[row] = (float)lp;
-    p.row_loss[row] = w * term;
+  if constexpr (KREG > 0) {
+    const VocabGeom g = vocab_geom(srow, V);
+    RowRegs<T, NT, KREG> r;
+    regs_load(r, srow, V, g);
+    const RowSum s = regs_sum<T, NT, KREG, false>(r, g, a.r.k, lds);
+    if (s.ok) {
+      if (threadIdx.x == 0) coef = policy_finish(a, p, row, rowsum_log_prob<false>(a.r, s, to_f32(srow[label])));
+      if (!grow) return;
+      __syncthreads();
+      const TokenGrad f(a.r.k, make_float2(s.c, s.z), coef);
+      regs_map(r, g, srow, grow, V, (int)label, [&](float x) { return f.other(x); }, [&](float x) { return f.label(x); });
+      return;
+    }
   }
-  if (grow) token_grad_row<T>(a.r, srow, grow, s.m, s.z, (float)(w * slope * a.r.inv_T), (int)label);
+  policy_row_walked<T, NT>(a, p, row, srow, grow, label);
 }
 
 // ---- host side ------------------------------------------------------------------
@@ -278,19 +428,39 @@ inline TokenWs token_carve(void* ws, int64_t n_rows, int64_t n_seq) {
 }
 
 template <typename T>
-int launch_token_stat(const TokenRows& a, const float* ref, float* logp, double* log_ratio, float2* stats,
-                      hipStream_t st) {
-  hipLaunchKernelGGL((token_stat_kernel<T>), dim3((unsigned)a.r.n_rows), dim3(kTokBlock), 0, st, a, ref, logp,
-                     log_ratio, stats);
+int launch_token_stat(const TokenRows& a, int64_t row0, int64_t rows, const float* ref, float* logp, double* log_ratio,
+                      float2* stats, hipStream_t st) {
+  const RowShape sh = row_shape<T>(a.r.V);
+#define TS_STAT(NT, KREG)                                                                                        \
+  hipLaunchKernelGGL((token_stat_kernel<T, NT, KREG>), dim3((unsigned)rows), dim3(NT), 0, st, a, row0, ref, logp, \
+                     log_ratio, stats)
+  if (sh.nt == 64)
+    TS_STAT(64, 4);
+  else if (sh.nt == 256)
+    TS_STAT(256, 4);
+  else
+    TS_STAT(512, 8);
+#undef TS_STAT
   return check_launch();
 }
 
 template <typename T>
-int launch_token_grad(const TokenRows& a, const float2* stats, const float* coef, int per_seq, void* grad,
-                      hipStream_t st) {
-  hipLaunchKernelGGL((token_grad_kernel<T>), dim3((unsigned)a.r.n_rows), dim3(kTokBlock), 0, st, a, stats, coef, per_seq,
-                     reinterpret_cast<T*>(grad));
-  return check_launch();
+int launch_token_grad(const TokenRows& a, int64_t row0, int64_t rows, const float2* stats, const float* coef,
+                      int per_seq, void* grad, hipStream_t st) {
+  const int64_t vecs = a.r.V / Vec16<T>::N;
+  const int64_t parts = vecs <= kGradPart ? 1 : (vecs + kGradPart - 1) / kGradPart;
+  // (the grid counts threads in 32 bits)
+  for (int64_t done = 0; done < rows;) {
+    int64_t n = rows - done;
+    if (n * parts > (1 << 23)) n = (1 << 23) / parts;
+    if (n < 1) return TS_ERR_RANGE;
+    hipLaunchKernelGGL((token_grad_kernel<T>), dim3((unsigned)(n * parts)), dim3(kTokBlock), 0, st, a, row0 + done,
+                       (int)parts, stats, coef, per_seq, reinterpret_cast<T*>(grad));
+    const int rc = check_launch();
+    if (rc) return rc;
+    done += n;
+  }
+  return TS_OK;
 }
 
 template <typename T>
@@ -299,7 +469,7 @@ int launch_preference(const TokenRows& a, const float* ref_tok, PrefArgs p, cons
   const int64_t pairs = n_seq / 2;
   int rc = TS_OK;
   if (a.r.n_rows > 0) {
-    rc = launch_token_stat<T>(a, ref_tok, nullptr, w.row, w.stats, st);
+    rc = launch_token_stat<T>(a, 0, a.r.n_rows, ref_tok, nullptr, w.row, w.stats, st);
     if (rc) return rc;
   }
   if (pairs > 0) {
@@ -311,7 +481,7 @@ int launch_preference(const TokenRows& a, const float* ref_tok, PrefArgs p, cons
                      (const int*)nullptr, loss_out);
   rc = check_launch();
   if (rc || !grad || a.r.n_rows == 0) return rc;
-  return launch_token_grad<T>(a, w.stats, w.seq, 1, grad, st);
+  return launch_token_grad<T>(a, 0, a.r.n_rows, w.stats, w.seq, 1, grad, st);
 }
 
 template <typename T>
@@ -322,7 +492,20 @@ int launch_policy(const TokenRows& a, const PolicyArgs& p, const TokenWs& w, int
   int rc = check_launch();
   if (rc) return rc;
   if (a.r.n_rows > 0) {
-    hipLaunchKernelGGL((policy_rows_kernel<T>), dim3((unsigned)a.r.n_rows), dim3(kTokBlock), 0, st, a, p);
+    const dim3 grid((unsigned)a.r.n_rows);
+    const RowShape sh = row_shape<T>(a.r.V);
+    if (sh.nt == 64)
+      hipLaunchKernelGGL((policy_rows_kernel<T, 64, 4>), grid, dim3(64), 0, st, a, p);
+    else if (sh.nt == 256)
+      hipLaunchKernelGGL((policy_rows_kernel<T, 256, 4>), grid, dim3(256), 0, st, a, p);
+    else if (sh.nt == 512)
+      hipLaunchKernelGGL((policy_rows_kernel<T, 512, 8>), grid, dim3(512), 0, st, a, p);
+    else if (sh.kreg == 8)
+      hipLaunchKernelGGL((policy_rows_kernel<T, 1024, 8>), grid, dim3(1024), 0, st, a, p);
+    else if (sh.kreg == 16)
+      hipLaunchKernelGGL((policy_rows_kernel<T, 1024, 16>), grid, dim3(1024), 0, st, a, p);
+    else
+      hipLaunchKernelGGL((policy_rows_kernel<T, 1024, 0>), grid, dim3(1024), 0, st, a, p);
     rc = check_launch();
     if (rc) return rc;
   }
@@ -366,7 +549,7 @@ int ts_token_logp_fwd(const void* s, int64_t n_seq, int64_t seq_len, int64_t V, 
   const ts::TokenRows a =
       ts::token_rows(s, n_seq, seq_len, V, ld_seq, ld_tok, labels, row_mask, ignore_index, temperature);
   hipStream_t st = (hipStream_t)stream;
-  TS_BY_DTYPE(dtype, (ts::launch_token_stat<T>(a, nullptr, logp, nullptr, (float2*)stats, st)))
+  TS_BY_DTYPE(dtype, (ts::launch_token_stat<T>(a, 0, a.r.n_rows, nullptr, logp, nullptr, (float2*)stats, st)))
 }
 
 int ts_token_logp_bwd(const void* s, int64_t n_seq, int64_t seq_len, int64_t V, int64_t ld_seq, int64_t ld_tok,
@@ -380,7 +563,7 @@ int ts_token_logp_bwd(const void* s, int64_t n_seq, int64_t seq_len, int64_t V, 
   const ts::TokenRows a =
       ts::token_rows(s, n_seq, seq_len, V, ld_seq, ld_tok, labels, row_mask, ignore_index, temperature);
   hipStream_t st = (hipStream_t)stream;
-  TS_BY_DTYPE(dtype, (ts::launch_token_grad<T>(a, (const float2*)stats, grad_logp, 0, grad, st)))
+  TS_BY_DTYPE(dtype, (ts::launch_token_grad<T>(a, 0, a.r.n_rows, (const float2*)stats, grad_logp, 0, grad, st)))
 }
 
 size_t ts_token_loss_workspace_bytes(int64_t n_seq, int64_t seq_len) {
@@ -440,9 +623,9 @@ int ts_policy_fwd_bwd(const void* s, int64_t n_seq, int64_t seq_len, int64_t V, 
   p.ref_logp = ref_logp;
   p.adv = advantages;
   p.adv_per_seq = adv_per_seq;
-  p.kl_weight = kl_weight;
-  p.clip_lo = clip_lo;
-  p.clip_hi = clip_hi;
+  p.kl_weight = (float)kl_weight;
+  p.clip_lo = (float)clip_lo;
+  p.clip_hi = (float)clip_hi;
   p.seq_weight = w.seq;
   p.logp = logp;
   p.row_loss = w.row;

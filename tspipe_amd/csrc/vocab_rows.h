@@ -111,9 +111,11 @@ __device__ __forceinline__ VocabStat vstat_block(VocabStat s, float k, VocabStat
   if (NW == 1) return s;
   if (threadIdx.x % kWave == 0) lds[threadIdx.x / kWave] = s;
   __syncthreads();
-  s = lds[0];
+  // lane i takes state i % NW, and the lanes merge (NW states at once would need 3 NW registers a lane)
+  s = lds[threadIdx.x % NW];
 #pragma unroll
-  for (int i = 1; i < NW; ++i) s = vstat_merge(s, lds[i], k);
+  for (int off = NW / 2; off > 0; off >>= 1)
+    s = vstat_merge(s, VocabStat{__shfl_xor(s.m, off, kWave), __shfl_xor(s.z, off, kWave), __shfl_xor(s.a, off, kWave)}, k);
   __syncthreads();  // lds may be used again
   return s;
 }
@@ -206,6 +208,241 @@ __device__ __forceinline__ void vocab_zero_row(T* grow, int64_t V) {
 #pragma unroll
   for (int i = 0; i < VEC; ++i) z.v[i] = zero;
   for (int64_t v = threadIdx.x; v < g.nvec; v += NT) store16(grow + g.head + v * VEC, z);
+}
+
+// ---------------------------------------------------------------------------
+// Rows held in registers.  NT threads hold a row of up to NT * KREG 16-byte
+// vectors, thread t the vectors t, t + NT, ...; what lies in front of the first
+// and behind the last 16-byte boundary is one element per lane of the first
+// wavefront.
+//
+// Sums are taken of 2^(x k + c) with an integer c per wavefront, so that
+// moving a sum from one c to another is exact and no row maximum is needed in
+// front: c = -rint(k x_0) with x_0 the largest of the wavefront's first
+// vectors.  Elements may exceed x_0; a sum that overflows for it (or one that
+// comes out 0 or NaN) is not ok, and the caller walks the row again with its
+// true maximum.  That drops a third of the vector instructions of a
+// maximum-first pass, and the first exponential waits for one vector instead of
+// for the whole row.
+// ---------------------------------------------------------------------------
+constexpr float kVrNoTerm = 1e9f;  // c of a wavefront without a finite element: its factor 2^(C - c) is 0
+
+template <typename T, int NT, int KREG>
+struct RowRegs {
+  Vec16<T> v[KREG];
+  float h, t;  // end elements, -inf where this thread has none
+};
+
+template <typename T, int NT, int KREG>
+__device__ __forceinline__ void regs_load(RowRegs<T, NT, KREG>& r, const T* row, int64_t V, const VocabGeom& g) {
+  constexpr int VEC = Vec16<T>::N;
+#pragma unroll
+  for (int j = 0; j < KREG; ++j) {
+    const int v = (int)threadIdx.x + j * NT;
+    if (v < (int)g.nvec) r.v[j] = load16_stream(row + g.head + (int64_t)v * VEC);
+  }
+  r.h = r.t = -__builtin_inff();
+  if ((int)threadIdx.x < g.head) r.h = to_f32(row[threadIdx.x]);
+  if (g.tail0 + threadIdx.x < V) r.t = to_f32(row[g.tail0 + threadIdx.x]);
+}
+
+// Makes the compiler forget what it knows of a vector, so that each pass
+// unpacks it again instead of keeping eight floats alive for it.
+template <typename T>
+__device__ __forceinline__ void forget(Vec16<T>& v) {
+  u32x4 b;
+  __builtin_memcpy(&b, &v, 16);
+  asm volatile("" : "+v"(b));
+  __builtin_memcpy(&v, &b, 16);
+}
+
+// Largest of the wavefront's first vectors and end elements, of all of its
+// vectors if those hold nothing finite.
+template <typename T, int NT, int KREG>
+__device__ __forceinline__ float regs_anchor(const RowRegs<T, NT, KREG>& r, const VocabGeom& g, float k) {
+  constexpr int VEC = Vec16<T>::N;
+  float m = fmaxf(r.h, r.t);
+  if ((int)threadIdx.x < (int)g.nvec) {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) m = fmaxf(m, to_f32(r.v[0].v[i]));
+  }
+  m = wave_max(m);
+  if (!(m > -1e30f)) {
+#pragma unroll
+    for (int j = 1; j < KREG; ++j) {
+      if ((int)threadIdx.x + j * NT < (int)g.nvec) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) m = fmaxf(m, to_f32(r.v[j].v[i]));
+      }
+    }
+    m = wave_max(m);
+    if (!(m > -1e30f)) return kVrNoTerm;
+  }
+  return m < 1e30f ? -rintf(m * k) : 0.f;  // (an infinite logit makes the sum overflow whatever c is)
+}
+
+struct RowSum {  // z = sum 2^(x k + c), a = sum 2^(x k + c) (x k + c)
+  float c, z, a;
+  bool ok;
+};
+
+// Merged over a workgroup of NW wavefronts; every thread gets the result.
+// `lds` holds NW RowSums and may be used again after another barrier.
+template <int NW, bool WITH_A>
+__device__ __forceinline__ RowSum rowsum_block(float c, float z, float a, RowSum* lds) {
+  z = wave_sum(z);
+  if (WITH_A) a = wave_sum(a);
+  RowSum r{c, z, a, true};
+  if (NW > 1) {
+    if (threadIdx.x % kWave == 0) lds[threadIdx.x / kWave] = r;
+    __syncthreads();
+    // lane i takes the sum of wavefront i % NW (all NW of them in every lane would need 3 NW registers)
+    const RowSum w = lds[threadIdx.x % NW];
+    float C = w.c;
+#pragma unroll
+    for (int off = NW / 2; off > 0; off >>= 1) C = fminf(C, __shfl_xor(C, off, kWave));
+    const float d = C - w.c, f = fast_exp2(d);
+    r = RowSum{C, w.z * f, WITH_A ? f * fmaf(w.z, d, w.a) : 0.f, true};
+#pragma unroll
+    for (int off = NW / 2; off > 0; off >>= 1) {
+      r.z += __shfl_xor(r.z, off, kWave);
+      if (WITH_A) r.a += __shfl_xor(r.a, off, kWave);
+    }
+  }
+  r.ok = r.z > 1e-30f && r.z < __builtin_inff() && r.c < kVrNoTerm;
+  return r;
+}
+
+// An fp32 number and what its rounding left out.  The log probabilities of a row
+// are formed in this type: a sum over a sequence of them, or the difference of
+// two that nearly agree, would show the last bits of fp32, and 64-bit
+// logarithms and exponentials in a kernel that holds a row in registers spill
+// (28 % of the policy loss's time at 8192 x 65536 bf16).
+struct Float2x {
+  float hi, lo;
+};
+
+__device__ __forceinline__ Float2x two_sum(float x, float y) {
+#pragma clang fp contract(off)
+  const float s = x + y, v = s - x;
+  return Float2x{s, (x - (s - v)) + (y - v)};
+}
+
+__device__ __forceinline__ Float2x two_mul(float x, float y) {
+#pragma clang fp contract(off)
+  const float p = x * y;
+  return Float2x{p, __builtin_fmaf(x, y, -p)};
+}
+
+// log2(z), z > 0 and normal, within 2e-7: the hardware's logarithm, corrected by what
+// its own power of two leaves of z.
+__device__ __forceinline__ Float2x log2_2x(float z) {
+  const float e = (float)(__builtin_amdgcn_frexp_expf(z));  // z = f 2^e, f in [1/2, 1)
+  const float f = __builtin_amdgcn_frexp_mantf(z);
+  const float l = __builtin_amdgcn_logf(f);
+  const Float2x s = two_sum(e, l);
+  return Float2x{s.hi, s.lo + kVrLog2e * fmaf(f, fast_exp2(-l), -1.f)};
+}
+
+// ln of the soft-max probability of a logit of the row.  Without the sum a the
+// factor k stays as rounded, in the logit's own exponent too: what the rounding
+// took then counts only for the logit's distance from the row's mean.
+template <bool WITH_A>
+__device__ __forceinline__ Float2x rowsum_log_prob(const VocabRows& r, const RowSum& s, float x) {
+#pragma clang fp contract(off)
+  const Float2x p = two_mul(x, r.k), q = two_sum(p.hi, s.c), l = log2_2x(s.z);
+  const Float2x h = two_sum(q.hi, -l.hi);
+  float lo = (p.lo + q.lo) + (h.lo - l.lo);
+  if (WITH_A) lo += r.k_rel * (p.hi - (s.a / s.z - s.c));  // a / z - c: mean of x k under the soft-max
+  if (!(__builtin_fabsf(h.hi) < __builtin_inff())) return Float2x{h.hi, 0.f};  // a logit of -inf
+  const Float2x m = two_mul(h.hi, 0.693147182464599609375f);
+  return two_sum(m.hi, m.lo + (lo * 0.693147182464599609375f + h.hi * -1.904654323e-09f));
+}
+
+// One thread's terms of its registers: f(x, exponent) per element.
+template <typename T, int NT, int KREG, typename F>
+__device__ __forceinline__ void regs_each(RowRegs<T, NT, KREG>& r, const VocabGeom& g, F f) {
+  constexpr int VEC = Vec16<T>::N;
+#pragma unroll
+  for (int j = 0; j < KREG; ++j) {
+    if ((int)threadIdx.x + j * NT < (int)g.nvec) {
+      forget(r.v[j]);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) f(to_f32(r.v[j].v[i]));
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  }
+}
+
+template <typename T, int NT, int KREG, bool WITH_A>
+__device__ __forceinline__ RowSum regs_sum(RowRegs<T, NT, KREG>& r, const VocabGeom& g, float k, RowSum* lds) {
+  const float c = regs_anchor(r, g, k);
+  float z = 0.f, a = 0.f;
+  auto add = [&](float x) {
+    const float d = fmaf(x, k, c), e = fast_exp2(d);
+    z += e;
+    if (WITH_A) a = fmaf(e, fmaxf(d, -1e30f), a);
+  };
+  if (threadIdx.x < kWave) {  // the end elements
+    add(r.h);
+    add(r.t);
+  }
+  regs_each(r, g, add);
+  return rowsum_block<NT / kWave, WITH_A>(c, z, a, lds);
+}
+
+// grow[j] = f(x[j]) from registers, but for element `special` (or -1), which
+// gets f_special(x).
+template <typename T, int NT, int KREG, typename F, typename G>
+__device__ __forceinline__ void regs_map(RowRegs<T, NT, KREG>& r, const VocabGeom& g, const T* row, T* grow, int64_t V,
+                                         int special, F f, G f_special) {
+  constexpr int VEC = Vec16<T>::N;
+  if ((int)threadIdx.x < g.head)
+    grow[threadIdx.x] = from_f32<T>((int)threadIdx.x == special ? f_special(r.h) : f(r.h));
+  const int64_t t = g.tail0 + threadIdx.x;
+  if (t < V) grow[t] = from_f32<T>((int)t == special ? f_special(r.t) : f(r.t));
+  const bool gvec = (((uintptr_t)grow ^ (uintptr_t)row) & 15u) == 0;
+  const int sv = special >= g.head ? (special - g.head) / VEC : -1;
+  const int si = special - g.head - sv * VEC;
+#pragma unroll
+  for (int j = 0; j < KREG; ++j) {
+    const int v = (int)threadIdx.x + j * NT;
+    if (v < (int)g.nvec) {
+      forget(r.v[j]);
+      Vec16<T> o;
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) o.v[i] = from_f32<T>(f(to_f32(r.v[j].v[i])));
+      if (v == sv) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i)
+          if (i == si) o.v[i] = from_f32<T>(f_special(to_f32(r.v[j].v[i])));
+      }
+      T* p = grow + g.head + (int64_t)v * VEC;
+      if (gvec) {
+        store16_stream(p, o);
+      } else {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) p[i] = o.v[i];
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  }
+}
+
+// How a row of V elements of T is held: threads and vectors per thread of the
+// smallest arrangement it fits, 0 threads for rows that fit none.
+struct RowShape {
+  int nt, kreg;
+};
+template <typename T>
+inline RowShape row_shape(int64_t V) {
+  const int64_t vecs = V / Vec16<T>::N;
+  if (vecs <= 64 * 4) return RowShape{64, 4};
+  if (vecs <= 256 * 4) return RowShape{256, 4};
+  if (vecs <= 512 * 8) return RowShape{512, 8};
+  if (vecs <= 1024 * 8) return RowShape{1024, 8};
+  if (vecs <= 1024 * 16) return RowShape{1024, 16};
+  return RowShape{0, 0};
 }
 
 // Sum of doubles over a workgroup of NW wavefronts, in a fixed order; every
