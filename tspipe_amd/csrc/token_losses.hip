@@ -101,7 +101,7 @@ __global__ __launch_bounds__(NT) void token_stat_kernel(const TokenRows a, int64
       __builtin_amdgcn_sched_barrier(0);
     }
   }
-  const RowSum s = rowsum_block<NT / kWave, true>(c, z, s_a, lds);
+  const RowSum s = rowsum_block<NT / kWave, kSumMean>(c, z, s_a, lds);
   Float2x lp;
   float2 st;
   if (s.ok) {
@@ -255,9 +255,7 @@ __global__ __launch_bounds__(kTokBlock) void pref_join_kernel(const TokenRows a,
 __global__ __launch_bounds__(1024) void sum_f64_kernel(const double* __restrict__ v, int64_t n, double scale,
                                                        const int* __restrict__ live, float* __restrict__ out) {
   __shared__ double lds[1024 / kWave];
-  double s = 0.0;
-  for (int64_t i = threadIdx.x; i < n; i += 1024) s += v[i];
-  s = block_sum_f64<1024 / kWave>(s, lds);
+  const double s = block_sum_f64<1024 / kWave>(thread_share_of_sum_f64<1024>(v, n), lds);
   if (threadIdx.x == 0) *out = (live ? *live != 0 : n != 0) ? (float)(s * scale) : __builtin_nanf("");
 }
 
@@ -383,7 +381,7 @@ __global__ __launch_bounds__(NT) void policy_rows_kernel(const TokenRows a, cons
     const VocabGeom g = vocab_geom(srow, V);
     RowRegs<T, NT, KREG> r;
     regs_load(r, srow, V, g);
-    const RowSum s = regs_sum<T, NT, KREG, false>(r, g, a.r.k, lds);
+    const RowSum s = regs_sum<T, NT, KREG>(r, g, a.r.k, lds);
     if (s.ok) {
       if (threadIdx.x == 0) coef = policy_finish(a, p, row, rowsum_log_prob<false>(a.r, s, to_f32(srow[label])));
       if (!grow) return;

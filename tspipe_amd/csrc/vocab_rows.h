@@ -281,17 +281,22 @@ __device__ __forceinline__ float regs_anchor(const RowRegs<T, NT, KREG>& r, cons
   return m < 1e30f ? -rintf(m * k) : 0.f;  // (an infinite logit makes the sum overflow whatever c is)
 }
 
-struct RowSum {  // z = sum 2^(x k + c), a = sum 2^(x k + c) (x k + c)
+struct RowSum {  // z = sum 2^(x k + c), a: nothing, or one of the two below
   float c, z, a;
   bool ok;
+};
+enum {
+  kSumOnly = 0,
+  kSumMean = 1,   // a = sum 2^(x k + c) (x k + c)
+  kSumSecond = 2  // a = another sum of 2^(x k + c); the row's sum is z + a
 };
 
 // Merged over a workgroup of NW wavefronts; every thread gets the result.
 // `lds` holds NW RowSums and may be used again after another barrier.
-template <int NW, bool WITH_A>
+template <int NW, int KIND>
 __device__ __forceinline__ RowSum rowsum_block(float c, float z, float a, RowSum* lds) {
   z = wave_sum(z);
-  if (WITH_A) a = wave_sum(a);
+  if (KIND != kSumOnly) a = wave_sum(a);
   RowSum r{c, z, a, true};
   if (NW > 1) {
     if (threadIdx.x % kWave == 0) lds[threadIdx.x / kWave] = r;
@@ -302,14 +307,15 @@ __device__ __forceinline__ RowSum rowsum_block(float c, float z, float a, RowSum
 #pragma unroll
     for (int off = NW / 2; off > 0; off >>= 1) C = fminf(C, __shfl_xor(C, off, kWave));
     const float d = C - w.c, f = fast_exp2(d);
-    r = RowSum{C, w.z * f, WITH_A ? f * fmaf(w.z, d, w.a) : 0.f, true};
+    r = RowSum{C, w.z * f, KIND == kSumMean ? f * fmaf(w.z, d, w.a) : KIND == kSumSecond ? f * w.a : 0.f, true};
 #pragma unroll
     for (int off = NW / 2; off > 0; off >>= 1) {
       r.z += __shfl_xor(r.z, off, kWave);
-      if (WITH_A) r.a += __shfl_xor(r.a, off, kWave);
+      if (KIND != kSumOnly) r.a += __shfl_xor(r.a, off, kWave);
     }
   }
-  r.ok = r.z > 1e-30f && r.z < __builtin_inff() && r.c < kVrNoTerm;
+  const float all = KIND == kSumSecond ? r.z + r.a : r.z;
+  r.ok = all > 1e-30f && all < __builtin_inff() && r.c < kVrNoTerm;
   return r;
 }
 
@@ -374,21 +380,17 @@ __device__ __forceinline__ void regs_each(RowRegs<T, NT, KREG>& r, const VocabGe
   }
 }
 
-template <typename T, int NT, int KREG, bool WITH_A>
+template <typename T, int NT, int KREG>
 __device__ __forceinline__ RowSum regs_sum(RowRegs<T, NT, KREG>& r, const VocabGeom& g, float k, RowSum* lds) {
   const float c = regs_anchor(r, g, k);
-  float z = 0.f, a = 0.f;
-  auto add = [&](float x) {
-    const float d = fmaf(x, k, c), e = fast_exp2(d);
-    z += e;
-    if (WITH_A) a = fmaf(e, fmaxf(d, -1e30f), a);
-  };
+  float z = 0.f;
+  auto add = [&](float x) { z += fast_exp2(fmaf(x, k, c)); };
   if (threadIdx.x < kWave) {  // the end elements
     add(r.h);
     add(r.t);
   }
   regs_each(r, g, add);
-  return rowsum_block<NT / kWave, WITH_A>(c, z, a, lds);
+  return rowsum_block<NT / kWave, kSumOnly>(c, z, 0.f, lds);
 }
 
 // grow[j] = f(x[j]) from registers, but for element `special` (or -1), which
@@ -427,6 +429,25 @@ __device__ __forceinline__ void regs_map(RowRegs<T, NT, KREG>& r, const VocabGeo
     }
     __builtin_amdgcn_sched_barrier(0);
   }
+}
+
+// This thread's share of sum(v[0..n)) when NT threads walk the array together, in a
+// fixed order, eight loads in flight each.
+template <int NT>
+__device__ __forceinline__ double thread_share_of_sum_f64(const double* __restrict__ v, int64_t n) {
+  constexpr int kInFlight = 8;
+  double s = 0.0;
+  for (int64_t i0 = threadIdx.x; i0 < n; i0 += (int64_t)NT * kInFlight) {
+    double x[kInFlight];
+#pragma unroll
+    for (int j = 0; j < kInFlight; ++j) {
+      const int64_t i = i0 + (int64_t)j * NT;
+      x[j] = i < n ? v[i] : 0.0;
+    }
+#pragma unroll
+    for (int j = 0; j < kInFlight; ++j) s += x[j];
+  }
+  return s;
 }
 
 // How a row of V elements of T is held: threads and vectors per thread of the
