@@ -392,7 +392,7 @@ int ts_top_logits(const void* s, int64_t n_seq, int64_t seq_len, int64_t V, int6
  * loss = weight * T^2 * mean of the terms over the rows of row_mask (NULL: all).
  * t_dtype: type of t_values [rows, k]; k <= 256; with t_logsumexp V <= 2^20
  * (else TS_ERR_RANGE). */
-size_t ts_top_distil_workspace_bytes(int64_t n_rows);
+size_t ts_top_distil_workspace_bytes(int64_t n_rows, int k);
 
 int ts_top_distil_fwd_bwd(const void* s, int64_t n_seq, int64_t seq_len, int64_t V, int64_t ld_seq,
                           int64_t ld_tok, const void* t_values, int t_dtype,

@@ -502,3 +502,127 @@ def test_training_steps_with_the_plug_in(device):
         assert abs(loss.item() - l64.item()) < 1e-4
         assert (wd.grad.cpu().double() - w64.grad).abs().max() < 1e-4 * w64.grad.abs().max() + 1e-5
         w64, wd = w64.detach() - 0.5 * w64.grad, wd.detach() - 0.5 * wd.grad
+
+
+# ---- the C++ node and the Python functions ----------------------------------------------------
+
+def _both_ways(monkeypatch, f):
+    from tspipe_amd import _vocab
+    assert _vocab.host_for(torch.zeros(1, device="cuda")) is not None
+    monkeypatch.setattr(_vocab, "_HOST_NODE", True)
+    a = f()
+    monkeypatch.setattr(_vocab, "_HOST_NODE", False)
+    return a, f()
+
+
+def test_host_node_and_python_functions_agree(device, monkeypatch):
+    x, labels, g = make((4, 13, 1501), torch.bfloat16, 111)
+    xd, lab = x.to(device), labels.to(device)
+    mask = (torch.rand(4, 13, generator=g) < 0.7).to(device)
+    ref = (torch.randn(4, 13, generator=g) - 8).to(device)
+    adv = torch.randn(4, generator=g).to(device)
+    top = ta.top_logits(xd, 20, 2.0)
+
+    def everything():
+        leaf = xd.clone().requires_grad_()
+        outs = []
+        for view in (leaf, leaf[:, :, :]):
+            lp = ta.token_log_probs(view, lab, 0.9, row_mask=mask)
+            l1, r = ta.preference_loss(view, lab, ref, 0.2, label_smoothing=0.1, row_mask=mask, return_rewards=True)
+            l2, lp2 = ta.clipped_policy_loss(view, lab, ref, adv, ref, 0.1, reduction="sequence", row_mask=mask,
+                                             return_log_probs=True)
+            l3 = ta.top_logits_distil_loss(view, top.values, top.indices, 2.0, row_mask=mask, t_logsumexp=top.logsumexp)
+            outs += [lp, l1, r, l2, lp2, l3, *ta.top_logits(view, 7)]
+            for loss in (lp.sum(), l1, l2 * 2.0, l3):
+                outs += torch.autograd.grad(loss, leaf)
+        return [o.detach() for o in outs]
+
+    a, b = _both_ways(monkeypatch, everything)
+    assert len(a) == len(b)
+    for i, (p, q) in enumerate(zip(a, b)):
+        assert bits_equal(p, q), i
+
+
+def test_both_refuse_alike(device, monkeypatch):
+    x, labels, _ = make((2, 5, 300), torch.float32, 121)
+    lab, ref = labels.to(device), torch.zeros(2, 5, device=device)
+
+    def twice():
+        leaf = x.to(device).requires_grad_()
+        loss = ta.preference_loss(leaf, lab, ref)
+        loss.backward()
+        with pytest.raises(RuntimeError):
+            loss.backward()
+        # log probabilities read their logits again: a change in between is noticed
+        mid = leaf * 1.0
+        lp = ta.token_log_probs(mid, lab).sum()
+        mid.add_(1.0)
+        with pytest.raises(RuntimeError):
+            lp.backward()
+        # a second derivative is refused
+        lp = ta.token_log_probs(leaf, lab).sum()
+        with pytest.raises(RuntimeError):
+            g, = torch.autograd.grad(lp, leaf, create_graph=True)
+            g.sum().backward()
+        for call in (lambda: ta.preference_loss(leaf, lab[:, :4], ref), lambda: ta.preference_loss(leaf, lab, ref[:, :4]),
+                     lambda: ta.clipped_policy_loss(leaf, lab, ref, ref[:1, 0]),
+                     lambda: ta.token_log_probs(leaf, lab.cpu()),
+                     lambda: ta.top_logits(leaf, 301), lambda: ta.top_logits(leaf, 0),
+                     lambda: ta.top_logits_distil_loss(leaf, ref, lab.to(torch.int32), 1.0)):
+            with pytest.raises(ValueError):
+                call()
+        for call in (lambda: ta.token_log_probs(leaf, lab.float()), lambda: ta.token_log_probs(leaf.double(), lab),
+                     lambda: ta.preference_loss(leaf, lab, lab), lambda: ta.top_logits(leaf.long(), 2)):
+            with pytest.raises(TypeError):
+                call()
+        return True
+
+    assert _both_ways(monkeypatch, twice) == (True, True)
+    # without gradients there is nothing to record
+    with torch.no_grad():
+        leaf = x.to(device).requires_grad_()
+        assert not ta.preference_loss(leaf, lab, ref).requires_grad
+    assert not ta.preference_loss(x.to(device), lab, ref).requires_grad
+
+
+def test_two_threads_on_two_streams(device):
+    import threading
+    x, labels, g = make((4, 40, 3000), torch.bfloat16, 131)
+    lab, ref = labels.to(device), (torch.randn(4, 40, generator=g) - 8).to(device)
+    adv = torch.randn(4, generator=g).to(device)
+    inputs = [(x.float() * s).to(torch.bfloat16).to(device) for s in (1.0, 0.7)]
+
+    def step(xd):
+        leaf = xd.clone().requires_grad_()
+        l1 = ta.preference_loss(leaf, lab, ref)
+        g1, = torch.autograd.grad(l1, leaf)
+        l2 = ta.clipped_policy_loss(leaf, lab, ref, adv, ref, 0.1)
+        g2, = torch.autograd.grad(l2, leaf)
+        top = ta.top_logits(leaf, 11)
+        l3 = ta.top_logits_distil_loss(leaf, top.values, top.indices, 2.0)
+        g3, = torch.autograd.grad(l3, leaf)
+        return [l1.detach(), g1, l2.detach(), g2, *top, l3.detach(), g3]
+
+    want = [step(t) for t in inputs]
+    torch.cuda.synchronize()
+    got, errors = [None, None], []
+
+    def work(i):
+        try:
+            s = torch.cuda.Stream()
+            with torch.cuda.stream(s):
+                for _ in range(5):
+                    got[i] = step(inputs[i])
+            s.synchronize()
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors
+    for w, h in zip(want, got):
+        for a, b in zip(w, h):
+            assert bits_equal(a, b)

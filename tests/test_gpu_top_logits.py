@@ -76,7 +76,7 @@ def test_top_logits_nan_and_infinities(device):
     i = top.indices.cpu()
     assert i[0, 0] == 77 and i[1, :2].tolist() == [5, 4000] and torch.isnan(top.values[1, :2]).all()
     assert i[2].tolist() == list(range(120)) and i[3, 100:].tolist() == list(range(100, 120))
-    assert torch.isnan(top.logsumexp[1]) and top.logsumexp[2].item() == float("-inf")
+    assert top.logsumexp[0].item() == float("inf") and torch.isnan(top.logsumexp[1]) and top.logsumexp[2].item() == float("-inf")
 
 
 @pytest.mark.parametrize("dtype", DTYPES)

@@ -35,7 +35,7 @@ def test_entry_points_validate_before_launching():
     assert dis(k=0) == ARG and dis(k=257) == RANGE and dis(tdt=5) == ARG and dis(T=-1.0) == ARG and dis(ws=P + 8) == ALIGN
     assert dis(V=(1 << 20) + 1, lse=P) == RANGE
     assert lib.ts_token_loss_workspace_bytes(-1, 4) == 0 and lib.ts_token_loss_workspace_bytes(4, 7) > 4 * 7 * 16
-    assert lib.ts_top_distil_workspace_bytes(5) >= 40
+    assert lib.ts_top_distil_workspace_bytes(5, 7) >= 5 * (8 + 7 * 4)
 
 
 def test_host_tensors_are_refused():

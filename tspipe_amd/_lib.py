@@ -60,7 +60,7 @@ SIGNATURES = {
                                   c_double, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p]),
     "ts_top_logits": (c_int, [c_void_p, c_int64, c_int64, c_int64, c_int64, c_int64, c_int, c_double, c_void_p,
                               c_void_p, c_void_p, c_int, c_void_p]),
-    "ts_top_distil_workspace_bytes": (c_size_t, [c_int64]),
+    "ts_top_distil_workspace_bytes": (c_size_t, [c_int64, c_int]),
     "ts_top_distil_fwd_bwd": (c_int, [c_void_p, c_int64, c_int64, c_int64, c_int64, c_int64, c_void_p, c_int, c_void_p,
                                       c_void_p, c_int, c_void_p, c_double, c_double, c_void_p, c_void_p, c_void_p,
                                       c_int, c_void_p]),
@@ -161,6 +161,11 @@ def host_helper():
                                         addr(handle.ts_mse_workspace_bytes), addr(handle.ts_mse_fwd_bwd),
                                         addr(handle.ts_cosine_workspace_bytes), addr(handle.ts_cosine_fwd_bwd),
                                         addr(handle.ts_byol_fwd_bwd))
+                    if hasattr(mod, "bind_vocab"):
+                        mod.bind_vocab(addr(handle.ts_token_logp_fwd), addr(handle.ts_token_logp_bwd),
+                                       addr(handle.ts_token_loss_workspace_bytes), addr(handle.ts_preference_fwd_bwd),
+                                       addr(handle.ts_policy_fwd_bwd), addr(handle.ts_top_logits),
+                                       addr(handle.ts_top_distil_workspace_bytes), addr(handle.ts_top_distil_fwd_bwd))
                 _host = mod
             _host_tried = True
     return _host

@@ -7,6 +7,26 @@ from torch import Tensor
 from . import _lib
 
 
+_HOST_NODE = True   # tests switch this off to reach the Python autograd.Functions
+
+
+def host_for(*tensors):
+    """The C++ host helper and the current stream's handle when it may take a
+    call on these tensors (plain device tensors, None allowed), else None: the
+    same entry points on the same arguments, so the same bits, without the
+    interpreter's share of the host time.  Its functions return None for calls
+    that are not plain, and the Python function takes those."""
+    host = _lib.host_helper() if _HOST_NODE else None
+    if host is None or not hasattr(host, "vocab_top"):
+        return None
+    for t in tensors:
+        if t is not None and type(t) is not Tensor:
+            return None
+    if not tensors[0].is_cuda:
+        return None
+    return host, _lib.current_stream_ptr(tensors[0].device)
+
+
 class Rows(NamedTuple):
     """Logits as the kernels take them: ``n_seq`` sequences of ``seq_len``
     tokens, strides in elements; ``x`` keeps the memory alive."""

@@ -20,8 +20,10 @@ struct TokenRows {
   int64_t ignore_index;
 };
 
+// `scalar`: the row is the same in every lane.
+template <bool scalar>
 __device__ __forceinline__ bool token_live(const TokenRows& a, int64_t row, int64_t* label) {
-  const int64_t l = a.labels[row];
+  const int64_t l = scalar ? scalar_load(a.labels + row) : a.labels[row];
   *label = l;
   return l != a.ignore_index && l >= 0 && l < a.r.V && (!a.mask || a.mask[row] != 0);
 }
@@ -60,7 +62,7 @@ __global__ __launch_bounds__(NT) void token_stat_kernel(const TokenRows a, int64
   __shared__ VocabStat lds_v[NT / kWave];
   const int64_t row = row0 + blockIdx.x;
   int64_t label;
-  if (!token_live(a, row, &label)) {
+  if (!token_live<true>(a, row, &label)) {
     if (threadIdx.x == 0) {
       if (logp) logp[row] = 0.f;
       if (log_ratio) log_ratio[row] = 0.0;
@@ -82,19 +84,19 @@ __global__ __launch_bounds__(NT) void token_stat_kernel(const TokenRows a, int64
     s_a = fmaf(e, fmaxf(d, -1e30f), s_a);
   };
   if (threadIdx.x < kWave) {
-    add(r.h);
-    add(r.t);
+    add(r.h());
+    add(r.t());
   }
   regs_each(r, g, add);
   for (int64_t v0 = NT * KREG; v0 < g.nvec; v0 += NT * KREG) {
+    const int left = g.nvec - v0 < NT * KREG ? (int)(g.nvec - v0) : NT * KREG;
+    const VecBuffer piece = vec_buffer(srow + g.head + v0 * VEC, left);
+#pragma unroll
+    for (int j = 0; j < KREG; ++j) r.v[j] = vec_load<T>(piece, threadIdx.x + j * NT);
 #pragma unroll
     for (int j = 0; j < KREG; ++j) {
-      const int64_t v = v0 + threadIdx.x + j * NT;
-      if (v < g.nvec) r.v[j] = load16_stream(srow + g.head + v * VEC);
-    }
-#pragma unroll
-    for (int j = 0; j < KREG; ++j) {
-      if (v0 + threadIdx.x + j * NT < g.nvec) {
+      if ((int)threadIdx.x + j * NT < left) {
+        forget(r.v[j]);
 #pragma unroll
         for (int i = 0; i < VEC; ++i) add(to_f32(r.v[j].v[i]));
       }
@@ -111,8 +113,7 @@ __global__ __launch_bounds__(NT) void token_stat_kernel(const TokenRows a, int64
   } else {
     const VocabStat sv = vstat_block<NT / kWave>(vocab_stat_walk<T, NT>(srow, V, k), k, lds_v);
     if (threadIdx.x != 0) return;
-    const double l = vstat_log_prob(a.r, sv, to_f32(srow[label]));
-    lp = Float2x{(float)l, isfinite(l) ? (float)(l - (double)(float)l) : 0.f};
+    lp = vstat_log_prob(a.r, sv, to_f32(srow[label]));
     st = make_float2(sv.m, -sv.z);
   }
   if (logp) logp[row] = lp.hi;
@@ -138,7 +139,7 @@ __global__ __launch_bounds__(kTokBlock) void token_grad_kernel(const TokenRows a
   const int tid = threadIdx.x;
   T* grow = grad + row * V;
   int64_t label;
-  if (!token_live(a, row, &label)) {
+  if (!token_live<true>(a, row, &label)) {
     const VocabGeom g = vocab_geom(grow, V);
     const T zero = from_f32<T>(0.f);
     if (part == 0 && tid < g.head) grow[tid] = zero;
@@ -156,22 +157,25 @@ __global__ __launch_bounds__(kTokBlock) void token_grad_kernel(const TokenRows a
   const T* srow = vocab_row<T>(a.r, row);
   const VocabGeom g = vocab_geom(srow, V);
   Vec16<T> x[kGradVecs];
+  const int64_t e0 = g.head + v0 * VEC, some = g.nvec - v0;  // this part's first element and vectors
+  const int left = some < kGradPart ? (int)some : kGradPart;
+  const VecBuffer from = vec_buffer(srow + e0, left);
 #pragma unroll
-  for (int j = 0; j < kGradVecs; ++j) {
-    const int64_t v = v0 + tid + j * kTokBlock;
-    if (v < g.nvec) x[j] = load16_stream(srow + g.head + v * VEC);
-  }
-  const TokenGrad f(a.r.k, stats[row], coef[per_seq ? row / a.r.seq_len : row] * (float)a.r.inv_T);
+  for (int j = 0; j < kGradVecs; ++j) x[j] = vec_load<T>(from, tid + j * kTokBlock);
+  const TokenGrad f(a.r.k, scalar_load(stats + row),
+                    scalar_load(coef + (per_seq ? (uint32_t)row / (uint32_t)a.r.seq_len : row)) * (float)a.r.inv_T);
   auto one = [&](float xv, int64_t j) { return from_f32<T>(j == label ? f.label(xv) : f.other(xv)); };
   if (part == 0 && tid < g.head) grow[tid] = one(to_f32(srow[tid]), tid);
   if (part == parts - 1 && g.tail0 + tid < V) grow[g.tail0 + tid] = one(to_f32(srow[g.tail0 + tid]), g.tail0 + tid);
   const bool gvec = (((uintptr_t)grow ^ (uintptr_t)srow) & 15u) == 0;
-  const int64_t lv = label >= g.head ? (label - g.head) / VEC : -1;
-  const int li = (int)(label - g.head - lv * VEC);
+  const VecBuffer to = vec_buffer(grow + e0, gvec ? left : 0);
+  const int64_t at = label - e0;
+  const int lv = at >= 0 && at / VEC < kGradPart ? (int)(at / VEC) : -1;
+  const int li = lv < 0 ? 0 : (int)(at - (int64_t)lv * VEC);
 #pragma unroll
   for (int j = 0; j < kGradVecs; ++j) {
-    const int64_t v = v0 + tid + j * kTokBlock;
-    if (v < g.nvec) {
+    const int v = tid + j * kTokBlock;
+    if (v < left) {
       forget(x[j]);
       Vec16<T> o;
 #pragma unroll
@@ -181,10 +185,10 @@ __global__ __launch_bounds__(kTokBlock) void token_grad_kernel(const TokenRows a
         for (int i = 0; i < VEC; ++i)
           if (i == li) o.v[i] = from_f32<T>(f.label(to_f32(x[j].v[i])));
       }
-      T* p = grow + g.head + v * VEC;
       if (gvec) {
-        store16_stream(p, o);
+        vec_store(to, (uint32_t)v, o);
       } else {
+        T* p = grow + e0 + v * VEC;
 #pragma unroll
         for (int i = 0; i < VEC; ++i) p[i] = o.v[i];
       }
@@ -222,7 +226,7 @@ __global__ __launch_bounds__(kTokBlock) void pref_join_kernel(const TokenRows a,
       s += p.log_ratio[row0 + i];
       if (p.average) {
         int64_t label;
-        c += token_live(a, row0 + i, &label) ? 1.0 : 0.0;
+        c += token_live<false>(a, row0 + i, &label) ? 1.0 : 0.0;
       }
     }
     R[side] = block_sum_f64<kTokBlock / kWave>(s, lds);
@@ -287,7 +291,7 @@ __global__ __launch_bounds__(1024) void policy_weight_kernel(const TokenRows a, 
     int c = 0;
     for (int64_t i = lane; i < L; i += kWave) {
       int64_t label;
-      c += token_live(a, q * L + i, &label);
+      c += token_live<false>(a, q * L + i, &label);
     }
 #pragma unroll
     for (int off = kWave / 2; off > 0; off >>= 1) c += __shfl_xor(c, off, kWave);
@@ -348,10 +352,7 @@ __device__ __forceinline__ void policy_row_walked(const TokenRows& a, const Poli
   __shared__ float coef;
   const float k = a.r.k;
   const VocabStat s = vstat_block<NT / kWave>(vocab_stat_walk<T, NT>(srow, a.r.V, k), k, lds);
-  if (threadIdx.x == 0) {
-    const double l = vstat_log_prob(a.r, s, to_f32(srow[label]));
-    coef = policy_finish(a, p, row, Float2x{(float)l, isfinite(l) ? (float)(l - (double)(float)l) : 0.f});
-  }
+  if (threadIdx.x == 0) coef = policy_finish(a, p, row, vstat_log_prob(a.r, s, to_f32(srow[label])));
   if (!grow) return;
   __syncthreads();
   const TokenGrad f(k, make_float2(s.m, -s.z), coef);
@@ -368,7 +369,7 @@ __global__ __launch_bounds__(NT) void policy_rows_kernel(const TokenRows a, cons
   const int64_t row = blockIdx.x, V = a.r.V;
   T* grow = p.grad ? reinterpret_cast<T*>(p.grad) + row * V : nullptr;
   int64_t label;
-  if (!token_live(a, row, &label)) {
+  if (!token_live<true>(a, row, &label)) {
     if (threadIdx.x == 0) {
       if (p.logp) p.logp[row] = 0.f;
       p.row_loss[row] = 0.0;

@@ -6,7 +6,6 @@ namespace ts {
 
 constexpr int kTopMax = 256;                   // entries a row may keep
 constexpr int64_t kTopTailVocab = 1 << 20;     // the kept entries are marked in LDS, a bit per vocabulary entry
-constexpr int64_t kTopSelfCountRows = 8192;    // up to this many rows every workgroup counts the mask itself
 
 // ---- the k largest logits --------------------------------------------------------
 
@@ -83,7 +82,12 @@ __device__ __forceinline__ void top_row_walked(const VocabRows& a, int64_t row, 
   const int64_t V = a.V;
   if (lse) {
     const VocabStat s = vstat_block<NT / kWave>(vocab_stat_walk<T, NT>(x, V, a.k), a.k, sh.stats);
-    if (threadIdx.x == 0) lse[row] = (float)((double)s.m * a.inv_T + kVrLn2 * vstat_log2z(s, a.k_rel));
+    const Float2x lz = log2_2x(s.z);  // (for -inf throughout, z = 0 and m is a stand-in)
+    float l = (float)((double)s.m * a.inv_T + kVrLn2 * ((double)lz.hi + (double)lz.lo));
+    if (s.m == __builtin_inff() &&  // uniform
+        top_count<T, NT>(x, V, sh.counts, [](float v, int) { return v != v; }) == 0)
+      l = s.m;
+    if (threadIdx.x == 0) lse[row] = l;
   }
   uint32_t t = 0;
   for (int bit = 31; bit >= 0; --bit) {
@@ -149,7 +153,7 @@ __device__ __forceinline__ void top_refine(TopShared<NT>& sh, int n, int k) {
 // groups: 68 expected) -- and the candidates' ranks are counted.  The row's sum
 // is taken in the same walk over the registers.
 template <typename T, int NT, int KREG>
-__global__ __launch_bounds__(NT) void top_logits_kernel(const VocabRows a, int k, T* __restrict__ values,
+__global__ __launch_bounds__(NT, NT > 256 ? (NT > 512 ? 8 : 6) : 1) void top_logits_kernel(const VocabRows a, int k, T* __restrict__ values,
                                                         int32_t* __restrict__ indices, float* __restrict__ lse) {
   constexpr int VEC = Vec16<T>::N;
   __shared__ TopShared<NT> sh;
@@ -163,21 +167,18 @@ __global__ __launch_bounds__(NT) void top_logits_kernel(const VocabRows a, int k
   regs_load(r, x, V, g);
   if (tid == 0) sh.n = 0;
   const float c = regs_anchor(r, g, kk);
-  float z = 0.f, s_a = 0.f, m0 = fmaxf(r.h, r.t), m1 = -__builtin_inff();
-  auto add = [&](float xv) {
-    const float d = fmaf(xv, kk, c), e = fast_exp2(d);
-    z += e;
-    s_a = fmaf(e, fmaxf(d, -1e30f), s_a);
-  };
+  float z = 0.f, m0 = fmaxf(r.h(), r.t()), m1 = -__builtin_inff();
+  auto add = [&](float xv) { z += fast_exp2(fmaf(xv, kk, c)); };
   if (tid < kWave) {
-    add(r.h);
-    add(r.t);
+    add(r.h());
+    add(r.t());
   }
   float bar = 0.f;
   for (int64_t v0 = 0;; v0 += NT * KREG) {
+    const int left = (int)(g.nvec - v0);
 #pragma unroll
     for (int j = 0; j < KREG; ++j) {
-      if (v0 + tid + j * NT < g.nvec) {
+      if (tid + j * NT < left) {
         forget(r.v[j]);
         float m = -__builtin_inff();
 #pragma unroll
@@ -198,17 +199,18 @@ __global__ __launch_bounds__(NT) void top_logits_kernel(const VocabRows a, int k
       if (two) sh.group[NT + tid] = top_key(m1);
       __syncthreads();
       if (tid < kWave) {
-        const int n = two ? 2 * NT : NT;
-        uint32_t key[2 * NT / kWave];
+        uint32_t key[NT / kWave];
 #pragma unroll
-        for (int i = 0; i < 2 * NT / kWave; ++i) key[i] = i * kWave < n ? sh.group[i * kWave + tid] : 0u;
+        for (int i = 0; i < NT / kWave; ++i) key[i] = sh.group[i * kWave + tid];
         uint32_t t = 0;
         const int enough = k + k / 8 + 4;
         for (int bit = 31; bit >= 0; --bit) {
           const uint32_t cnd = t | (1u << bit);
           int cnt = 0;
 #pragma unroll
-          for (int i = 0; i < 2 * NT / kWave; ++i) cnt += (int)__popcll(__ballot(key[i] >= cnd));
+          for (int i = 0; i < NT / kWave; ++i) cnt += (int)__popcll(__ballot(key[i] >= cnd));
+          if (two)
+            for (int i = 0; i < NT / kWave; ++i) cnt += (int)__popcll(__ballot(sh.group[NT + i * kWave + tid] >= cnd));
           if (cnt >= k) {
             t = cnd;
             if (cnt <= enough) break;
@@ -220,33 +222,33 @@ __global__ __launch_bounds__(NT) void top_logits_kernel(const VocabRows a, int k
       bar = sh.bar;
     }
     // candidates among the registers (and the end elements, with the first piece)
-    auto take = [&](float xv, int64_t i) {
+    auto take = [&](float xv, int i) {
       if (xv >= bar) {
         const int at = atomicAdd(&sh.n, 1);
         if (at < kTopCand) sh.cand[at] = ((uint64_t)top_key(xv) << 32) | (uint32_t)~(uint32_t)i;
       }
     };
     if (v0 == 0) {
-      if (tid < g.head) take(r.h, tid);
-      if (g.tail0 + tid < V) take(r.t, g.tail0 + tid);
+      if (tid < g.head) take(r.h(), tid);
+      if (g.tail0 + tid < V) take(r.t(), (int)g.tail0 + tid);
     }
     if (fmaxf(m0, m1) >= bar) {
 #pragma unroll
       for (int j = 0; j < KREG; ++j) {
-        const int64_t v = v0 + tid + j * NT;
-        if (v < g.nvec) {
+        if (tid + j * NT < left) {
           forget(r.v[j]);
+          const int e0 = g.head + ((int)v0 + tid + j * NT) * VEC;
 #pragma unroll
-          for (int i = 0; i < VEC; ++i) take(to_f32(r.v[j].v[i]), g.head + v * VEC + i);
+          for (int i = 0; i < VEC; ++i) take(to_f32(r.v[j].v[i]), e0 + i);
         }
+        __builtin_amdgcn_sched_barrier(0);
       }
     }
-    if (v0 + NT * KREG >= g.nvec) break;
+    if (left <= NT * KREG) break;
+    const int next = left - NT * KREG < NT * KREG ? left - NT * KREG : NT * KREG;
+    const VecBuffer piece = vec_buffer(x + g.head + (v0 + NT * KREG) * VEC, next);
 #pragma unroll
-    for (int j = 0; j < KREG; ++j) {
-      const int64_t v = v0 + NT * KREG + tid + j * NT;
-      if (v < g.nvec) r.v[j] = load16_stream(x + g.head + v * VEC);
-    }
+    for (int j = 0; j < KREG; ++j) r.v[j] = vec_load<T>(piece, tid + j * NT);
     m0 = m1 = -__builtin_inff();
     __syncthreads();
     const int n = sh.n;
@@ -256,7 +258,7 @@ __global__ __launch_bounds__(NT) void top_logits_kernel(const VocabRows a, int k
       top_refine<NT>(sh, n, k);
     }
   }
-  const RowSum s = rowsum_block<NT / kWave, kSumMean>(c, z, s_a, sh.sums);
+  const RowSum s = rowsum_block<NT / kWave, kSumOnly>(c, z, 0.f, sh.sums);
   __syncthreads();
   int n = sh.n;
   if (!s.ok || n > kTopCand) {
@@ -264,7 +266,7 @@ __global__ __launch_bounds__(NT) void top_logits_kernel(const VocabRows a, int k
     top_row_walked<T, NT>(a, row, x, k, values, indices, lse, sh);
     return;
   }
-  if (tid == 0 && lse) lse[row] = -rowsum_log_prob<true>(a, s, 0.f).hi;  // the log probability of a logit of 0
+  if (tid == 0 && lse) lse[row] = -rowsum_log_prob<false>(a, s, 0.f).hi;  // the log probability of a logit of 0
   if (n > 2 * kTopMax) {
     __syncthreads();
     top_refine<NT>(sh, n, k);
@@ -275,6 +277,13 @@ __global__ __launch_bounds__(NT) void top_logits_kernel(const VocabRows a, int k
 
 // ---- distillation from a teacher's largest logits ----------------------------------
 
+// A row's teacher: sum p ln p over its entries (and of the rest r = 1 - sum p,
+// r ln r), the probabilities' whole sum, and r.
+struct TopTeacher {
+  double p_ln_p;
+  float whole, rest;
+};
+
 struct TopDistilArgs {
   VocabRows r;
   const void* t_values;
@@ -283,8 +292,10 @@ struct TopDistilArgs {
   const float* t_lse;  // null: the kept entries' probabilities are normalised among themselves
   int k;
   const uint8_t* mask;  // may be null
-  const int* live;      // number of rows of the mask, or null: counted by every workgroup
   float gscale;         // weight * T
+  int* live;            // rows of the mask
+  TopTeacher* teacher;  // per row
+  float* entry_p;       // per entry: the probability of all the row's entries for its token; -1 if absent or not the first of them
   double* row_loss;
   void* grad;  // may be null
 };
@@ -295,70 +306,128 @@ __device__ __forceinline__ float top_value(const void* v, int dtype, int64_t i) 
   return to_f32(reinterpret_cast<const f16_t*>(v)[i]);
 }
 
-// The teacher's entries of a row, NE a thread, and what the row's terms need of
-// them.  Probabilities are taken in 64 bits: what the teacher leaves to all other
-// tokens is one minus their sum.
-template <int NE>
-struct TopEntries {
-  int idx[NE];  // -1: absent
-  float x[NE];  // the student's logit
-  double lp[NE], p[NE];
-  float p_all[NE];  // of all entries that name this token
-  bool first[NE];   // the first to name it
-};
+__device__ __forceinline__ double wave_sum_f64(double v) {
+#pragma unroll
+  for (int off = kWave / 2; off > 0; off >>= 1) v += __shfl_xor(v, off, kWave);
+  return v;
+}
+
+// Everything that depends on the teacher alone, in 64 bits (what the teacher
+// leaves to all other tokens is one minus a sum), one wavefront per row.  In a
+// launch of its own because these few numbers per row would otherwise set the
+// registers, and with them the occupancy, of the kernel that holds the
+// student's row.  The last workgroup counts the mask.
+constexpr int kTeacherBlock = 256;
+
+__global__ __launch_bounds__(kTeacherBlock) void top_teacher_kernel(const TopDistilArgs a) {
+  constexpr int NE = kTopMax / kWave;
+  __shared__ __align__(16) int ent_idx[kTeacherBlock / kWave][kTopMax];
+  __shared__ float ent_p[kTeacherBlock / kWave][kTopMax];
+  __shared__ float lds_f[kTeacherBlock / kWave];
+  if (blockIdx.x == gridDim.x - 1) {
+    const float n = a.mask ? mask_count_block<kTeacherBlock>(a.mask, a.r.n_rows, lds_f) : (float)a.r.n_rows;
+    if (threadIdx.x == 0) *a.live = (int)n;
+    return;
+  }
+  const int w = threadIdx.x / kWave, lane = threadIdx.x % kWave, k = a.k;
+  const int64_t row = (int64_t)blockIdx.x * (kTeacherBlock / kWave) + w;
+  const bool on = row < a.r.n_rows && !(a.mask && a.mask[row] == 0);
+  int idx[NE];
+  double lp[NE];
+  float p[NE];
+  float m = kVrLowest;
+#pragma unroll
+  for (int i = 0; i < NE; ++i) {
+    const int at = lane + i * kWave;
+    idx[i] = -1;
+    float v = 0.f;
+    if (on && at < k) {
+      const int j = a.t_indices[row * k + at];
+      if (j >= 0 && j < a.r.V) {
+        idx[i] = j;
+        v = top_value(a.t_values, a.t_dtype, row * k + at);
+        m = fmaxf(m, v);
+      }
+    }
+    lp[i] = (double)v;
+  }
+  m = wave_max(m);
+  double off = 0.0;
+  if (a.t_lse) {
+    if (on) off = (double)a.t_lse[row];
+  } else {
+    double z = 0.0;
+#pragma unroll
+    for (int i = 0; i < NE; ++i)
+      if (idx[i] >= 0) z += exp((lp[i] - (double)m) * a.r.inv_T);
+    off = (double)m * a.r.inv_T + log(wave_sum_f64(z));
+  }
+  double sum = 0.0, p_ln_p = 0.0;
+#pragma unroll
+  for (int i = 0; i < NE; ++i) {
+    const bool none = idx[i] < 0 || lp[i] == -__builtin_inf();
+    lp[i] = lp[i] * a.r.inv_T - off;
+    const double pd = none ? 0.0 : exp(lp[i]);
+    p[i] = (float)pd;
+    sum += pd;
+    // with p as it was rounded, so that p ln p - p ln q keeps its difference's accuracy
+    if (!none && p[i] != 0.f) p_ln_p += (double)p[i] * lp[i];
+    ent_idx[w][lane + i * kWave] = idx[i];
+    ent_p[w][lane + i * kWave] = p[i];
+  }
+  sum = wave_sum_f64(sum);
+  p_ln_p = wave_sum_f64(p_ln_p);
+  __syncthreads();
+  // the same token named twice: the first naming stands for all of them.  Every entry is compared with
+  // all others, four at a read (one at a time this took 21 us for 1024 rows of 128 entries).
+  float all[NE];
+  bool first[NE];
+#pragma unroll
+  for (int i = 0; i < NE; ++i) {
+    all[i] = 0.f;
+    first[i] = idx[i] >= 0;
+  }
+#pragma unroll 4
+  for (int q0 = 0; q0 < k; q0 += 4) {  // (entries from k on are absent)
+    const int4 other = *reinterpret_cast<const int4*>(&ent_idx[w][q0]);
+    const int o[4] = {other.x, other.y, other.z, other.w};
+#pragma unroll
+    for (int i = 0; i < NE; ++i) {
+      if (i * kWave >= k) break;  // uniform
+      const bool any = idx[i] == o[0] || idx[i] == o[1] || idx[i] == o[2] || idx[i] == o[3];
+      if (any && idx[i] >= 0) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          if (o[q] == idx[i]) {
+            first[i] = first[i] && q0 + q >= lane + i * kWave;
+            all[i] += ent_p[w][q0 + q];
+          }
+      }
+    }
+  }
+  int distinct = 0;
+#pragma unroll
+  for (int i = 0; i < NE; ++i) {
+    const int at = lane + i * kWave;
+    if (on && at < k) a.entry_p[row * k + at] = first[i] ? all[i] : -1.f;
+    distinct += first[i];
+  }
+#pragma unroll
+  for (int o = kWave / 2; o > 0; o >>= 1) distinct += __shfl_xor(distinct, o, kWave);
+  if (!on || lane != 0) return;
+  // (nothing is left over where every token has an entry)
+  const float rest = a.t_lse && distinct < a.r.V ? (float)fmax(1.0 - sum, 0.0) : 0.f;
+  if (rest > 0.f) p_ln_p += (double)rest * log((double)rest);
+  a.teacher[row] = TopTeacher{p_ln_p, (float)(sum + (double)rest), rest};
+}
 
 template <int NT>
 struct TopDistilShared {
-  int idx[kTopMax];
-  float p[kTopMax];
   RowSum sums[NT / kWave];
   VocabStat stats[NT / kWave];
   double d[NT / kWave];
-  float f[NT / kWave];
   float go;  // factor of the other tokens' probabilities
-  double P;
 };
-
-template <int NT, int NE>
-__device__ __forceinline__ double top_entry_probs(const TopDistilArgs& a, int64_t row, TopEntries<NE>& e, float (&v)[NE],
-                                                  TopDistilShared<NT>& sh) {
-  constexpr int NW = NT / kWave;
-  double sum = 0.0;
-  if (a.t_lse) {
-    const double lse = (double)a.t_lse[row];
-#pragma unroll
-    for (int i = 0; i < NE; ++i) e.lp[i] = (double)v[i] * a.r.inv_T - lse;
-  } else {
-    float m = kVrLowest;
-#pragma unroll
-    for (int i = 0; i < NE; ++i)
-      if (e.idx[i] >= 0) m = fmaxf(m, v[i]);
-    m = wave_max(m);
-    if (NW > 1) {
-      if (threadIdx.x % kWave == 0) sh.f[threadIdx.x / kWave] = m;
-      __syncthreads();
-      m = sh.f[threadIdx.x % NW];
-#pragma unroll
-      for (int off = NW / 2; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off, kWave));
-    }
-    double z = 0.0;
-#pragma unroll
-    for (int i = 0; i < NE; ++i) {
-      e.lp[i] = ((double)v[i] - (double)m) * a.r.inv_T;
-      if (e.idx[i] >= 0) z += exp(e.lp[i]);
-    }
-    const double lz = log(block_sum_f64<NW>(z, sh.d));
-#pragma unroll
-    for (int i = 0; i < NE; ++i) e.lp[i] -= lz;
-  }
-#pragma unroll
-  for (int i = 0; i < NE; ++i) {
-    e.p[i] = 0.0;
-    if (e.idx[i] >= 0 && v[i] != -__builtin_inff()) e.p[i] = exp(e.lp[i]);
-    sum += e.p[i];
-  }
-  return block_sum_f64<NW>(sum, sh.d);
-}
 
 // Bit of element j in the marks: vector v of the row owns bits 8 + v * VEC on, so
 // that a vector's marks are one byte (or half of one).
@@ -366,7 +435,7 @@ __device__ __forceinline__ uint32_t top_mark_bit(int j, const VocabGeom& g) { re
 
 // KREG = 0: the row is walked for its sums and again for its gradient.
 template <typename T, int NT, int KREG, bool TAIL>
-__global__ __launch_bounds__(NT) void top_distil_kernel(const TopDistilArgs a) {
+__global__ __launch_bounds__(NT, (KREG > 8 ? 4 : NT > 256 ? (NT > 512 ? 8 : 6) : 1)) void top_distil_kernel(const TopDistilArgs a) {
   constexpr int NW = NT / kWave, NE = (kTopMax + NT - 1) / NT, VEC = Vec16<T>::N;
   extern __shared__ uint32_t marks[];  // TAIL: a bit per vocabulary entry
   __shared__ TopDistilShared<NT> sh;
@@ -380,95 +449,69 @@ __global__ __launch_bounds__(NT) void top_distil_kernel(const TopDistilArgs a) {
   }
   const T* x = vocab_row<T>(a.r, row);
   const VocabGeom g = vocab_geom(x, V);
+  const float kk = a.r.k;
   RowRegs<T, NT, KREG ? KREG : 1> r;
-  if constexpr (KREG > 0) regs_load(r, x, V, g);
-
-  TopEntries<NE> e;
-  float v[NE];
+  int idx[NE];
+  float p[NE];  // the teacher's probability of the token
+  T xe[NE];     // the student's logit
+  auto ex = [&](int i) { return to_f32(xe[i]); };
 #pragma unroll
   for (int i = 0; i < NE; ++i) {
     const int at = tid + i * NT;
-    e.idx[i] = -1;
-    e.x[i] = 0.f;
-    v[i] = 0.f;
+    p[i] = -1.f;
+    idx[i] = -1;
     if (at < k) {
-      const int j = a.t_indices[row * k + at];
-      if (j >= 0 && j < V) {
-        e.idx[i] = j;
-        e.x[i] = to_f32(x[j]);
-        v[i] = top_value(a.t_values, a.t_dtype, row * k + at);
-      }
+      p[i] = a.entry_p[row * k + at];
+      idx[i] = a.t_indices[row * k + at];
     }
   }
-  if (TAIL)
-    for (int64_t i = tid; i < (V + 8 + 31) / 32; i += NT) marks[i] = 0u;
-  const double p_sum = top_entry_probs<NT, NE>(a, row, e, v, sh);
+  if constexpr (KREG > 0) regs_load(r, x, V, g);
 #pragma unroll
-  for (int i = 0; i < NE; ++i) {
-    const int at = tid + i * NT;
-    if (at < kTopMax) {
-      sh.idx[at] = e.idx[i];
-      sh.p[at] = (float)e.p[i];
-    }
-  }
-  __syncthreads();
-  // the same token named twice: the first naming stands for all of them
-  double distinct = 0.0;
+  for (int i = 0; i < NE; ++i)
+    if (p[i] < 0.f) idx[i] = -1;
 #pragma unroll
-  for (int i = 0; i < NE; ++i) {
-    e.first[i] = e.idx[i] >= 0;
-    e.p_all[i] = 0.f;
-    if (e.idx[i] >= 0) {
-      const int at = tid + i * NT;
-      for (int q = 0; q < k; ++q) {
-        const bool same = sh.idx[q] == e.idx[i];
-        e.first[i] = e.first[i] && !(same && q < at);
-        e.p_all[i] += same ? sh.p[q] : 0.f;
-      }
-      if (TAIL) {
-        const uint32_t bit = top_mark_bit(e.idx[i], g);
+  for (int i = 0; i < NE; ++i) xe[i] = x[idx[i] >= 0 ? idx[i] : 0];
+  if (TAIL) {
+    for (int i = tid; i < (int)((V + 8 + 31) / 32); i += NT) marks[i] = 0u;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < NE; ++i)
+      if (idx[i] >= 0) {
+        const uint32_t bit = top_mark_bit(idx[i], g);
         atomicOr(&marks[bit >> 5], 1u << (bit & 31));
       }
-      distinct += e.first[i] ? 1.0 : 0.0;
-    }
+    __syncthreads();
   }
-  const float n_live = a.live ? (float)*a.live
-                              : a.mask ? mask_count_block<NT>(a.mask, a.r.n_rows, sh.f) : (float)a.r.n_rows;
-  const bool covered = TAIL && block_sum_f64<NW>(distinct, sh.d) == (double)V;
-  __syncthreads();
-  const float gs = a.gscale / n_live, kk = a.r.k;
-
-  // Loss and gradient factors from the student's sums: lq(x) = ln of its probability of a logit x, and
-  // with TAIL the part q_rest of its probability that lies outside the kept entries.
-  auto finish = [&](auto lq, double lq_rest, double inv_q_rest) {
+  const TopTeacher t = scalar_load(a.teacher + row);
+  const float gs = a.gscale / (float)scalar_load(a.live);
+  // Loss and gradient factor from the student's sums: lq(x) = ln of its probability of a logit x, and
+  // with TAIL the ln of what it leaves to the tokens without an entry, and one over that.
+  auto finish = [&](auto lq, Float2x lq_rest, float inv_q_rest) {
     double term = 0.0;
 #pragma unroll
     for (int i = 0; i < NE; ++i)
-      if (e.idx[i] >= 0 && !(e.p[i] == 0.0)) term += e.p[i] * (e.lp[i] - lq(e.x[i]));
+      if (idx[i] >= 0 && !(p[i] == 0.f)) {
+        const Float2x l = lq(ex(i));
+        term -= (double)p[i] * ((double)l.hi + (double)l.lo);
+      }
     term = block_sum_f64<NW>(term, sh.d);
     if (tid == 0) {
-      double P = p_sum, outside = p_sum;
-      if (TAIL) {
-        const double rest = covered ? 0.0 : fmax(1.0 - p_sum, 0.0);
-        P += rest;
-        outside = P;
-        if (rest > 0.0) {
-          term += rest * (log(rest) - lq_rest);
-          if (inv_q_rest < __builtin_inf()) outside -= rest * inv_q_rest;
-        }
+      term += t.p_ln_p;
+      float outside = t.whole;
+      if (TAIL && t.rest > 0.f) {
+        term -= (double)t.rest * ((double)lq_rest.hi + (double)lq_rest.lo);
+        if (inv_q_rest < __builtin_inff()) outside = fmaf(-t.rest, inv_q_rest, outside);
       }
       a.row_loss[row] = term;
-      sh.go = (float)((double)gs * outside);
-      sh.P = P;
+      sh.go = gs * outside;
     }
     __syncthreads();
   };
   auto patch = [&](auto q_of) {  // the kept entries' gradients replace what the walk over the row wrote
     __syncthreads();
-    const float P = (float)sh.P;
 #pragma unroll
     for (int i = 0; i < NE; ++i)
-      if (e.first[i]) grow[e.idx[i]] = from_f32<T>(gs * (q_of(e.x[i]) * P - e.p_all[i]));
+      if (idx[i] >= 0) grow[idx[i]] = from_f32<T>(gs * fmaf(q_of(ex(i)), t.whole, -p[i]));
   };
 
   if constexpr (KREG > 0) {
@@ -478,8 +521,8 @@ __global__ __launch_bounds__(NT) void top_distil_kernel(const TopDistilArgs a) {
       float out = 0.f, in = 0.f;
       const uint8_t* mark8 = reinterpret_cast<const uint8_t*>(marks);
       auto marked = [&](uint32_t bit) { return ((marks[bit >> 5] >> (bit & 31)) & 1u) != 0; };
-      if (tid < g.head && !marked(top_mark_bit(tid, g))) out += fast_exp2(fmaf(r.h, kk, c));
-      if (g.tail0 + tid < V && !marked(top_mark_bit((int)g.tail0 + tid, g))) out += fast_exp2(fmaf(r.t, kk, c));
+      if (tid < g.head && !marked(top_mark_bit(tid, g))) out += fast_exp2(fmaf(r.h(), kk, c));
+      if (g.tail0 + tid < V && !marked(top_mark_bit((int)g.tail0 + tid, g))) out += fast_exp2(fmaf(r.t(), kk, c));
 #pragma unroll
       for (int j = 0; j < KREG; ++j) {
         const int vv = tid + j * NT;
@@ -489,37 +532,27 @@ __global__ __launch_bounds__(NT) void top_distil_kernel(const TopDistilArgs a) {
           const uint32_t m = mark8[bit0 >> 3] >> (bit0 & 7u);
 #pragma unroll
           for (int i = 0; i < VEC; ++i) {
-            const float ex = fast_exp2(fmaf(to_f32(r.v[j].v[i]), kk, c));
-            out += (m >> i) & 1u ? 0.f : ex;
+            const float e = fast_exp2(fmaf(to_f32(r.v[j].v[i]), kk, c));
+            out += (m >> i) & 1u ? 0.f : e;
           }
         }
         __builtin_amdgcn_sched_barrier(0);
       }
 #pragma unroll
       for (int i = 0; i < NE; ++i)
-        if (e.first[i]) in += fast_exp2(fmaf(e.x[i], kk, c));
+        if (idx[i] >= 0) in += fast_exp2(fmaf(ex(i), kk, c));
       // (a wavefront of nothing but -inf has no exponent of its own to take entries by)
       if (!(c < kVrNoTerm) && in > 0.f) in = __builtin_inff();
       s = rowsum_block<NW, kSumSecond>(c, out, in, sh.sums);
-      s.ok = s.ok && (covered || s.z > 1e-30f);
+      s.ok = s.ok && (t.rest == 0.f || s.z > 1e-30f);
     } else {
       s = regs_sum<T, NT, KREG>(r, g, kk, sh.sums);
     }
     if (s.ok) {
       const float rest_z = s.z;
       if (TAIL) s.z += s.a;
-      double lq_rest = 0.0, inv_q_rest = 0.0;
-      if (TAIL && !covered) {
-        const Float2x lo = log2_2x(rest_z), la = log2_2x(s.z);
-        lq_rest = kVrLn2 * (((double)lo.hi - (double)la.hi) + ((double)lo.lo - (double)la.lo));
-        inv_q_rest = (double)s.z / (double)rest_z;
-      }
-      finish(
-          [&](float xv) {
-            const Float2x l = rowsum_log_prob<false>(a.r, s, xv);
-            return (double)l.hi + (double)l.lo;
-          },
-          lq_rest, inv_q_rest);
+      finish([&](float xv) { return rowsum_log_prob<false>(a.r, s, xv); },
+             TAIL ? ln_share(log2_2x(rest_z), s.z) : Float2x{0.f, 0.f}, s.z / rest_z);
       if (!grow) return;
       const float rz = 1.f / s.z, go = sh.go * rz, c = s.c;
       regs_map(r, g, x, grow, V, -1, [=](float xv) { return go * fast_exp2(fmaf(xv, kk, c)); }, [](float) { return 0.f; });
@@ -540,18 +573,26 @@ __global__ __launch_bounds__(NT) void top_distil_kernel(const TopDistilArgs a) {
     VocabStat in = vstat_init();
 #pragma unroll
     for (int i = 0; i < NE; ++i)
-      if (e.first[i]) {
-        float x1[1] = {e.x[i]};
+      if (idx[i] >= 0) {
+        float x1[1] = {ex(i)};
         vstat_fold<1>(in, x1, kk);
       }
     all = vstat_merge(out, vstat_block<NW>(in, kk, sh.stats), kk);
   } else {
     all = vstat_block<NW>(vocab_stat_walk<T, NT>(x, V, kk), kk, sh.stats);
   }
-  const double log2z = vstat_log2z(all, a.r.k_rel);
-  const double lq_rest =
-      TAIL ? ((double)out.m - (double)all.m) * a.r.inv_T + kVrLn2 * (vstat_log2z(out, a.r.k_rel) - log2z) : 0.0;
-  finish([&](float xv) { return ((double)xv - (double)all.m) * a.r.inv_T - kVrLn2 * log2z; }, lq_rest, exp(-lq_rest));
+  // the rest's share: its sum, moved to the row's maximum, which may underflow where its logarithm does not
+  Float2x lq_rest{0.f, 0.f};
+  float inv_q_rest = 0.f;
+  if (TAIL) {
+    const Float2x d = two_sum(out.m, -all.m), e = two_mul(d.hi, kk), l = log2_2x(out.z), h = two_sum(e.hi, l.hi);
+    if (out.z > 0.f || out.z != out.z)
+      lq_rest = ln_share(Float2x{h.hi, h.lo + (l.lo + (e.lo + d.lo * kk))}, all.z);
+    else
+      lq_rest.hi = -__builtin_inff();
+    inv_q_rest = fast_exp2(-e.hi) * (all.z / out.z);
+  }
+  finish([&](float xv) { return vstat_log_prob(a.r, all, xv); }, lq_rest, inv_q_rest);
   if (!grow) return;
   const float rz = 1.f / all.z, go = sh.go * rz, m = all.m;
   vocab_map_walk<T, NT>(x, grow, V, [=](float xv, int) { return go * fast_exp2((xv - m) * kk); });
@@ -559,19 +600,11 @@ __global__ __launch_bounds__(NT) void top_distil_kernel(const TopDistilArgs a) {
 }
 
 __global__ __launch_bounds__(1024) void top_distil_sum_kernel(const double* __restrict__ v, int64_t n,
-                                                              const uint8_t* __restrict__ mask, double scale,
+                                                              const int* __restrict__ live, double scale,
                                                               float* __restrict__ out) {
   __shared__ double lds[1024 / kWave];
-  __shared__ float lds_f[1024 / kWave];
-  const float live = mask ? mask_count_block<1024>(mask, n, lds_f) : (float)n;
   const double s = block_sum_f64<1024 / kWave>(thread_share_of_sum_f64<1024>(v, n), lds);
-  if (threadIdx.x == 0) *out = live > 0.f ? (float)(scale * s / (double)live) : __builtin_nanf("");
-}
-
-__global__ __launch_bounds__(1024) void top_live_kernel(const uint8_t* __restrict__ mask, int64_t n, int* __restrict__ out) {
-  __shared__ float lds[1024 / kWave];
-  const float live = mask_count_block<1024>(mask, n, lds);
-  if (threadIdx.x == 0) *out = (int)live;
+  if (threadIdx.x == 0) *out = *live > 0 ? (float)(scale * s / (double)*live) : __builtin_nanf("");
 }
 
 template <typename T>
@@ -615,20 +648,21 @@ int launch_top_distil_shape(const TopDistilArgs& a, hipStream_t st) {
 }
 
 template <typename T>
-int launch_top_distil(TopDistilArgs a, int* live, double loss_scale, float* loss_out, hipStream_t st) {
-  int rc = TS_OK;
-  if (a.mask && a.r.n_rows > kTopSelfCountRows) {
-    hipLaunchKernelGGL(top_live_kernel, dim3(1), dim3(1024), 0, st, a.mask, a.r.n_rows, live);
-    rc = check_launch();
-    if (rc) return rc;
-    a.live = live;
-  }
+int launch_top_distil(const TopDistilArgs& a, double loss_scale, float* loss_out, hipStream_t st) {
+  constexpr int64_t kRows = kTeacherBlock / kWave;
+  hipLaunchKernelGGL(top_teacher_kernel, dim3((unsigned)((a.r.n_rows + kRows - 1) / kRows + 1)), dim3(kTeacherBlock), 0,
+                     st, a);
+  int rc = check_launch();
+  if (rc) return rc;
   if (a.r.n_rows > 0) rc = a.t_lse ? launch_top_distil_shape<T, true>(a, st) : launch_top_distil_shape<T, false>(a, st);
   if (rc) return rc;
-  hipLaunchKernelGGL(top_distil_sum_kernel, dim3(1), dim3(1024), 0, st, a.row_loss, a.r.n_rows, a.mask, loss_scale,
+  hipLaunchKernelGGL(top_distil_sum_kernel, dim3(1), dim3(1024), 0, st, a.row_loss, a.r.n_rows, a.live, loss_scale,
                      loss_out);
   return check_launch();
 }
+
+// Workspace: live count (16 bytes), loss terms and teacher numbers per row, probabilities per entry.
+inline size_t top_ws_bytes(int64_t n_rows, int64_t k) { return 16 + (size_t)n_rows * (8 + 16) + (size_t)(n_rows * k) * 4; }
 
 }  // namespace ts
 
@@ -650,7 +684,9 @@ int ts_top_logits(const void* s, int64_t n_seq, int64_t seq_len, int64_t V, int6
   TS_BY_DTYPE(dtype, (ts::launch_top_logits<T>(a, k, values, indices, logsumexp, st)))
 }
 
-size_t ts_top_distil_workspace_bytes(int64_t n_rows) { return n_rows < 0 ? 0 : 16 + (size_t)n_rows * 8; }
+size_t ts_top_distil_workspace_bytes(int64_t n_rows, int k) {
+  return n_rows < 0 || k < 0 ? 0 : ts::top_ws_bytes(n_rows, k);
+}
 
 int ts_top_distil_fwd_bwd(const void* s, int64_t n_seq, int64_t seq_len, int64_t V, int64_t ld_seq, int64_t ld_tok,
                           const void* t_values, int t_dtype, const int32_t* t_indices, const float* t_logsumexp, int k,
@@ -674,12 +710,15 @@ int ts_top_distil_fwd_bwd(const void* s, int64_t n_seq, int64_t seq_len, int64_t
   a.k = k;
   a.mask = row_mask;
   a.gscale = (float)(weight * temperature);
-  a.live = nullptr;
-  a.row_loss = reinterpret_cast<double*>((char*)workspace + 16);
+  char* ws = reinterpret_cast<char*>(workspace);
+  a.live = reinterpret_cast<int*>(ws);
+  a.teacher = reinterpret_cast<ts::TopTeacher*>(ws + 16);
+  a.row_loss = reinterpret_cast<double*>(ws + 16 + a.r.n_rows * 16);
+  a.entry_p = reinterpret_cast<float*>(ws + 16 + a.r.n_rows * 24);
   a.grad = grad;
   const double scale = weight * temperature * temperature;
   hipStream_t st = (hipStream_t)stream;
-  TS_BY_DTYPE(dtype, (ts::launch_top_distil<T>(a, reinterpret_cast<int*>(workspace), scale, loss_out, st)))
+  TS_BY_DTYPE(dtype, (ts::launch_top_distil<T>(a, scale, loss_out, st)))
 }
 
 }  // extern "C"

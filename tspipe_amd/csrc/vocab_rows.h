@@ -56,42 +56,79 @@ inline int vocab_rows_status(const void* s, int64_t n_seq, int64_t seq_len, int6
   return TS_OK;
 }
 
+// The row's address, the same in every lane of the wavefront: said to the
+// compiler, whose 64-bit division leaves it in vector registers, so that it and
+// all that follows from it stay scalar.
 template <typename T>
 __device__ __forceinline__ const T* vocab_row(const VocabRows& a, int64_t row) {
-  const int64_t q = row / a.seq_len;
-  return reinterpret_cast<const T*>(a.s) + q * a.ld_seq + (row - q * a.seq_len) * a.ld_tok;
+  const uint32_t q = (uint32_t)row / (uint32_t)a.seq_len;  // fewer than 2^22 rows
+  const T* p = reinterpret_cast<const T*>(a.s) + q * a.ld_seq + (row - (int64_t)q * a.seq_len) * a.ld_tok;
+  const uint64_t b = (uint64_t)p;
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)b);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(b >> 32));
+  return reinterpret_cast<const T*>(((uint64_t)hi << 32) | lo);
 }
 
-// m = max x, z = sum 2^((x - m) k), a = sum 2^((x - m) k) (x - m) k
-struct VocabStat {
-  float m, z, a;
+// An fp32 number and what its rounding left out.  The log probabilities of a row
+// are formed in this type: a sum over a sequence of them, or the difference of
+// two that nearly agree, would show the last bits of fp32, and 64-bit
+// logarithms and exponentials in a kernel that holds a row in registers spill
+// (28 % of the policy loss's time at 8192 x 65536 bf16).
+struct Float2x {
+  float hi, lo;
 };
 
-__device__ __forceinline__ VocabStat vstat_init() { return VocabStat{kVrLowest, 0.f, 0.f}; }
+__device__ __forceinline__ Float2x two_sum(float x, float y) {
+#pragma clang fp contract(off)
+  const float s = x + y, v = s - x;
+  return Float2x{s, (x - (s - v)) + (y - v)};
+}
+
+__device__ __forceinline__ Float2x two_mul(float x, float y) {
+#pragma clang fp contract(off)
+  const float p = x * y;
+  return Float2x{p, __builtin_fmaf(x, y, -p)};
+}
+
+// log2(z) within 2e-7 for normal z > 0 (-inf for 0): the hardware's logarithm, corrected by what
+// its own power of two leaves of z.
+__device__ __forceinline__ Float2x log2_2x(float z) {
+  if (!(z > 0.f && z < __builtin_inff())) return Float2x{__builtin_amdgcn_logf(z), 0.f};
+  const float e = (float)(__builtin_amdgcn_frexp_expf(z));  // z = f 2^e, f in [1/2, 1)
+  const float f = __builtin_amdgcn_frexp_mantf(z);
+  const float l = __builtin_amdgcn_logf(f);
+  const Float2x s = two_sum(e, l);
+  return Float2x{s.hi, s.lo + kVrLog2e * fmaf(f, fast_exp2(-l), -1.f)};
+}
+
+// ln 2 times (e - log2 z): the log probability of a term 2^e of a sum z.
+__device__ __forceinline__ Float2x ln_share(Float2x e, float z) {
+#pragma clang fp contract(off)
+  const Float2x l = log2_2x(z), h = two_sum(e.hi, -l.hi);
+  if (!(__builtin_fabsf(h.hi) < __builtin_inff())) return Float2x{h.hi, 0.f};  // a logit of -inf
+  const float lo = e.lo + (h.lo - l.lo);
+  const Float2x m = two_mul(h.hi, 0.693147182464599609375f);
+  return two_sum(m.hi, m.lo + (lo * 0.693147182464599609375f + h.hi * -1.904654323e-09f));
+}
+
+// m = max x, z = sum 2^((x - m) k)
+struct VocabStat {
+  float m, z;
+};
+
+__device__ __forceinline__ VocabStat vstat_init() { return VocabStat{kVrLowest, 0.f}; }
 
 // The state re-based onto the larger maximum m.
 __device__ __forceinline__ VocabStat vstat_rebase(VocabStat s, float m, float k) {
-  const float d = fmaxf((s.m - m) * k, -1e30f);  // finite, so that an empty state stays 0 and not 0 * inf
-  const float r = fast_exp2(d);
-  return VocabStat{m, s.z * r, r * fmaf(s.z, d, s.a)};
+  return VocabStat{m, s.z * fast_exp2((s.m - m) * k)};
 }
 
 __device__ __forceinline__ VocabStat vstat_merge(VocabStat p, VocabStat q, float k) {
   const float m = fmaxf(p.m, q.m);
-  p = vstat_rebase(p, m, k);
-  q = vstat_rebase(q, m, k);
-  return VocabStat{m, p.z + q.z, p.a + q.a};
+  return VocabStat{m, vstat_rebase(p, m, k).z + vstat_rebase(q, m, k).z};
 }
 
-// Adds one logit to sums whose maximum is settled.  A NaN logit makes z NaN; a
-// logit of -inf (a masked vocabulary entry) adds nothing, also not to a.
-__device__ __forceinline__ void vstat_add(VocabStat& s, float x, float k) {
-  const float d = (x - s.m) * k;
-  const float e = fast_exp2(d);
-  s.z += e;
-  s.a = fmaf(e, fmaxf(d, -1e30f), s.a);
-}
-
+// A NaN logit makes z NaN; a logit of -inf (a masked vocabulary entry) adds nothing.
 template <int N>
 __device__ __forceinline__ void vstat_fold(VocabStat& s, const float (&x)[N], float k) {
   float m = s.m;
@@ -99,7 +136,7 @@ __device__ __forceinline__ void vstat_fold(VocabStat& s, const float (&x)[N], fl
   for (int i = 0; i < N; ++i) m = fmaxf(m, x[i]);
   if (m > s.m) s = vstat_rebase(s, m, k);
 #pragma unroll
-  for (int i = 0; i < N; ++i) vstat_add(s, x[i], k);
+  for (int i = 0; i < N; ++i) s.z += fast_exp2((x[i] - s.m) * k);
 }
 
 // Merged over a workgroup of NW wavefronts; every thread gets the result.
@@ -107,28 +144,41 @@ template <int NW>
 __device__ __forceinline__ VocabStat vstat_block(VocabStat s, float k, VocabStat* lds) {
 #pragma unroll
   for (int off = kWave / 2; off > 0; off >>= 1)
-    s = vstat_merge(s, VocabStat{__shfl_xor(s.m, off, kWave), __shfl_xor(s.z, off, kWave), __shfl_xor(s.a, off, kWave)}, k);
+    s = vstat_merge(s, VocabStat{__shfl_xor(s.m, off, kWave), __shfl_xor(s.z, off, kWave)}, k);
   if (NW == 1) return s;
   if (threadIdx.x % kWave == 0) lds[threadIdx.x / kWave] = s;
   __syncthreads();
-  // lane i takes state i % NW, and the lanes merge (NW states at once would need 3 NW registers a lane)
+  // lane i takes state i % NW, and the lanes merge (NW states at once would need 2 NW registers a lane)
   s = lds[threadIdx.x % NW];
 #pragma unroll
   for (int off = NW / 2; off > 0; off >>= 1)
-    s = vstat_merge(s, VocabStat{__shfl_xor(s.m, off, kWave), __shfl_xor(s.z, off, kWave), __shfl_xor(s.a, off, kWave)}, k);
+    s = vstat_merge(s, VocabStat{__shfl_xor(s.m, off, kWave), __shfl_xor(s.z, off, kWave)}, k);
   __syncthreads();  // lds may be used again
   return s;
 }
 
-// log2 of the row's sum of 2^((x - m) k_exact), in 64 bits; -inf for a row of nothing but -inf.
-__device__ __forceinline__ double vstat_log2z(const VocabStat& s, float k_rel) {
-  if (s.z == 0.f) return -__builtin_inf();
-  return log2((double)s.z) + (double)k_rel * ((double)s.a / (double)s.z);
+// ln of the soft-max probability of a logit x of the row.
+__device__ __forceinline__ Float2x vstat_log_prob(const VocabRows& r, const VocabStat& s, float x) {
+#pragma clang fp contract(off)
+  const float k = r.k;
+  const Float2x d = two_sum(x, -s.m), p = two_mul(d.hi, k);
+  if (d.hi < -1e38f && d.hi > -__builtin_inff()) return Float2x{(float)((double)d.hi * r.inv_T), 0.f};  // (d k may overflow)
+  return ln_share(Float2x{p.hi, p.lo + d.lo * k}, s.z);
 }
 
-// ln of the soft-max probability of a logit x of the row.
-__device__ __forceinline__ double vstat_log_prob(const VocabRows& a, const VocabStat& s, float x) {
-  return ((double)x - (double)s.m) * a.inv_T - kVrLn2 * vstat_log2z(s, a.k_rel);
+// A value at a uniform address that nothing writes while the kernel runs, through
+// the scalar unit: it takes no vector register, and waiting for it is no wait for
+// the row's loads.
+template <typename X>
+__device__ __forceinline__ X scalar_load(const X* p) {
+  static_assert(sizeof(X) % 4 == 0, "whole words");
+  const auto* w = (const __attribute__((address_space(4))) uint32_t*)(uint64_t)p;
+  uint32_t words[sizeof(X) / 4];
+#pragma unroll
+  for (unsigned i = 0; i < sizeof(X) / 4; ++i) words[i] = w[i];
+  X x;
+  __builtin_memcpy(&x, words, sizeof(X));
+  return x;
 }
 
 // Split of a row into scalar head, 16-byte vectors and scalar tail.
@@ -227,23 +277,71 @@ __device__ __forceinline__ void vocab_zero_row(T* grow, int64_t V) {
 // ---------------------------------------------------------------------------
 constexpr float kVrNoTerm = 1e9f;  // c of a wavefront without a finite element: its factor 2^(C - c) is 0
 
+// `count` 16-byte vectors behind a 16-byte aligned address, the same in every
+// lane.  Loads beyond them return 0 and stores beyond them do nothing (the
+// buffer's own range check), so that a thread issues all its loads with no
+// branch between them and one register of addresses; vectors that a lane does
+// not have are left out where they are used.  With predicated loads the
+// compiler kept an address and a mask for each and spilled them between the
+// loads.  All of the offset is the lane's (the range check takes a scalar
+// offset off the length first).
+struct VecBuffer {
+  __amdgpu_buffer_rsrc_t rsrc;
+};
+constexpr int kNonTemporal = 2;
+
+template <typename T>
+__device__ __forceinline__ VecBuffer vec_buffer(const T* base, int count) {
+  return VecBuffer{__builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(base), (short)0, count * 16, 0x00020000)};
+}
+template <typename T>
+__device__ __forceinline__ Vec16<T> vec_load(const VecBuffer& b, uint32_t v) {
+  const auto raw = __builtin_amdgcn_raw_buffer_load_b128(b.rsrc, (int)(v * 16u), 0, kNonTemporal);
+  Vec16<T> r;
+  __builtin_memcpy(&r, &raw, 16);
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ void vec_store(const VecBuffer& b, uint32_t v, const Vec16<T>& x) {
+  u32x4 raw;
+  __builtin_memcpy(&raw, &x, 16);
+  __builtin_amdgcn_raw_buffer_store_b128(raw, b.rsrc, (int)(v * 16u), 0, kNonTemporal);
+}
+
+// Element i of `count` (0 beyond them), as fp32.
+template <typename T>
+__device__ __forceinline__ T elem_load(const T* base, int count, uint32_t i) {
+  const VecBuffer b{__builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(base), (short)0, count * (int)sizeof(T), 0x00020000)};
+  T r;
+  if constexpr (sizeof(T) == 4) {
+    const auto raw = __builtin_amdgcn_raw_buffer_load_b32(b.rsrc, (int)(i * 4u), 0, 0);
+    __builtin_memcpy(&r, &raw, 4);
+  } else {
+    const auto raw = __builtin_amdgcn_raw_buffer_load_b16(b.rsrc, (int)(i * 2u), 0, 0);
+    __builtin_memcpy(&r, &raw, 2);
+  }
+  return r;
+}
+
 template <typename T, int NT, int KREG>
 struct RowRegs {
   Vec16<T> v[KREG];
-  float h, t;  // end elements, -inf where this thread has none
+  T head, tail;  // end elements
+  bool has_h, has_t;
+  __device__ __forceinline__ float h() const { return has_h ? to_f32(head) : -__builtin_inff(); }
+  __device__ __forceinline__ float t() const { return has_t ? to_f32(tail) : -__builtin_inff(); }
 };
 
 template <typename T, int NT, int KREG>
 __device__ __forceinline__ void regs_load(RowRegs<T, NT, KREG>& r, const T* row, int64_t V, const VocabGeom& g) {
-  constexpr int VEC = Vec16<T>::N;
+  // (the end elements without a branch as well: a wait for them inside one would be a wait for all)
+  r.has_h = (int)threadIdx.x < g.head;
+  r.has_t = g.tail0 + threadIdx.x < V;
+  r.head = elem_load(row, g.head, threadIdx.x);
+  r.tail = elem_load(row + g.tail0, (int)(V - g.tail0), threadIdx.x);
+  const VecBuffer body = vec_buffer(row + g.head, g.nvec < NT * KREG ? (int)g.nvec : NT * KREG);
 #pragma unroll
-  for (int j = 0; j < KREG; ++j) {
-    const int v = (int)threadIdx.x + j * NT;
-    if (v < (int)g.nvec) r.v[j] = load16_stream(row + g.head + (int64_t)v * VEC);
-  }
-  r.h = r.t = -__builtin_inff();
-  if ((int)threadIdx.x < g.head) r.h = to_f32(row[threadIdx.x]);
-  if (g.tail0 + threadIdx.x < V) r.t = to_f32(row[g.tail0 + threadIdx.x]);
+  for (int j = 0; j < KREG; ++j) r.v[j] = vec_load<T>(body, threadIdx.x + j * NT);
 }
 
 // Makes the compiler forget what it knows of a vector, so that each pass
@@ -261,7 +359,7 @@ __device__ __forceinline__ void forget(Vec16<T>& v) {
 template <typename T, int NT, int KREG>
 __device__ __forceinline__ float regs_anchor(const RowRegs<T, NT, KREG>& r, const VocabGeom& g, float k) {
   constexpr int VEC = Vec16<T>::N;
-  float m = fmaxf(r.h, r.t);
+  float m = fmaxf(r.h(), r.t());
   if ((int)threadIdx.x < (int)g.nvec) {
 #pragma unroll
     for (int i = 0; i < VEC; ++i) m = fmaxf(m, to_f32(r.v[0].v[i]));
@@ -319,50 +417,17 @@ __device__ __forceinline__ RowSum rowsum_block(float c, float z, float a, RowSum
   return r;
 }
 
-// An fp32 number and what its rounding left out.  The log probabilities of a row
-// are formed in this type: a sum over a sequence of them, or the difference of
-// two that nearly agree, would show the last bits of fp32, and 64-bit
-// logarithms and exponentials in a kernel that holds a row in registers spill
-// (28 % of the policy loss's time at 8192 x 65536 bf16).
-struct Float2x {
-  float hi, lo;
-};
-
-__device__ __forceinline__ Float2x two_sum(float x, float y) {
-#pragma clang fp contract(off)
-  const float s = x + y, v = s - x;
-  return Float2x{s, (x - (s - v)) + (y - v)};
-}
-
-__device__ __forceinline__ Float2x two_mul(float x, float y) {
-#pragma clang fp contract(off)
-  const float p = x * y;
-  return Float2x{p, __builtin_fmaf(x, y, -p)};
-}
-
-// log2(z), z > 0 and normal, within 2e-7: the hardware's logarithm, corrected by what
-// its own power of two leaves of z.
-__device__ __forceinline__ Float2x log2_2x(float z) {
-  const float e = (float)(__builtin_amdgcn_frexp_expf(z));  // z = f 2^e, f in [1/2, 1)
-  const float f = __builtin_amdgcn_frexp_mantf(z);
-  const float l = __builtin_amdgcn_logf(f);
-  const Float2x s = two_sum(e, l);
-  return Float2x{s.hi, s.lo + kVrLog2e * fmaf(f, fast_exp2(-l), -1.f)};
-}
-
 // ln of the soft-max probability of a logit of the row.  Without the sum a the
 // factor k stays as rounded, in the logit's own exponent too: what the rounding
 // took then counts only for the logit's distance from the row's mean.
-template <bool WITH_A>
+template <bool WITH_MEAN>
 __device__ __forceinline__ Float2x rowsum_log_prob(const VocabRows& r, const RowSum& s, float x) {
 #pragma clang fp contract(off)
-  const Float2x p = two_mul(x, r.k), q = two_sum(p.hi, s.c), l = log2_2x(s.z);
-  const Float2x h = two_sum(q.hi, -l.hi);
-  float lo = (p.lo + q.lo) + (h.lo - l.lo);
-  if (WITH_A) lo += r.k_rel * (p.hi - (s.a / s.z - s.c));  // a / z - c: mean of x k under the soft-max
-  if (!(__builtin_fabsf(h.hi) < __builtin_inff())) return Float2x{h.hi, 0.f};  // a logit of -inf
-  const Float2x m = two_mul(h.hi, 0.693147182464599609375f);
-  return two_sum(m.hi, m.lo + (lo * 0.693147182464599609375f + h.hi * -1.904654323e-09f));
+  const Float2x p = two_mul(x, r.k), q = two_sum(p.hi, s.c);
+  if (x < -1e38f && x > -__builtin_inff()) return Float2x{(float)((double)x * r.inv_T), 0.f};  // (x k may overflow)
+  float lo = p.lo + q.lo;
+  if (WITH_MEAN) lo += r.k_rel * (p.hi - (s.a / s.z - s.c));  // a / z - c: mean of x k under the soft-max
+  return ln_share(Float2x{q.hi, lo}, s.z);
 }
 
 // One thread's terms of its registers: f(x, exponent) per element.
@@ -386,8 +451,8 @@ __device__ __forceinline__ RowSum regs_sum(RowRegs<T, NT, KREG>& r, const VocabG
   float z = 0.f;
   auto add = [&](float x) { z += fast_exp2(fmaf(x, k, c)); };
   if (threadIdx.x < kWave) {  // the end elements
-    add(r.h);
-    add(r.t);
+    add(r.h());
+    add(r.t());
   }
   regs_each(r, g, add);
   return rowsum_block<NT / kWave, kSumOnly>(c, z, 0.f, lds);
@@ -400,12 +465,13 @@ __device__ __forceinline__ void regs_map(RowRegs<T, NT, KREG>& r, const VocabGeo
                                          int special, F f, G f_special) {
   constexpr int VEC = Vec16<T>::N;
   if ((int)threadIdx.x < g.head)
-    grow[threadIdx.x] = from_f32<T>((int)threadIdx.x == special ? f_special(r.h) : f(r.h));
+    grow[threadIdx.x] = from_f32<T>((int)threadIdx.x == special ? f_special(r.h()) : f(r.h()));
   const int64_t t = g.tail0 + threadIdx.x;
-  if (t < V) grow[t] = from_f32<T>((int)t == special ? f_special(r.t) : f(r.t));
+  if (t < V) grow[t] = from_f32<T>((int)t == special ? f_special(r.t()) : f(r.t()));
   const bool gvec = (((uintptr_t)grow ^ (uintptr_t)row) & 15u) == 0;
   const int sv = special >= g.head ? (special - g.head) / VEC : -1;
   const int si = special - g.head - sv * VEC;
+  const VecBuffer body = vec_buffer(grow + g.head, gvec ? (int)g.nvec : 0);
 #pragma unroll
   for (int j = 0; j < KREG; ++j) {
     const int v = (int)threadIdx.x + j * NT;
@@ -419,10 +485,10 @@ __device__ __forceinline__ void regs_map(RowRegs<T, NT, KREG>& r, const VocabGeo
         for (int i = 0; i < VEC; ++i)
           if (i == si) o.v[i] = from_f32<T>(f_special(to_f32(r.v[j].v[i])));
       }
-      T* p = grow + g.head + (int64_t)v * VEC;
       if (gvec) {
-        store16_stream(p, o);
+        vec_store(body, (uint32_t)v, o);
       } else {
+        T* p = grow + g.head + v * VEC;
 #pragma unroll
         for (int i = 0; i < VEC; ++i) p[i] = o.v[i];
       }
@@ -476,9 +542,9 @@ __device__ __forceinline__ double block_sum_f64(double v, double* lds) {
   __syncthreads();
   if (threadIdx.x % kWave == 0) lds[threadIdx.x / kWave] = v;
   __syncthreads();
-  double r = 0.0;
+  double r = lds[threadIdx.x % NW];
 #pragma unroll
-  for (int i = 0; i < NW; ++i) r += lds[i];
+  for (int off = NW / 2; off > 0; off >>= 1) r += __shfl_xor(r, off, kWave);
   return r;
 }
 

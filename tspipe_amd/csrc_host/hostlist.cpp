@@ -3,10 +3,14 @@
 // (data_ptr, numel, dtype/device/shape/contiguity checks) costs more than the
 // EMA kernel itself; here it is one call.  No GPU work happens in this module.
 #include <torch/extension.h>
+#include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/autograd/saved_variable.h>
 #include <ATen/detail/CUDAHooksInterface.h>
 
 #include <algorithm>
+#include <array>
 #include <cstdint>
 #include <vector>
 
@@ -489,6 +493,311 @@ py::object row_loss(int64_t kind, const at::Tensor& x1, const at::Tensor& y1, co
   return py::cast(loss);
 }
 
+// ---------------------------------------------------------------------------
+// The losses on rows of vocabulary logits.  Same division of labour: the entry
+// points compute, these functions own the buffers and record the gradient.
+// The graph node is written against autograd's Node directly: a node whose
+// gradient is already there has nothing to save, and Function<>'s bookkeeping
+// costs more than the kernels of a short answer.
+// Every function returns None when the call is not of the plain kind; the
+// Python function then takes it and raises the proper errors.
+// ---------------------------------------------------------------------------
+typedef int (*logp_fwd_fn)(const void*, int64_t, int64_t, int64_t, int64_t, int64_t, const int64_t*, const uint8_t*,
+                           int64_t, double, float*, float*, int, void*);
+typedef int (*logp_bwd_fn)(const void*, int64_t, int64_t, int64_t, int64_t, int64_t, const int64_t*, const uint8_t*,
+                           int64_t, double, const float*, const float*, void*, int, void*);
+typedef size_t (*token_ws_fn)(int64_t, int64_t);
+typedef int (*pref_fn)(const void*, int64_t, int64_t, int64_t, int64_t, int64_t, const int64_t*, const uint8_t*, int64_t,
+                       const float*, int, double, int, double, int, double, void*, float*, float*, void*, int, void*);
+typedef int (*policy_fn)(const void*, int64_t, int64_t, int64_t, int64_t, int64_t, const int64_t*, const uint8_t*,
+                         int64_t, double, const float*, const float*, const float*, int, double, double, double, int,
+                         double, void*, float*, float*, void*, int, void*);
+typedef int (*top_fn)(const void*, int64_t, int64_t, int64_t, int64_t, int64_t, int, double, void*, int32_t*, float*, int,
+                      void*);
+typedef size_t (*top_ws_fn)(int64_t, int);
+typedef int (*top_distil_fn)(const void*, int64_t, int64_t, int64_t, int64_t, int64_t, const void*, int, const int32_t*,
+                             const float*, int, const uint8_t*, double, double, void*, float*, void*, int, void*);
+static struct {
+  logp_fwd_fn logp_fwd = nullptr;
+  logp_bwd_fn logp_bwd = nullptr;
+  token_ws_fn token_ws = nullptr;
+  pref_fn pref = nullptr;
+  policy_fn policy = nullptr;
+  top_fn top = nullptr;
+  top_ws_fn top_ws = nullptr;
+  top_distil_fn top_distil = nullptr;
+} g_vocab;
+
+void bind_vocab(uintptr_t logp_fwd, uintptr_t logp_bwd, uintptr_t token_ws, uintptr_t pref, uintptr_t policy,
+                uintptr_t top, uintptr_t top_ws, uintptr_t top_distil) {
+  g_vocab.logp_fwd = reinterpret_cast<logp_fwd_fn>(logp_fwd);
+  g_vocab.logp_bwd = reinterpret_cast<logp_bwd_fn>(logp_bwd);
+  g_vocab.token_ws = reinterpret_cast<token_ws_fn>(token_ws);
+  g_vocab.pref = reinterpret_cast<pref_fn>(pref);
+  g_vocab.policy = reinterpret_cast<policy_fn>(policy);
+  g_vocab.top = reinterpret_cast<top_fn>(top);
+  g_vocab.top_ws = reinterpret_cast<top_ws_fn>(top_ws);
+  g_vocab.top_distil = reinterpret_cast<top_distil_fn>(top_distil);
+}
+
+// Logits as the entry points take them.
+struct VocabView {
+  const void* s;
+  int64_t n_seq, seq_len, V, ld_seq, ld_tok;
+  int code;
+};
+
+// False when the logits are not two- or three-dimensional device tensors with a dense last dimension.
+bool vocab_view(const at::Tensor& x, VocabView* v) {
+  if (!x.is_cuda() || x.layout() != at::kStrided || (x.dim() != 2 && x.dim() != 3)) return false;
+  v->code = dtype_code(x.scalar_type());
+  v->V = x.size(-1);
+  if (v->code < 0 || v->V < 1 || (v->V > 1 && x.stride(-1) != 1)) return false;
+  const bool seq = x.dim() == 3;
+  v->n_seq = seq ? x.size(0) : 1;
+  v->seq_len = x.size(-2);
+  v->ld_seq = seq ? x.stride(0) : 0;
+  v->ld_tok = x.stride(-2);
+  v->s = x.data_ptr();
+  return v->n_seq * v->seq_len > 0;
+}
+
+// A dense tensor of a type, on the logits' device, with one entry per row.
+bool per_row(const at::Tensor& t, const at::Tensor& x, at::ScalarType type) {
+  return t.is_cuda() && t.device() == x.device() && t.scalar_type() == type && t.is_contiguous() &&
+         t.dim() == x.dim() - 1 && t.sizes() == x.sizes().slice(0, x.dim() - 1);
+}
+
+bool row_mask_ok(const c10::optional<at::Tensor>& mask, const at::Tensor& x, const uint8_t** p) {
+  *p = nullptr;
+  if (!mask.has_value()) return true;
+  if (!per_row(*mask, x, at::kBool)) return false;
+  *p = static_cast<const uint8_t*>(mask->data_ptr());
+  return true;
+}
+
+inline at::Tensor like(const at::Tensor& x, at::IntArrayRef sizes, at::ScalarType type) {
+  return at::empty(sizes, x.options().dtype(type).requires_grad(false));
+}
+
+inline bool records(const at::Tensor& x) { return at::GradMode::is_enabled() && x.requires_grad(); }
+
+// Hands out a gradient that the forward pass computed, scaled by the incoming one.
+struct ReadyGradNode : public torch::autograd::Node {
+  at::Tensor grad;
+  void* stream = nullptr;
+  bool done = false;
+  torch::autograd::variable_list apply(torch::autograd::variable_list&& grad_out) override {
+    TORCH_CHECK(!done, "the fused loss keeps one gradient buffer: backward can run once per forward");
+    done = true;
+    at::Tensor g = std::move(grad);  // autograd can adopt it as .grad instead of copying
+    grad = at::Tensor();
+    at::Tensor go = grad_out[0];
+    if (!go.defined()) return {at::Tensor()};
+    c10::DeviceGuard guard(g.device());
+    if (go.scalar_type() != at::kFloat) go = go.to(at::kFloat);
+    const int64_t V = g.size(-1);
+    const int rc = g_scale(g.data_ptr(), g.numel() / V, V, V, go.data_ptr<float>(), dtype_code(g.scalar_type()), stream);
+    TORCH_CHECK(rc == 0, "ts_scale_rows: status ", rc);
+    return {g};
+  }
+  std::string name() const override { return "TSPipeAmdReadyGrad"; }
+};
+
+void record_ready(const at::Tensor& x, const at::Tensor& grad, void* stream, at::Tensor& loss) {
+  auto node = std::shared_ptr<ReadyGradNode>(new ReadyGradNode(), torch::autograd::deleteNode);
+  node->grad = grad;
+  node->stream = stream;
+  node->set_next_edges(torch::autograd::collect_next_edges(x));
+  torch::autograd::set_history(loss, node);
+}
+
+struct LogProbNode : public torch::autograd::Node {
+  torch::autograd::SavedVariable logits, labels, mask, stats;
+  int64_t ignore_index = -100;
+  double temperature = 1.0;
+  void* stream = nullptr;
+  torch::autograd::variable_list apply(torch::autograd::variable_list&& grad_out) override {
+    at::Tensor go = grad_out[0];
+    if (!go.defined()) return {at::Tensor()};
+    TORCH_CHECK(!at::GradMode::is_enabled(),
+                "the log probabilities' gradient cannot be differentiated again (create_graph)");
+    const at::Tensor x = logits.unpack(), lab = labels.unpack(), m = mask.unpack(), st = stats.unpack();
+    c10::DeviceGuard guard(x.device());
+    go = go.to(at::kFloat).contiguous();
+    VocabView v;
+    TORCH_CHECK(vocab_view(x, &v), "token_log_probs: the logits changed their layout");
+    at::Tensor g = like(x, x.sizes(), x.scalar_type());
+    const int rc = g_vocab.logp_bwd(v.s, v.n_seq, v.seq_len, v.V, v.ld_seq, v.ld_tok, lab.data_ptr<int64_t>(),
+                                    m.defined() ? static_cast<const uint8_t*>(m.data_ptr()) : nullptr, ignore_index,
+                                    temperature, st.data_ptr<float>(), go.data_ptr<float>(), g.data_ptr(), v.code, stream);
+    TORCH_CHECK(rc == 0, "ts_token_logp_bwd: status ", rc);
+    return {g};
+  }
+  void release_variables() override {
+    logits.reset_data();
+    labels.reset_data();
+    mask.reset_data();
+    stats.reset_data();
+  }
+  std::string name() const override { return "TSPipeAmdTokenLogProbs"; }
+};
+
+py::object vocab_log_probs(const at::Tensor& x, const at::Tensor& labels, const c10::optional<at::Tensor>& mask,
+                           double temperature, int64_t ignore_index, int64_t stream) {
+  VocabView v;
+  const uint8_t* m;
+  if (!g_vocab.logp_fwd || !vocab_view(x, &v) || !per_row(labels, x, at::kLong) || !row_mask_ok(mask, x, &m))
+    return py::none();
+  at::Tensor out;
+  {
+    py::gil_scoped_release no_gil;
+    c10::DeviceGuard guard(x.device());
+    const bool record = records(x);
+    out = like(x, labels.sizes(), at::kFloat);
+    at::Tensor stats;
+    if (record) stats = like(x, {v.n_seq * v.seq_len, 2}, at::kFloat);
+    const int rc = g_vocab.logp_fwd(v.s, v.n_seq, v.seq_len, v.V, v.ld_seq, v.ld_tok, labels.data_ptr<int64_t>(), m,
+                                    ignore_index, temperature, out.data_ptr<float>(),
+                                    record ? stats.data_ptr<float>() : nullptr, v.code, reinterpret_cast<void*>(stream));
+    TORCH_CHECK(rc == 0, "ts_token_logp_fwd: status ", rc);
+    if (record) {
+      auto node = std::shared_ptr<LogProbNode>(new LogProbNode(), torch::autograd::deleteNode);
+      node->set_next_edges(torch::autograd::collect_next_edges(x));
+      node->logits = torch::autograd::SavedVariable(x, false);
+      node->labels = torch::autograd::SavedVariable(labels, false);
+      node->mask = torch::autograd::SavedVariable(mask.has_value() ? *mask : at::Tensor(), false);
+      node->stats = torch::autograd::SavedVariable(stats, false);
+      node->ignore_index = ignore_index;
+      node->temperature = temperature;
+      node->stream = reinterpret_cast<void*>(stream);
+      torch::autograd::set_history(out, node);
+    }
+  }
+  return py::cast(out);
+}
+
+// f = {beta, smoothing, weight}; n = {kind, average, ignore_index}
+py::object vocab_preference(const at::Tensor& x, const at::Tensor& labels, const at::Tensor& ref,
+                            const c10::optional<at::Tensor>& mask, std::array<double, 3> f, std::array<int64_t, 3> n,
+                            int64_t stream) {
+  VocabView v;
+  const uint8_t* m;
+  if (!g_vocab.pref || x.dim() != 3 || x.size(0) % 2 || !vocab_view(x, &v) || !per_row(labels, x, at::kLong) ||
+      !row_mask_ok(mask, x, &m))
+    return py::none();
+  const bool per_token = ref.dim() == 2;
+  if (ref.device() != x.device() || ref.scalar_type() != at::kFloat || !ref.is_contiguous() ||
+      !(per_token ? ref.sizes() == labels.sizes() : ref.dim() == 1 && ref.size(0) == x.size(0)))
+    return py::none();
+  at::Tensor loss, rewards;
+  {
+    py::gil_scoped_release no_gil;
+    c10::DeviceGuard guard(x.device());
+    void* st = reinterpret_cast<void*>(stream);
+    const bool record = records(x);
+    at::Tensor ws = like(x, {(int64_t)g_vocab.token_ws(v.n_seq, v.seq_len)}, at::kByte), grad;
+    loss = like(x, {}, at::kFloat);
+    rewards = like(x, {v.n_seq}, at::kFloat);
+    if (record) grad = like(x, x.sizes(), x.scalar_type());
+    const int rc = g_vocab.pref(v.s, v.n_seq, v.seq_len, v.V, v.ld_seq, v.ld_tok, labels.data_ptr<int64_t>(), m, n[2],
+                                ref.data_ptr<float>(), per_token, f[0], (int)n[0], f[1], (int)n[1], f[2], ws.data_ptr(),
+                                loss.data_ptr<float>(), rewards.data_ptr<float>(), record ? grad.data_ptr() : nullptr,
+                                v.code, st);
+    TORCH_CHECK(rc == 0, "ts_preference_fwd_bwd: status ", rc);
+    if (record) record_ready(x, grad, st, loss);
+  }
+  return py::make_tuple(loss, rewards);
+}
+
+// f = {kl_weight, clip_lo, clip_hi, temperature, weight}; n = {per_seq, ignore_index}
+py::object vocab_policy(const at::Tensor& x, const at::Tensor& labels, const at::Tensor& old_lp, const at::Tensor& adv,
+                        const c10::optional<at::Tensor>& ref, const c10::optional<at::Tensor>& mask,
+                        std::array<double, 5> f, std::array<int64_t, 2> n, int64_t stream) {
+  VocabView v;
+  const uint8_t* m;
+  if (!g_vocab.policy || x.dim() != 3 || !vocab_view(x, &v) || !per_row(labels, x, at::kLong) ||
+      !row_mask_ok(mask, x, &m) || !per_row(old_lp, x, at::kFloat) || (ref.has_value() && !per_row(*ref, x, at::kFloat)) ||
+      (!ref.has_value() && f[0] != 0.0))
+    return py::none();
+  const bool adv_per_seq = adv.dim() == 1;
+  if (adv.device() != x.device() || adv.scalar_type() != at::kFloat || !adv.is_contiguous() ||
+      !(adv_per_seq ? adv.size(0) == x.size(0) : adv.sizes() == labels.sizes()))
+    return py::none();
+  at::Tensor loss, logp;
+  {
+    py::gil_scoped_release no_gil;
+    c10::DeviceGuard guard(x.device());
+    void* st = reinterpret_cast<void*>(stream);
+    const bool record = records(x);
+    at::Tensor ws = like(x, {(int64_t)g_vocab.token_ws(v.n_seq, v.seq_len)}, at::kByte), grad;
+    loss = like(x, {}, at::kFloat);
+    logp = like(x, labels.sizes(), at::kFloat);
+    if (record) grad = like(x, x.sizes(), x.scalar_type());
+    const int rc = g_vocab.policy(v.s, v.n_seq, v.seq_len, v.V, v.ld_seq, v.ld_tok, labels.data_ptr<int64_t>(), m, n[1],
+                                  f[3], old_lp.data_ptr<float>(), ref.has_value() ? ref->data_ptr<float>() : nullptr,
+                                  adv.data_ptr<float>(), adv_per_seq, f[0], f[1], f[2], (int)n[0], f[4], ws.data_ptr(),
+                                  loss.data_ptr<float>(), logp.data_ptr<float>(), record ? grad.data_ptr() : nullptr,
+                                  v.code, st);
+    TORCH_CHECK(rc == 0, "ts_policy_fwd_bwd: status ", rc);
+    if (record) record_ready(x, grad, st, loss);
+  }
+  return py::make_tuple(loss, logp);
+}
+
+py::object vocab_top(const at::Tensor& x, int64_t k, double temperature, int64_t stream) {
+  VocabView v;
+  if (!g_vocab.top || !vocab_view(x, &v)) return py::none();
+  at::Tensor values, indices, lse;
+  {
+    py::gil_scoped_release no_gil;
+    c10::DeviceGuard guard(x.device());
+    std::vector<int64_t> sizes(x.sizes().begin(), x.sizes().end());
+    sizes.back() = k;
+    values = like(x, sizes, x.scalar_type());
+    indices = like(x, sizes, at::kInt);
+    sizes.pop_back();
+    lse = like(x, sizes, at::kFloat);
+    const int rc = g_vocab.top(v.s, v.n_seq, v.seq_len, v.V, v.ld_seq, v.ld_tok, (int)k, temperature, values.data_ptr(),
+                               indices.data_ptr<int32_t>(), lse.data_ptr<float>(), v.code, reinterpret_cast<void*>(stream));
+    TORCH_CHECK(rc == 0, "ts_top_logits: status ", rc);
+  }
+  return py::make_tuple(values, indices, lse);
+}
+
+py::object vocab_top_distil(const at::Tensor& x, const at::Tensor& values, const at::Tensor& indices,
+                            const c10::optional<at::Tensor>& lse, const c10::optional<at::Tensor>& mask,
+                            double temperature, double weight, int64_t stream) {
+  VocabView v;
+  const uint8_t* m;
+  if (!g_vocab.top_distil || !vocab_view(x, &v) || !row_mask_ok(mask, x, &m) ||
+      (lse.has_value() && !per_row(*lse, x, at::kFloat)) || values.dim() != x.dim() || indices.sizes() != values.sizes())
+    return py::none();
+  const int64_t k = values.size(-1);
+  const int t_code = dtype_code(values.scalar_type());
+  if (k < 1 || k > 256 || t_code < 0 || values.device() != x.device() || indices.device() != x.device() ||
+      indices.scalar_type() != at::kInt || !values.is_contiguous() || !indices.is_contiguous() ||
+      values.sizes().slice(0, x.dim() - 1) != x.sizes().slice(0, x.dim() - 1) || (lse.has_value() && v.V > (1 << 20)))
+    return py::none();
+  at::Tensor loss;
+  {
+    py::gil_scoped_release no_gil;
+    c10::DeviceGuard guard(x.device());
+    void* st = reinterpret_cast<void*>(stream);
+    const bool record = records(x);
+    at::Tensor ws = like(x, {(int64_t)g_vocab.top_ws(v.n_seq * v.seq_len, (int)k)}, at::kByte), grad;
+    loss = like(x, {}, at::kFloat);
+    if (record) grad = like(x, x.sizes(), x.scalar_type());
+    const int rc = g_vocab.top_distil(v.s, v.n_seq, v.seq_len, v.V, v.ld_seq, v.ld_tok, values.data_ptr(), t_code,
+                                      indices.data_ptr<int32_t>(), lse.has_value() ? lse->data_ptr<float>() : nullptr,
+                                      (int)k, m, temperature, weight, ws.data_ptr(), loss.data_ptr<float>(),
+                                      record ? grad.data_ptr() : nullptr, v.code, st);
+    TORCH_CHECK(rc == 0, "ts_top_distil_fwd_bwd: status ", rc);
+    if (record) record_ready(x, grad, st, loss);
+  }
+  return py::cast(loss);
+}
+
 // Test aid: a C++ owner of a tensor that Python cannot see.  hold() keeps the
 // tensor alive inside this module until drop() is called.
 static std::vector<at::Tensor> g_held;
@@ -506,6 +815,12 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("bind_bn", &bind_bn);
   m.def("bind_losses", &bind_losses);
   m.def("row_loss", &row_loss);
+  m.def("bind_vocab", &bind_vocab);
+  m.def("vocab_log_probs", &vocab_log_probs);
+  m.def("vocab_preference", &vocab_preference);
+  m.def("vocab_policy", &vocab_policy);
+  m.def("vocab_top", &vocab_top);
+  m.def("vocab_top_distil", &vocab_top_distil);
   m.def("bn_train", &bn_train);
   m.def("hold", &hold);
   m.def("drop", &drop);

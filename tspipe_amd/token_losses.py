@@ -18,7 +18,7 @@ import torch
 from torch import Tensor
 
 from . import _lib
-from ._vocab import floats_of, labels_of, mask_of, ptr, recorded, rows_of, same_device, temperature_of
+from ._vocab import floats_of, host_for, labels_of, mask_of, ptr, recorded, rows_of, same_device, temperature_of
 from .losses import _once, _scale_saved_grad
 
 
@@ -66,8 +66,13 @@ def token_log_probs(logits: Tensor, labels: Tensor, temperature: float = 1.0, ig
     of ``labels`` (``logits.shape[:-1]``).  Rows whose label is ``ignore_index``
     or outside the classes, or whose ``row_mask`` entry is 0, are not read: 0,
     with a zero gradient."""
-    return _TokenLogProbsFn.apply(recorded(logits), labels, row_mask, temperature_of(temperature, "token_log_probs"),
-                                  int(ignore_index))
+    temperature, ignore_index = temperature_of(temperature, "token_log_probs"), int(ignore_index)
+    host = host_for(logits, labels, row_mask)
+    if host is not None:
+        out = host[0].vocab_log_probs(logits, labels, row_mask, temperature, ignore_index, host[1])
+        if out is not None:
+            return out
+    return _TokenLogProbsFn.apply(recorded(logits), labels, row_mask, temperature, ignore_index)
 
 
 _PREFERENCE_KINDS = {"sigmoid": 0, "hinge": 1, "ipo": 2}
@@ -146,9 +151,16 @@ def preference_loss(logits: Tensor, labels: Tensor, ref_log_probs: Tensor, beta:
         raise ValueError(f"preference_loss needs a positive beta, got {beta}")
     if not 0 <= label_smoothing <= 1 or (label_smoothing and loss_type != "sigmoid"):
         raise ValueError(f"label_smoothing {label_smoothing} with loss_type {loss_type!r}")
-    loss, rewards = _PreferenceFn.apply(recorded(logits), labels, ref_log_probs, row_mask, float(beta),
-                                        _PREFERENCE_KINDS[loss_type], float(label_smoothing), bool(length_average),
-                                        float(weight), int(ignore_index))
+    kind = _PREFERENCE_KINDS[loss_type]
+    host, out = host_for(logits, labels, ref_log_probs, row_mask), None
+    if host is not None:
+        out = host[0].vocab_preference(logits, labels, ref_log_probs, row_mask,
+                                       (float(beta), float(label_smoothing), float(weight)),
+                                       (kind, 1 if length_average else 0, int(ignore_index)), host[1])
+    if out is None:
+        out = _PreferenceFn.apply(recorded(logits), labels, ref_log_probs, row_mask, float(beta), kind,
+                                  float(label_smoothing), bool(length_average), float(weight), int(ignore_index))
+    loss, rewards = out
     return (loss, rewards) if return_rewards else loss
 
 
@@ -213,10 +225,17 @@ def clipped_policy_loss(logits: Tensor, labels: Tensor, old_log_probs: Tensor, a
         raise ValueError("a KL term needs ref_log_probs")
     if not (clip_low >= 0 and clip_high >= 0):
         raise ValueError(f"clipping range [1 - {clip_low}, 1 + {clip_high}]")
-    loss, logp = _PolicyFn.apply(recorded(logits), labels, old_log_probs, advantages, ref_log_probs, row_mask, float(kl_weight),
-                                 1.0 - float(clip_low), 1.0 + float(clip_high),
-                                 temperature_of(temperature, "clipped_policy_loss"), reduction == "sequence",
-                                 float(weight), int(ignore_index))
+    temperature = temperature_of(temperature, "clipped_policy_loss")
+    numbers = (float(kl_weight), 1.0 - float(clip_low), 1.0 + float(clip_high), temperature)
+    host, out = host_for(logits, labels, old_log_probs, advantages, ref_log_probs, row_mask), None
+    if host is not None:
+        out = host[0].vocab_policy(logits, labels, old_log_probs, advantages, ref_log_probs, row_mask,
+                                   (*numbers, float(weight)), (1 if reduction == "sequence" else 0, int(ignore_index)),
+                                   host[1])
+    if out is None:
+        out = _PolicyFn.apply(recorded(logits), labels, old_log_probs, advantages, ref_log_probs, row_mask, *numbers,
+                              reduction == "sequence", float(weight), int(ignore_index))
+    loss, logp = out
     return (loss, logp) if return_log_probs else loss
 
 

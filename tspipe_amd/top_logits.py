@@ -12,7 +12,7 @@ import torch
 from torch import Tensor
 
 from . import _lib
-from ._vocab import floats_of, mask_of, ptr, recorded, rows_of, same_device, temperature_of
+from ._vocab import floats_of, host_for, mask_of, ptr, recorded, rows_of, same_device, temperature_of
 from .losses import _once, _scale_saved_grad
 
 MAX_ENTRIES = 256  # entries a row may keep
@@ -24,14 +24,18 @@ class TopLogits(NamedTuple):
     logsumexp: Tensor   # [...], fp32, of logits / temperature
 
 
-@torch.no_grad()
 def top_logits(logits: Tensor, k: int, temperature: float = 1.0) -> TopLogits:
     """The ``k`` largest logits of each row (last dimension), largest first and
     equal ones by their place, with the log-sum-exp of ``logits / temperature``;
     all detached.  ``1 <= k <= min(classes, 256)``."""
-    r = rows_of(logits, "top_logits")
     t = temperature_of(temperature, "top_logits")
     k = int(k)
+    host = host_for(logits)
+    if host is not None and logits.dim() > 0 and 1 <= k <= min(int(logits.shape[-1]), MAX_ENTRIES):
+        out = host[0].vocab_top(logits, k, t, host[1])
+        if out is not None:
+            return TopLogits(*out)
+    r = rows_of(logits, "top_logits")
     if not 1 <= k <= min(r.V, MAX_ENTRIES):
         raise ValueError(f"top_logits keeps 1 to {min(r.V, MAX_ENTRIES)} of {r.V} classes, asked for {k}")
     dev = logits.device
@@ -72,7 +76,7 @@ class _TopDistilFn(torch.autograd.Function):
         mask = mask_of(row_mask, shape, what)
         dev = s_logits.device
         lib = _lib.lib()
-        ws = torch.empty(lib.ts_top_distil_workspace_bytes(r.count), dtype=torch.uint8, device=dev)
+        ws = torch.empty(lib.ts_top_distil_workspace_bytes(r.count, k), dtype=torch.uint8, device=dev)
         loss = torch.empty((), dtype=torch.float32, device=dev)
         grad = torch.empty(s_logits.shape, dtype=s_logits.dtype, device=dev) if ctx.needs_input_grad[0] else None
         with _lib.on_device(dev):
@@ -108,8 +112,13 @@ def top_logits_distil_loss(s_logits: Tensor, t_values: Tensor, t_indices: Tensor
     Entries with an index outside the classes are absent and those of value
     -inf weigh nothing; a token named twice counts with both its entries.  Up
     to 256 entries a row; the teacher's type may differ from the student's."""
-    return _TopDistilFn.apply(recorded(s_logits), t_values, t_indices, t_logsumexp, row_mask,
-                              temperature_of(T, "top_logits_distil_loss"), float(weight))
+    T = temperature_of(T, "top_logits_distil_loss")
+    host = host_for(s_logits, t_values, t_indices, t_logsumexp, row_mask)
+    if host is not None:
+        out = host[0].vocab_top_distil(s_logits, t_values, t_indices, t_logsumexp, row_mask, T, float(weight), host[1])
+        if out is not None:
+            return out
+    return _TopDistilFn.apply(recorded(s_logits), t_values, t_indices, t_logsumexp, row_mask, T, float(weight))
 
 
 def top_distil_loss_fn(student_outputs, teacher_outputs, labels, tspipe_args, params, epoch: int) -> Tensor:
