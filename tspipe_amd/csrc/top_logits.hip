@@ -38,32 +38,100 @@ __device__ __forceinline__ float top_unkey(uint32_t key) {
   return __uint_as_float((key & 0x80000000u) ? key & 0x7fffffffu : ~key);
 }
 
-constexpr int kTopCand = 2304;  // candidates a row may have: all of a row that 64 threads hold, and more
+// Vectors with a candidate and candidates a row may have at a time.  64 threads
+// may have to take a whole row of theirs (k close to V).
+template <int NT>
+constexpr int top_hit_cap() { return NT == 64 ? 288 : NT == 256 ? 512 : 1024; }
+template <int NT>
+constexpr int top_cand_cap() { return NT == 64 ? 2304 : 1536; }
 
 template <int NT>
 struct TopShared {
   union {
     uint32_t group[2 * NT];  // order numbers of the groups' maxima
     uint64_t kept[kTopMax];
+    u32x4 hit[top_hit_cap<NT>()];  // vectors with a candidate
   };
-  uint64_t cand[kTopCand];  // order number and place, larger for smaller places
+  int hit_at[top_hit_cap<NT>()];  // their first elements' places
+  uint64_t cand[top_cand_cap<NT>()];  // order number and place, larger for smaller places
   RowSum sums[NT / kWave];
   VocabStat stats[NT / kWave];
   int counts[NT / kWave];
-  int n;
+  int rank[2 * kTopMax];
+  int n, n_hit;
   float bar;
 };
 
-// Every thread's rank among n candidates; the first k leave.
+// The largest of a vector's elements by their bits as signed numbers: two
+// sixteen-bit maxima, or one of 32 bits.  For logits above zero that is their
+// order; of a vector without such a one it is just one of its elements.
+template <typename T>
+struct RawMax {
+  int32_t m;
+  static constexpr int32_t kNone = sizeof(T) == 4 ? (int32_t)0x80000000 : (int32_t)0x80008000;
+  __device__ __forceinline__ static int32_t max2(int32_t a, int32_t b) {
+    if constexpr (sizeof(T) == 4) {
+      return a > b ? a : b;
+    } else {
+      typedef int16_t s16x2 __attribute__((ext_vector_type(2)));
+      s16x2 x, y;
+      __builtin_memcpy(&x, &a, 4);
+      __builtin_memcpy(&y, &b, 4);
+      const s16x2 z = __builtin_elementwise_max(x, y);
+      int32_t r;
+      __builtin_memcpy(&r, &z, 4);
+      return r;
+    }
+  }
+  __device__ __forceinline__ static int32_t of(const Vec16<T>& v) {
+    int32_t w[4];
+    __builtin_memcpy(w, &v, 16);
+    return max2(max2(w[0], w[1]), max2(w[2], w[3]));
+  }
+  // the element that `m` stands for, as fp32
+  __device__ __forceinline__ static float value(int32_t m) {
+    if constexpr (sizeof(T) == 4) {
+      return __int_as_float(m);
+    } else {
+      const int16_t lo = (int16_t)(m & 0xffff), hi = (int16_t)(m >> 16);
+      const int16_t top = lo > hi ? lo : hi;
+      T t;
+      __builtin_memcpy(&t, &top, 2);
+      return to_f32(t);
+    }
+  }
+};
+
+// Ranks the n candidates by counting, for each one, those that are larger; the
+// first k leave.  With fewer candidates than threads several threads count for
+// each.  sh.rank is 0 on entry.
 template <typename T, int NT>
-__device__ __forceinline__ void top_emit(const uint64_t* cand, int n, const T* x, int64_t row, int k,
+__device__ __forceinline__ void top_emit(TopShared<NT>& sh, int n, const T* x, int64_t row, int k,
                                          T* __restrict__ values, int32_t* __restrict__ indices) {
-  for (int c = threadIdx.x; c < n; c += NT) {
-    const uint64_t me = cand[c];
+  constexpr int NW = NT / kWave;
+  const int all = __builtin_amdgcn_readfirstlane(n);
+  const int waves = (all + kWave - 1) / kWave;  // wavefronts that hold one candidate a lane
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave);
+  int part = 0, first = wave, parts = 1;
+  if (waves < NW) {
+    parts = 0;
+    for (int w = waves; w <= NW; w += waves) ++parts;
+    for (; first >= waves; first -= waves) ++part;
+  }
+  const int per = (int)(((float)all + (float)parts - 0.5f) / (float)parts);  // all / parts, rounded up
+  const int lo = part * per, hi = part < parts ? (lo + per < all ? lo + per : all) : lo;
+  for (int c = first * kWave + (int)threadIdx.x % kWave; c < all; c += NT) {
+    const uint64_t me = sh.cand[c];
     int rank = 0;
-    for (int i = 0; i < n; ++i) rank += cand[i] > me;
+#pragma unroll 4
+    for (int i = lo; i < hi; ++i) rank += sh.cand[i] > me;
+    if (rank) atomicAdd(&sh.rank[c], rank);
+  }
+  __syncthreads();
+  for (int c = threadIdx.x; c < n; c += NT) {
+    const int rank = sh.rank[c];
     if (rank < k) {
-      const int32_t i = (int32_t)~(uint32_t)me;
+      const int32_t i = (int32_t)~(uint32_t)sh.cand[c];
       indices[row * k + rank] = i;
       values[row * k + rank] = x[i];
     }
@@ -112,7 +180,7 @@ __device__ __forceinline__ void top_row_walked(const VocabRows& a, int64_t row, 
     }
   }
   __syncthreads();
-  top_emit<T, NT>(sh.cand, k, x, row, k, values, indices);
+  top_emit<T, NT>(sh, k, x, row, k, values, indices);
 }
 
 // Reduces n > k candidates to the k largest.
@@ -145,17 +213,100 @@ __device__ __forceinline__ void top_refine(TopShared<NT>& sh, int n, int k) {
   __syncthreads();
 }
 
+// The largest order number (to within the `enough` that end the search early)
+// that at least k of a wavefront's numbers reach, N of them a lane; 0 when
+// fewer than k are above 0.  Called by one whole wavefront.
+template <int N>
+__device__ __forceinline__ uint32_t top_bar(const uint32_t (&key)[N], int k) {
+  uint32_t t = 0;
+  const int enough = k + k / 8 + 4;
+  for (int bit = 31; bit >= 0; --bit) {
+    const uint32_t cnd = t | (1u << bit);
+    int cnt = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) cnt += (int)__popcll(__ballot(key[i] >= cnd));
+    if (cnt >= k) {
+      t = cnd;
+      if (cnt <= enough) break;
+    }
+  }
+  return t;
+}
+
+// Elements that reach the bar, of the vectors noted since the last call, become
+// candidates; false when they do not all fit.  With many more vectors noted
+// than k the bar first rises to the k-th largest of their maxima: ranking costs
+// the square of the candidates (k = 128 of 131072 in two pieces, 270 of them:
+// 22 of 105 us).
+template <typename T, int NT, bool LAST, bool MULTI>
+__device__ __forceinline__ bool top_expand(TopShared<NT>& sh, int k) {
+  constexpr int VEC = Vec16<T>::N, kCap = top_cand_cap<NT>();
+  __syncthreads();
+  const int hits = sh.n_hit;
+  if (hits > top_hit_cap<NT>()) return false;  // uniform
+  if (MULTI && hits > k + k / 2) {
+    constexpr int N = (top_hit_cap<NT>() + kWave - 1) / kWave / 2;
+    if (hits <= N * kWave && threadIdx.x < kWave) {
+      uint32_t key[N];
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int at = i * kWave + (int)threadIdx.x;
+        key[i] = 0u;
+        if (at < hits) {
+          Vec16<T> v;
+          __builtin_memcpy(&v, &sh.hit[at], 16);
+          key[i] = top_key(RawMax<T>::value(RawMax<T>::of(v)));
+          if (key[i] == 0xffffffffu) key[i] = 0u;  // a NaN sets no bar
+        }
+      }
+      const uint32_t t = top_bar<N>(key, k);
+      if (threadIdx.x == 0 && t) sh.bar = fmaxf(sh.bar, top_unkey(t));
+    }
+    __syncthreads();
+  }
+  const float bar = sh.bar;
+  for (int e = threadIdx.x; e < hits * VEC; e += NT) {
+    const T* v = reinterpret_cast<const T*>(&sh.hit[e / VEC]);
+    const float x = to_f32(v[e % VEC]);
+    if (x >= bar) {
+      const int at = atomicAdd(&sh.n, 1);
+      if (at < kCap) sh.cand[at] = ((uint64_t)top_key(x) << 32) | (uint32_t)~(uint32_t)(sh.hit_at[e / VEC] + e % VEC);
+    }
+  }
+  __syncthreads();
+  const int n = sh.n;
+  if (n > kCap) return false;
+  if (LAST && n <= 2 * kTopMax) return true;
+  __syncthreads();  // (nobody changes it before everybody has read it)
+  if (threadIdx.x == 0) sh.n_hit = 0;
+  if (n > 2 * kTopMax) top_refine<NT>(sh, n, k);
+  __syncthreads();
+  return true;
+}
+
 // One pass over a row by one workgroup, in pieces of NT * KREG vectors.  The
 // first piece gives a bar: the threads' maxima (two each when k is large) are
-// maxima of disjoint groups, so the k-th largest of them is reached by at least
-// k elements.  Every element that reaches the bar is a candidate -- few more
-// than k, since the best k mostly lie in different groups (k = 64 of 512
+// elements of disjoint groups, so the k-th largest of them is reached by at
+// least k elements.  Every element that reaches the bar is a candidate -- few
+// more than k, since the best k mostly lie in different groups (k = 64 of 512
 // groups: 68 expected) -- and the candidates' ranks are counted.  The row's sum
 // is taken in the same walk over the registers.
-template <typename T, int NT, int KREG>
-__global__ __launch_bounds__(NT, NT > 256 ? (NT > 512 ? 8 : 6) : 1) void top_logits_kernel(const VocabRows a, int k, T* __restrict__ values,
-                                                        int32_t* __restrict__ indices, float* __restrict__ lse) {
+//
+// The walk is bound by its vector instructions, four of every seven an
+// exponential's.  So the maxima compare raw bits, two 16-bit logits at a time,
+// and a vector that reaches the bar is only noted; its elements are looked at
+// when the noted vectors are spread over all threads.
+//
+// MULTI: the row has more than one piece.  Eight wavefronts a SIMD: 64 registers
+// are enough, and with 80 and six of them 4096 x 30522 bf16 takes 67 us instead
+// of 58, 1024 x 131072 96 instead of 79.
+template <typename T, int NT, int KREG, bool MULTI>
+__global__ __launch_bounds__(NT, NT > 256 ? 8 : 1) void top_logits_kernel(const VocabRows a, int k,
+                                                                          T* __restrict__ values,
+                                                                          int32_t* __restrict__ indices,
+                                                                          float* __restrict__ lse) {
   constexpr int VEC = Vec16<T>::N;
+  typedef RawMax<T> Raw;
   __shared__ TopShared<NT> sh;
   const int64_t row = blockIdx.x, V = a.V;
   const T* x = vocab_row<T>(a, row);
@@ -165,114 +316,131 @@ __global__ __launch_bounds__(NT, NT > 256 ? (NT > 512 ? 8 : 6) : 1) void top_log
   const bool two = k > NT / 4;  // two groups per thread
   RowRegs<T, NT, KREG> r;
   regs_load(r, x, V, g);
-  if (tid == 0) sh.n = 0;
+  if (tid == 0) sh.n = sh.n_hit = 0;
+  for (int i = tid; i < 2 * kTopMax; i += NT) sh.rank[i] = 0;
   const float c = regs_anchor(r, g, kk);
-  float z = 0.f, m0 = fmaxf(r.h(), r.t()), m1 = -__builtin_inff();
+  float z = 0.f;
   auto add = [&](float xv) { z += fast_exp2(fmaf(xv, kk, c)); };
   if (tid < kWave) {
     add(r.h());
     add(r.t());
   }
-  float bar = 0.f;
-  for (int64_t v0 = 0;; v0 += NT * KREG) {
-    const int left = (int)(g.nvec - v0);
+  // the first piece: its sum, the groups' maxima, the bar
+  const int n0 = g.nvec < NT * KREG ? (int)g.nvec : NT * KREG;
+  int32_t m0 = Raw::kNone, m1 = Raw::kNone;
+#pragma unroll
+  for (int j = 0; j < KREG; ++j) {
+    if (tid + j * NT < n0) {
+      forget(r.v[j]);
+      if (j < KREG / 2)
+        m0 = Raw::max2(m0, Raw::of(r.v[j]));
+      else
+        m1 = Raw::max2(m1, Raw::of(r.v[j]));
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) add(to_f32(r.v[j].v[i]));
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  {
+    float f0 = fmaxf(r.h(), r.t()), f1 = -__builtin_inff();
+    bool has0 = r.has_h || r.has_t;
+    if (tid < n0) {
+      f0 = fmaxf(f0, Raw::value(m0));
+      has0 = true;
+    }
+    const bool has1 = tid + KREG / 2 * NT < n0;
+    if (has1) f1 = Raw::value(m1);
+    if (!two) f0 = fmaxf(f0, f1);
+    sh.group[tid] = has0 ? top_key(f0) : 0u;
+    if (two) sh.group[NT + tid] = has1 ? top_key(f1) : 0u;
+  }
+  __syncthreads();
+  if (tid < kWave) {
+    // in registers: read from LDS for every bit, 4096 rows of 30522 took 76 us instead of 57
+    constexpr int kKeys = 2 * NT / kWave;
+    uint32_t key[kKeys];
+#pragma unroll
+    for (int i = 0; i < kKeys; ++i) key[i] = two || i < NT / kWave ? sh.group[i * kWave + tid] : 0u;
+    uint32_t t;
+    if (two) {  // uniform
+      t = top_bar<kKeys>(key, k);
+    } else {
+      uint32_t half[NT / kWave];
+#pragma unroll
+      for (int i = 0; i < NT / kWave; ++i) half[i] = key[i];
+      t = top_bar<NT / kWave>(half, k);
+    }
+    if (tid == 0) sh.bar = top_unkey(t);
+  }
+  __syncthreads();
+  const float bar = sh.bar;
+  const bool raw = bar > 0.f;  // raw bits order the logits from there up
+  int32_t below = 0;  // raw bits (twice, for 16-bit types) that a logit which reaches the bar exceeds
+  if constexpr (sizeof(T) == 4) {
+    below = __float_as_int(bar) - 1;
+  } else {
+    // (two steps below the rounded bar: rounding may have gone up; the elements are compared exactly later)
+    const T t = from_f32<T>(bar);
+    uint16_t bits;
+    __builtin_memcpy(&bits, &t, 2);
+    const int32_t b = bits > 1 ? bits - 2 : 0;
+    below = (b << 16) | b;
+  }
+  auto take = [&](float xv, int i) {
+    if (xv >= bar) {
+      const int at = atomicAdd(&sh.n, 1);
+      if (at < top_cand_cap<NT>()) sh.cand[at] = ((uint64_t)top_key(xv) << 32) | (uint32_t)~(uint32_t)i;
+    }
+  };
+  if (tid < g.head) take(r.h(), tid);
+  if (g.tail0 + tid < V) take(r.t(), (int)g.tail0 + tid);
+  auto reaches = [&](const Vec16<T>& v) {
+    if (raw) return Raw::max2(Raw::of(v), below) != below;
+    float m = -__builtin_inff();
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) m = fmaxf(m, to_f32(v.v[i]));
+    return m >= bar;
+  };
+  // Candidates, piece by piece.  A register that is done with takes the next piece's vector at once, so
+  // that loads are always under way; later pieces are summed in this walk.
+  bool fits = true;
+  for (int64_t v0 = 0; fits; v0 += NT * KREG) {
+    const int left = !MULTI ? n0 : g.nvec - v0 < NT * KREG ? (int)(g.nvec - v0) : NT * KREG;
+    const int64_t after = MULTI ? g.nvec - v0 - left : 0;  // vectors behind this piece
+    const VecBuffer next = vec_buffer(x + g.head + (v0 + left) * VEC, after < NT * KREG ? (int)after : NT * KREG);
 #pragma unroll
     for (int j = 0; j < KREG; ++j) {
       if (tid + j * NT < left) {
         forget(r.v[j]);
-        float m = -__builtin_inff();
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          const float xv = to_f32(r.v[j].v[i]);
-          add(xv);
-          m = fmaxf(m, xv);
-        }
-        if (j < KREG / 2)
-          m0 = fmaxf(m0, m);
-        else
-          m1 = fmaxf(m1, m);
-      }
-      __builtin_amdgcn_sched_barrier(0);
-    }
-    if (v0 == 0) {
-      sh.group[tid] = top_key(two ? m0 : fmaxf(m0, m1));
-      if (two) sh.group[NT + tid] = top_key(m1);
-      __syncthreads();
-      if (tid < kWave) {
-        uint32_t key[NT / kWave];
-#pragma unroll
-        for (int i = 0; i < NT / kWave; ++i) key[i] = sh.group[i * kWave + tid];
-        uint32_t t = 0;
-        const int enough = k + k / 8 + 4;
-        for (int bit = 31; bit >= 0; --bit) {
-          const uint32_t cnd = t | (1u << bit);
-          int cnt = 0;
-#pragma unroll
-          for (int i = 0; i < NT / kWave; ++i) cnt += (int)__popcll(__ballot(key[i] >= cnd));
-          if (two)
-            for (int i = 0; i < NT / kWave; ++i) cnt += (int)__popcll(__ballot(sh.group[NT + i * kWave + tid] >= cnd));
-          if (cnt >= k) {
-            t = cnd;
-            if (cnt <= enough) break;
+        if (reaches(r.v[j])) {
+          const int at = atomicAdd(&sh.n_hit, 1);
+          if (at < top_hit_cap<NT>()) {
+            __builtin_memcpy(&sh.hit[at], &r.v[j], 16);
+            sh.hit_at[at] = g.head + ((int)v0 + tid + j * NT) * VEC;
           }
         }
-        if (tid == 0) sh.bar = top_unkey(t);
-      }
-      __syncthreads();
-      bar = sh.bar;
-    }
-    // candidates among the registers (and the end elements, with the first piece)
-    auto take = [&](float xv, int i) {
-      if (xv >= bar) {
-        const int at = atomicAdd(&sh.n, 1);
-        if (at < kTopCand) sh.cand[at] = ((uint64_t)top_key(xv) << 32) | (uint32_t)~(uint32_t)i;
-      }
-    };
-    if (v0 == 0) {
-      if (tid < g.head) take(r.h(), tid);
-      if (g.tail0 + tid < V) take(r.t(), (int)g.tail0 + tid);
-    }
-    if (fmaxf(m0, m1) >= bar) {
+        if (MULTI && v0 > 0) {
 #pragma unroll
-      for (int j = 0; j < KREG; ++j) {
-        if (tid + j * NT < left) {
-          forget(r.v[j]);
-          const int e0 = g.head + ((int)v0 + tid + j * NT) * VEC;
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) take(to_f32(r.v[j].v[i]), e0 + i);
+          for (int i = 0; i < VEC; ++i) add(to_f32(r.v[j].v[i]));
         }
-        __builtin_amdgcn_sched_barrier(0);
       }
+      if (MULTI && after > 0) r.v[j] = vec_load<T>(next, tid + j * NT);
+      __builtin_amdgcn_sched_barrier(0);
     }
-    if (left <= NT * KREG) break;
-    const int next = left - NT * KREG < NT * KREG ? left - NT * KREG : NT * KREG;
-    const VecBuffer piece = vec_buffer(x + g.head + (v0 + NT * KREG) * VEC, next);
-#pragma unroll
-    for (int j = 0; j < KREG; ++j) r.v[j] = vec_load<T>(piece, tid + j * NT);
-    m0 = m1 = -__builtin_inff();
-    __syncthreads();
-    const int n = sh.n;
-    __syncthreads();  // (nobody adds to it before everybody has read it)
-    if (n > kTopCand / 2) {  // room for the next piece's
-      if (n > kTopCand) break;
-      top_refine<NT>(sh, n, k);
-    }
+    if (!MULTI || after == 0) break;
+    if ((v0 / (NT * KREG)) % 2 == 1) fits = top_expand<T, NT, false, MULTI>(sh, k);
   }
-  const RowSum s = rowsum_block<NT / kWave, kSumOnly>(c, z, 0.f, sh.sums);
-  __syncthreads();
-  int n = sh.n;
-  if (!s.ok || n > kTopCand) {
+  const RowSum mine = rowsum_put<NT / kWave, kSumOnly>(c, z, 0.f, sh.sums);
+  fits = fits && top_expand<T, NT, true, MULTI>(sh, k);
+  const RowSum s = rowsum_get<NT / kWave, kSumOnly>(mine, sh.sums);
+  if (!s.ok || !fits) {
     __syncthreads();
+    for (int i = tid; i < 2 * kTopMax; i += NT) sh.rank[i] = 0;
     top_row_walked<T, NT>(a, row, x, k, values, indices, lse, sh);
     return;
   }
   if (tid == 0 && lse) lse[row] = -rowsum_log_prob<false>(a, s, 0.f).hi;  // the log probability of a logit of 0
-  if (n > 2 * kTopMax) {
-    __syncthreads();
-    top_refine<NT>(sh, n, k);
-    n = k;
-  }
-  top_emit<T, NT>(sh.cand, n, x, row, k, values, indices);
+  top_emit<T, NT>(sh, sh.n, x, row, k, values, indices);
 }
 
 // ---- distillation from a teacher's largest logits ----------------------------------
@@ -613,11 +781,13 @@ int launch_top_logits(const VocabRows& a, int k, void* values, int32_t* indices,
   T* out = reinterpret_cast<T*>(values);
   const dim3 grid((unsigned)a.n_rows);
   if (sh.nt == 64)
-    hipLaunchKernelGGL((top_logits_kernel<T, 64, 4>), grid, dim3(64), 0, st, a, k, out, indices, lse);
+    hipLaunchKernelGGL((top_logits_kernel<T, 64, 4, false>), grid, dim3(64), 0, st, a, k, out, indices, lse);
   else if (sh.nt == 256)
-    hipLaunchKernelGGL((top_logits_kernel<T, 256, 4>), grid, dim3(256), 0, st, a, k, out, indices, lse);
+    hipLaunchKernelGGL((top_logits_kernel<T, 256, 4, false>), grid, dim3(256), 0, st, a, k, out, indices, lse);
+  else if (sh.nt == 512)
+    hipLaunchKernelGGL((top_logits_kernel<T, 512, 8, false>), grid, dim3(512), 0, st, a, k, out, indices, lse);
   else
-    hipLaunchKernelGGL((top_logits_kernel<T, 512, 8>), grid, dim3(512), 0, st, a, k, out, indices, lse);
+    hipLaunchKernelGGL((top_logits_kernel<T, 512, 8, true>), grid, dim3(512), 0, st, a, k, out, indices, lse);
   return check_launch();
 }
 

@@ -389,16 +389,20 @@ enum {
   kSumSecond = 2  // a = another sum of 2^(x k + c); the row's sum is z + a
 };
 
-// Merged over a workgroup of NW wavefronts; every thread gets the result.
-// `lds` holds NW RowSums and may be used again after another barrier.
+// Merged over a workgroup of NW wavefronts: each leaves its sums in `lds` (NW
+// RowSums), and after a barrier every thread gets the whole.
 template <int NW, int KIND>
-__device__ __forceinline__ RowSum rowsum_block(float c, float z, float a, RowSum* lds) {
+__device__ __forceinline__ RowSum rowsum_put(float c, float z, float a, RowSum* lds) {
   z = wave_sum(z);
   if (KIND != kSumOnly) a = wave_sum(a);
-  RowSum r{c, z, a, true};
+  const RowSum r{c, z, a, true};
+  if (NW > 1 && threadIdx.x % kWave == 0) lds[threadIdx.x / kWave] = r;
+  return r;
+}
+
+template <int NW, int KIND>
+__device__ __forceinline__ RowSum rowsum_get(RowSum r, const RowSum* lds) {
   if (NW > 1) {
-    if (threadIdx.x % kWave == 0) lds[threadIdx.x / kWave] = r;
-    __syncthreads();
     // lane i takes the sum of wavefront i % NW (all NW of them in every lane would need 3 NW registers)
     const RowSum w = lds[threadIdx.x % NW];
     float C = w.c;
@@ -415,6 +419,13 @@ __device__ __forceinline__ RowSum rowsum_block(float c, float z, float a, RowSum
   const float all = KIND == kSumSecond ? r.z + r.a : r.z;
   r.ok = all > 1e-30f && all < __builtin_inff() && r.c < kVrNoTerm;
   return r;
+}
+
+template <int NW, int KIND>
+__device__ __forceinline__ RowSum rowsum_block(float c, float z, float a, RowSum* lds) {
+  const RowSum r = rowsum_put<NW, KIND>(c, z, a, lds);
+  if (NW > 1) __syncthreads();
+  return rowsum_get<NW, KIND>(r, lds);
 }
 
 // ln of the soft-max probability of a logit of the row.  Without the sum a the
