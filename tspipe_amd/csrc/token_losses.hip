@@ -56,7 +56,8 @@ struct TokenGrad {
 template <typename T, int NT, int KREG>
 __global__ __launch_bounds__(NT) void token_stat_kernel(const TokenRows a, int64_t row0, const float* __restrict__ ref,
                                                         float* __restrict__ logp, double* __restrict__ log_ratio,
-                                                        float2* __restrict__ stats) {
+                                                        float2* __restrict__ stats, unsigned* __restrict__ ticket) {
+  if (ticket && blockIdx.x == 0 && threadIdx.x == 0) *ticket = 0u;  // of the next kernel
   constexpr int VEC = Vec16<T>::N;
   __shared__ RowSum lds[NT / kWave];
   __shared__ VocabStat lds_v[NT / kWave];
@@ -74,6 +75,7 @@ __global__ __launch_bounds__(NT) void token_stat_kernel(const TokenRows a, int64
   const int64_t V = a.r.V;
   const float k = a.r.k;
   const VocabGeom g = vocab_geom(srow, V);
+  const T label_logit = srow[label];
   RowRegs<T, NT, KREG> r;
   regs_load(r, srow, V, g);
   const float c = regs_anchor(r, g, k);
@@ -108,12 +110,12 @@ __global__ __launch_bounds__(NT) void token_stat_kernel(const TokenRows a, int64
   float2 st;
   if (s.ok) {
     if (threadIdx.x != 0) return;
-    lp = rowsum_log_prob<true>(a.r, s, to_f32(srow[label]));
+    lp = rowsum_log_prob<true>(a.r, s, to_f32(label_logit));
     st = make_float2(s.c, s.z);
   } else {
     const VocabStat sv = vstat_block<NT / kWave>(vocab_stat_walk<T, NT>(srow, V, k), k, lds_v);
     if (threadIdx.x != 0) return;
-    lp = vstat_log_prob(a.r, sv, to_f32(srow[label]));
+    lp = vstat_log_prob(a.r, sv, to_f32(label_logit));
     st = make_float2(sv.m, -sv.z);
   }
   if (logp) logp[row] = lp.hi;
@@ -209,14 +211,17 @@ struct PrefArgs {
   float* rewards;       // per sequence, may be null
   float* coef;          // per sequence
   double* pair_loss;    // per pair
+  unsigned* ticket;
+  float* loss;
 };
 
 __device__ __forceinline__ double softplus_f64(double x) { return fmax(x, 0.0) + log1p(exp(-fabs(x))); }
 
 // One workgroup per pair: both sequences' sums, the pair's loss and the factors
-// c of its two sequences.
+// c of its two sequences; the last one takes the mean of all pairs' losses.
 __global__ __launch_bounds__(kTokBlock) void pref_join_kernel(const TokenRows a, const PrefArgs p, int64_t pairs) {
   __shared__ double lds[kTokBlock / kWave];
+  __shared__ bool last;
   const int64_t pair = blockIdx.x, L = a.r.seq_len;
   double R[2], n[2];
   for (int side = 0; side < 2; ++side) {
@@ -233,35 +238,46 @@ __global__ __launch_bounds__(kTokBlock) void pref_join_kernel(const TokenRows a,
     n[side] = p.average ? fmax(block_sum_f64<kTokBlock / kWave>(c, lds), 1.0) : 1.0;
     R[side] = R[side] / n[side] - (p.ref_seq ? (double)p.ref_seq[2 * pair + side] : 0.0);
   }
-  if (threadIdx.x != 0) return;
-  const double h = R[0] - R[1], bh = p.beta * h;
-  double loss, slope;  // slope = d loss / d h
-  if (p.kind == kPrefSigmoid) {
-    loss = (1.0 - p.smoothing) * softplus_f64(-bh) + p.smoothing * softplus_f64(bh);
-    slope = p.beta * (p.smoothing - 1.0 / (1.0 + exp(bh)));
-  } else if (p.kind == kPrefHinge) {
-    loss = bh < 1.0 ? 1.0 - bh : (bh >= 1.0 ? 0.0 : bh);  // (a NaN stays one)
-    slope = bh < 1.0 ? -p.beta : 0.0;
-  } else {
-    const double e = h - 0.5 / p.beta;
-    loss = e * e;
-    slope = 2.0 * e;
+  if (threadIdx.x == 0) {
+    const double h = R[0] - R[1], bh = p.beta * h;
+    double loss, slope;  // slope = d loss / d h
+    if (p.kind == kPrefSigmoid) {
+      loss = (1.0 - p.smoothing) * softplus_f64(-bh) + p.smoothing * softplus_f64(bh);
+      slope = p.beta * (p.smoothing - 1.0 / (1.0 + exp(bh)));
+    } else if (p.kind == kPrefHinge) {
+      loss = bh < 1.0 ? 1.0 - bh : (bh >= 1.0 ? 0.0 : bh);  // (a NaN stays one)
+      slope = bh < 1.0 ? -p.beta : 0.0;
+    } else {
+      const double e = h - 0.5 / p.beta;
+      loss = e * e;
+      slope = 2.0 * e;
+    }
+    const double c = slope * p.weight / (double)pairs;
+    for (int side = 0; side < 2; ++side) {
+      p.coef[2 * pair + side] = (float)((side ? -c : c) / n[side]);
+      if (p.rewards) p.rewards[2 * pair + side] = (float)(p.beta * R[side]);
+    }
+    last = publish_term(p.pair_loss + pair, loss, p.ticket, pairs);
   }
-  p.pair_loss[pair] = loss;
-  const double c = slope * p.weight / (double)pairs;
-  for (int side = 0; side < 2; ++side) {
-    p.coef[2 * pair + side] = (float)((side ? -c : c) / n[side]);
-    if (p.rewards) p.rewards[2 * pair + side] = (float)(p.beta * R[side]);
-  }
+  __syncthreads();
+  if (!last) return;
+  const double s = sum_terms<kTokBlock>(p.pair_loss, pairs, lds);
+  if (threadIdx.x == 0) *p.loss = (float)(s * p.weight / (double)pairs);
 }
 
-// out = scale * sum(v) / denom; NaN when there is nothing to average.
-__global__ __launch_bounds__(1024) void sum_f64_kernel(const double* __restrict__ v, int64_t n, double scale,
-                                                       const int* __restrict__ live, float* __restrict__ out) {
+// The mean over nothing.
+__global__ void nan_kernel(float* __restrict__ out) { *out = __builtin_nanf(""); }
+
+// out = the sum of the rows' terms; without a row that counts the mean is one over nothing.
+__global__ __launch_bounds__(1024) void policy_sum_kernel(const double* __restrict__ v, int64_t n,
+                                                          const int* __restrict__ live, float* __restrict__ out) {
   __shared__ double lds[1024 / kWave];
   const double s = block_sum_f64<1024 / kWave>(thread_share_of_sum_f64<1024>(v, n), lds);
-  if (threadIdx.x == 0) *out = (live ? *live != 0 : n != 0) ? (float)(s * scale) : __builtin_nanf("");
+  if (threadIdx.x == 0) *out = *live > 0 ? (float)s : __builtin_nanf("");
 }
+
+// Clears a ticket counter where no other kernel runs in front.
+__global__ void clear_ticket_kernel(unsigned* __restrict__ ticket) { *ticket = 0u; }
 
 // ---- clipped policy loss ------------------------------------------------------
 
@@ -330,29 +346,43 @@ __device__ __forceinline__ void policy_term(const PolicyArgs& p, Float2x lp, flo
   }
 }
 
+// A row's numbers besides its logits, fetched before them: after the row's sum
+// they would be waited for with the row's registers held.
+template <typename T>
+struct PolicyRow {
+  float old_lp, ref_lp, adv, weight;
+  T label_logit;
+  __device__ __forceinline__ PolicyRow(const TokenRows& a, const PolicyArgs& p, int64_t row, const T* srow, int64_t label) {
+    const int64_t seq = (uint32_t)row / (uint32_t)a.r.seq_len;
+    old_lp = scalar_load(p.old_logp + row);
+    ref_lp = p.ref_logp ? scalar_load(p.ref_logp + row) : 0.f;
+    adv = scalar_load(p.adv + (p.adv_per_seq ? seq : row));
+    weight = scalar_load(p.seq_weight + seq);
+    label_logit = srow[label];
+  }
+};
+
 // What one thread of a row's workgroup does with the row's log probability:
 // outputs, and the factor of its gradient.
-__device__ __forceinline__ float policy_finish(const TokenRows& a, const PolicyArgs& p, int64_t row, Float2x lp) {
-  const int64_t seq = row / a.r.seq_len;
+template <typename T>
+__device__ __forceinline__ float policy_finish(const TokenRows& a, const PolicyArgs& p, const PolicyRow<T>& r,
+                                               int64_t row, Float2x lp) {
   float term, slope;
-  policy_term(p, lp, p.old_logp[row], p.ref_logp ? p.ref_logp[row] : 0.f, p.adv[p.adv_per_seq ? seq : row], &term,
-              &slope);
-  const float w = p.seq_weight[seq];
+  policy_term(p, lp, r.old_lp, r.ref_lp, r.adv, &term, &slope);
   if (p.logp) p.logp[row] = lp.hi;
-  p.row_loss[row] = (double)w * (double)term;
-  return w * slope * (float)a.r.inv_T;
+  p.row_loss[row] = (double)r.weight * (double)term;
+  return r.weight * slope * (float)a.r.inv_T;
 }
 
 // Rows whose sum needs the true maximum, and rows too long for registers: two
 // walks over the row.
 template <typename T, int NT>
-__device__ __forceinline__ void policy_row_walked(const TokenRows& a, const PolicyArgs& p, int64_t row, const T* srow,
-                                                  T* grow, int64_t label) {
+__device__ __forceinline__ void policy_row_walked(const TokenRows& a, const PolicyArgs& p, const PolicyRow<T>& pr,
+                                                  int64_t row, const T* srow, T* grow, int64_t label, float& coef) {
   __shared__ VocabStat lds[NT / kWave];
-  __shared__ float coef;
   const float k = a.r.k;
   const VocabStat s = vstat_block<NT / kWave>(vocab_stat_walk<T, NT>(srow, a.r.V, k), k, lds);
-  if (threadIdx.x == 0) coef = policy_finish(a, p, row, vstat_log_prob(a.r, s, to_f32(srow[label])));
+  if (threadIdx.x == 0) coef = policy_finish(a, p, pr, row, vstat_log_prob(a.r, s, to_f32(pr.label_logit)));
   if (!grow) return;
   __syncthreads();
   const TokenGrad f(k, make_float2(s.m, -s.z), coef);
@@ -378,13 +408,14 @@ __global__ __launch_bounds__(NT) void policy_rows_kernel(const TokenRows a, cons
     return;
   }
   const T* srow = vocab_row<T>(a.r, row);
+  const PolicyRow<T> pr(a, p, row, srow, label);
   if constexpr (KREG > 0) {
     const VocabGeom g = vocab_geom(srow, V);
     RowRegs<T, NT, KREG> r;
     regs_load(r, srow, V, g);
     const RowSum s = regs_sum<T, NT, KREG>(r, g, a.r.k, lds);
     if (s.ok) {
-      if (threadIdx.x == 0) coef = policy_finish(a, p, row, rowsum_log_prob<false>(a.r, s, to_f32(srow[label])));
+      if (threadIdx.x == 0) coef = policy_finish(a, p, pr, row, rowsum_log_prob<false>(a.r, s, to_f32(pr.label_logit)));
       if (!grow) return;
       __syncthreads();
       const TokenGrad f(a.r.k, make_float2(s.c, s.z), coef);
@@ -392,7 +423,7 @@ __global__ __launch_bounds__(NT) void policy_rows_kernel(const TokenRows a, cons
       return;
     }
   }
-  policy_row_walked<T, NT>(a, p, row, srow, grow, label);
+  policy_row_walked<T, NT>(a, p, pr, row, srow, grow, label, coef);
 }
 
 // ---- host side ------------------------------------------------------------------
@@ -428,11 +459,11 @@ inline TokenWs token_carve(void* ws, int64_t n_rows, int64_t n_seq) {
 
 template <typename T>
 int launch_token_stat(const TokenRows& a, int64_t row0, int64_t rows, const float* ref, float* logp, double* log_ratio,
-                      float2* stats, hipStream_t st) {
+                      float2* stats, unsigned* ticket, hipStream_t st) {
   const RowShape sh = row_shape<T>(a.r.V);
 #define TS_STAT(NT, KREG)                                                                                        \
   hipLaunchKernelGGL((token_stat_kernel<T, NT, KREG>), dim3((unsigned)rows), dim3(NT), 0, st, a, row0, ref, logp, \
-                     log_ratio, stats)
+                     log_ratio, stats, ticket)
   if (sh.nt == 64)
     TS_STAT(64, 4);
   else if (sh.nt == 256)
@@ -462,22 +493,31 @@ int launch_token_grad(const TokenRows& a, int64_t row0, int64_t rows, const floa
   return TS_OK;
 }
 
+inline int launch_nan(float* out, hipStream_t st) {
+  hipLaunchKernelGGL(nan_kernel, dim3(1), dim3(1), 0, st, out);
+  return check_launch();
+}
+
+// Three launches: the rows' log ratios, the pairs (which need whole sequences of
+// them), the gradient.  The logits are read twice, 734 + 524 MB at 16 sequences
+// of 512 x 32000 bf16 with 70 % of the rows counting.  (Pair by pair, so that the
+// second reading finds the rows in the last-level cache, is no faster: the
+// gradient's writes bound that kernel, 34 us for two pairs either way, and the
+// smaller launches cost more than they save, 275 against 226 us in all.)
 template <typename T>
-int launch_preference(const TokenRows& a, const float* ref_tok, PrefArgs p, const TokenWs& w, int64_t n_seq,
-                      float* loss_out, void* grad, hipStream_t st) {
+int launch_preference(const TokenRows& a, const float* ref_tok, const PrefArgs& p, const TokenWs& w, int64_t n_seq,
+                      void* grad, hipStream_t st) {
   const int64_t pairs = n_seq / 2;
-  int rc = TS_OK;
+  if (pairs == 0) return launch_nan(p.loss, st);
+  int rc;
   if (a.r.n_rows > 0) {
-    rc = launch_token_stat<T>(a, 0, a.r.n_rows, ref_tok, nullptr, w.row, w.stats, st);
-    if (rc) return rc;
-  }
-  if (pairs > 0) {
-    hipLaunchKernelGGL(pref_join_kernel, dim3((unsigned)pairs), dim3(kTokBlock), 0, st, a, p, pairs);
+    rc = launch_token_stat<T>(a, 0, a.r.n_rows, ref_tok, nullptr, w.row, w.stats, p.ticket, st);
+  } else {
+    hipLaunchKernelGGL(clear_ticket_kernel, dim3(1), dim3(1), 0, st, p.ticket);
     rc = check_launch();
-    if (rc) return rc;
   }
-  hipLaunchKernelGGL(sum_f64_kernel, dim3(1), dim3(1024), 0, st, w.pair, pairs, pairs ? p.weight / (double)pairs : 0.0,
-                     (const int*)nullptr, loss_out);
+  if (rc) return rc;
+  hipLaunchKernelGGL(pref_join_kernel, dim3((unsigned)pairs), dim3(kTokBlock), 0, st, a, p, pairs);
   rc = check_launch();
   if (rc || !grad || a.r.n_rows == 0) return rc;
   return launch_token_grad<T>(a, 0, a.r.n_rows, w.stats, w.seq, 1, grad, st);
@@ -486,29 +526,27 @@ int launch_preference(const TokenRows& a, const float* ref_tok, PrefArgs p, cons
 template <typename T>
 int launch_policy(const TokenRows& a, const PolicyArgs& p, const TokenWs& w, int64_t n_seq, int per_seq, float weight,
                   float* loss_out, hipStream_t st) {
-  hipLaunchKernelGGL(policy_weight_kernel, dim3(1), dim3(1024), 0, st, a, a.r.seq_len ? n_seq : 0, per_seq, weight,
-                     w.seq, w.counts);
+  if (a.r.n_rows == 0) return launch_nan(loss_out, st);
+  hipLaunchKernelGGL(policy_weight_kernel, dim3(1), dim3(1024), 0, st, a, n_seq, per_seq, weight, w.seq, w.counts);
   int rc = check_launch();
   if (rc) return rc;
-  if (a.r.n_rows > 0) {
-    const dim3 grid((unsigned)a.r.n_rows);
-    const RowShape sh = row_shape<T>(a.r.V);
-    if (sh.nt == 64)
-      hipLaunchKernelGGL((policy_rows_kernel<T, 64, 4>), grid, dim3(64), 0, st, a, p);
-    else if (sh.nt == 256)
-      hipLaunchKernelGGL((policy_rows_kernel<T, 256, 4>), grid, dim3(256), 0, st, a, p);
-    else if (sh.nt == 512)
-      hipLaunchKernelGGL((policy_rows_kernel<T, 512, 8>), grid, dim3(512), 0, st, a, p);
-    else if (sh.kreg == 8)
-      hipLaunchKernelGGL((policy_rows_kernel<T, 1024, 8>), grid, dim3(1024), 0, st, a, p);
-    else if (sh.kreg == 16)
-      hipLaunchKernelGGL((policy_rows_kernel<T, 1024, 16>), grid, dim3(1024), 0, st, a, p);
-    else
-      hipLaunchKernelGGL((policy_rows_kernel<T, 1024, 0>), grid, dim3(1024), 0, st, a, p);
-    rc = check_launch();
-    if (rc) return rc;
-  }
-  hipLaunchKernelGGL(sum_f64_kernel, dim3(1), dim3(1024), 0, st, w.row, a.r.n_rows, 1.0, (const int*)w.counts, loss_out);
+  const dim3 grid((unsigned)a.r.n_rows);
+  const RowShape sh = row_shape<T>(a.r.V);
+  if (sh.nt == 64)
+    hipLaunchKernelGGL((policy_rows_kernel<T, 64, 4>), grid, dim3(64), 0, st, a, p);
+  else if (sh.nt == 256)
+    hipLaunchKernelGGL((policy_rows_kernel<T, 256, 4>), grid, dim3(256), 0, st, a, p);
+  else if (sh.nt == 512)
+    hipLaunchKernelGGL((policy_rows_kernel<T, 512, 8>), grid, dim3(512), 0, st, a, p);
+  else if (sh.kreg == 8)
+    hipLaunchKernelGGL((policy_rows_kernel<T, 1024, 8>), grid, dim3(1024), 0, st, a, p);
+  else if (sh.kreg == 16)
+    hipLaunchKernelGGL((policy_rows_kernel<T, 1024, 16>), grid, dim3(1024), 0, st, a, p);
+  else
+    hipLaunchKernelGGL((policy_rows_kernel<T, 1024, 0>), grid, dim3(1024), 0, st, a, p);
+  rc = check_launch();
+  if (rc) return rc;
+  hipLaunchKernelGGL(policy_sum_kernel, dim3(1), dim3(1024), 0, st, w.row, a.r.n_rows, (const int*)w.counts, loss_out);
   return check_launch();
 }
 
@@ -548,7 +586,7 @@ int ts_token_logp_fwd(const void* s, int64_t n_seq, int64_t seq_len, int64_t V, 
   const ts::TokenRows a =
       ts::token_rows(s, n_seq, seq_len, V, ld_seq, ld_tok, labels, row_mask, ignore_index, temperature);
   hipStream_t st = (hipStream_t)stream;
-  TS_BY_DTYPE(dtype, (ts::launch_token_stat<T>(a, 0, a.r.n_rows, nullptr, logp, nullptr, (float2*)stats, st)))
+  TS_BY_DTYPE(dtype, (ts::launch_token_stat<T>(a, 0, a.r.n_rows, nullptr, logp, nullptr, (float2*)stats, nullptr, st)))
 }
 
 int ts_token_logp_bwd(const void* s, int64_t n_seq, int64_t seq_len, int64_t V, int64_t ld_seq, int64_t ld_tok,
@@ -597,9 +635,11 @@ int ts_preference_fwd_bwd(const void* s, int64_t n_seq, int64_t seq_len, int64_t
   p.rewards = rewards;
   p.coef = w.seq;
   p.pair_loss = w.pair;
+  p.ticket = reinterpret_cast<unsigned*>(w.counts);
+  p.loss = loss_out;
   const float* ref_tok = ref_per_token ? ref_logp : nullptr;
   hipStream_t st = (hipStream_t)stream;
-  TS_BY_DTYPE(dtype, (ts::launch_preference<T>(a, ref_tok, p, w, n_seq, loss_out, grad, st)))
+  TS_BY_DTYPE(dtype, (ts::launch_preference<T>(a, ref_tok, p, w, n_seq, grad, st)))
 }
 
 int ts_policy_fwd_bwd(const void* s, int64_t n_seq, int64_t seq_len, int64_t V, int64_t ld_seq, int64_t ld_tok,

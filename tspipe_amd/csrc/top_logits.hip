@@ -602,8 +602,13 @@ struct TopDistilShared {
 __device__ __forceinline__ uint32_t top_mark_bit(int j, const VocabGeom& g) { return (uint32_t)(j - g.head + 8); }
 
 // KREG = 0: the row is walked for its sums and again for its gradient.
+//
+// 64 registers a thread for up to eight vectors of a row, but for the 512-thread
+// arrangement, which would spill there: with six wavefronts a SIMD instead of
+// eight 4096 x 30522 bf16 takes 88 us instead of 99.
 template <typename T, int NT, int KREG, bool TAIL>
-__global__ __launch_bounds__(NT, (KREG > 8 ? 4 : NT > 256 ? (NT > 512 ? 8 : 6) : 1)) void top_distil_kernel(const TopDistilArgs a) {
+__global__ __launch_bounds__(NT, (KREG > 8 ? 4 : NT > 256 ? (NT > 512 ? 8 : 6) : 1)) void top_distil_kernel(
+    const TopDistilArgs a) {
   constexpr int NW = NT / kWave, NE = (kTopMax + NT - 1) / NT, VEC = Vec16<T>::N;
   extern __shared__ uint32_t marks[];  // TAIL: a bit per vocabulary entry
   __shared__ TopDistilShared<NT> sh;
@@ -886,9 +891,8 @@ int ts_top_distil_fwd_bwd(const void* s, int64_t n_seq, int64_t seq_len, int64_t
   a.row_loss = reinterpret_cast<double*>(ws + 16 + a.r.n_rows * 16);
   a.entry_p = reinterpret_cast<float*>(ws + 16 + a.r.n_rows * 24);
   a.grad = grad;
-  const double scale = weight * temperature * temperature;
   hipStream_t st = (hipStream_t)stream;
-  TS_BY_DTYPE(dtype, (ts::launch_top_distil<T>(a, scale, loss_out, st)))
+  TS_BY_DTYPE(dtype, (ts::launch_top_distil<T>(a, weight * temperature * temperature, loss_out, st)))
 }
 
 }  // extern "C"

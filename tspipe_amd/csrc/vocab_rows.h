@@ -508,8 +508,24 @@ __device__ __forceinline__ void regs_map(RowRegs<T, NT, KREG>& r, const VocabGeo
   }
 }
 
-// This thread's share of sum(v[0..n)) when NT threads walk the array together, in a
-// fixed order, eight loads in flight each.
+// Sum of doubles over a workgroup of NW wavefronts, in a fixed order; every
+// thread gets the result.
+template <int NW>
+__device__ __forceinline__ double block_sum_f64(double v, double* lds) {
+#pragma unroll
+  for (int off = kWave / 2; off > 0; off >>= 1) v += __shfl_xor(v, off, kWave);
+  if (NW == 1) return v;
+  __syncthreads();
+  if (threadIdx.x % kWave == 0) lds[threadIdx.x / kWave] = v;
+  __syncthreads();
+  double r = lds[threadIdx.x % NW];
+#pragma unroll
+  for (int off = NW / 2; off > 0; off >>= 1) r += __shfl_xor(r, off, kWave);
+  return r;
+}
+
+// This thread's share of sum(v[0..n)) when NT threads walk the array together, in
+// a fixed order, eight loads in flight each.
 template <int NT>
 __device__ __forceinline__ double thread_share_of_sum_f64(const double* __restrict__ v, int64_t n) {
   constexpr int kInFlight = 8;
@@ -527,6 +543,43 @@ __device__ __forceinline__ double thread_share_of_sum_f64(const double* __restri
   return s;
 }
 
+// ---- sums over workgroups without a launch of their own ------------------------
+// Every workgroup publishes one term and draws a ticket; the one that draws the
+// last adds all the terms up, in the order of their places, so that the sum does
+// not depend on who that is.  The ticket counter is 0 when the kernel starts (a
+// kernel in front clears it).  For kernels of few workgroups: two chained
+// atomics in each of 8192 rows cost the policy loss 40 us, the launch it saves 5.
+
+// One thread: true for the last of `total` callers.  The exchange's old value is
+// waited for, so the term has arrived before the ticket is drawn.
+__device__ __forceinline__ bool publish_term(double* at, double term, unsigned* ticket, int64_t total) {
+  unsigned long long* p = reinterpret_cast<unsigned long long*>(at);
+  const unsigned long long old = __hip_atomic_exchange(p, (unsigned long long)__double_as_longlong(term),
+                                                       __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  asm volatile("" : : "v"((uint32_t)old), "v"((uint32_t)(old >> 32)) : "memory");
+  const unsigned drawn = __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  return drawn == (unsigned)(total - 1);
+}
+
+// The workgroup of the last caller: the sum of all terms, in every thread.
+template <int NT>
+__device__ __forceinline__ double sum_terms(const double* terms, int64_t n, double* lds) {
+  constexpr int kInFlight = 8;
+  const unsigned long long* p = reinterpret_cast<const unsigned long long*>(terms);
+  double s = 0.0;
+  for (int64_t i0 = threadIdx.x; i0 < n; i0 += (int64_t)NT * kInFlight) {
+    unsigned long long x[kInFlight];
+#pragma unroll
+    for (int j = 0; j < kInFlight; ++j) {
+      const int64_t i = i0 + (int64_t)j * NT;
+      x[j] = i < n ? __hip_atomic_load(p + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0ull;
+    }
+#pragma unroll
+    for (int j = 0; j < kInFlight; ++j) s += __longlong_as_double((long long)x[j]);
+  }
+  return block_sum_f64<NT / kWave>(s, lds);
+}
+
 // How a row of V elements of T is held: threads and vectors per thread of the
 // smallest arrangement it fits, 0 threads for rows that fit none.
 struct RowShape {
@@ -541,22 +594,6 @@ inline RowShape row_shape(int64_t V) {
   if (vecs <= 1024 * 8) return RowShape{1024, 8};
   if (vecs <= 1024 * 16) return RowShape{1024, 16};
   return RowShape{0, 0};
-}
-
-// Sum of doubles over a workgroup of NW wavefronts, in a fixed order; every
-// thread gets the result.
-template <int NW>
-__device__ __forceinline__ double block_sum_f64(double v, double* lds) {
-#pragma unroll
-  for (int off = kWave / 2; off > 0; off >>= 1) v += __shfl_xor(v, off, kWave);
-  if (NW == 1) return v;
-  __syncthreads();
-  if (threadIdx.x % kWave == 0) lds[threadIdx.x / kWave] = v;
-  __syncthreads();
-  double r = lds[threadIdx.x % NW];
-#pragma unroll
-  for (int off = NW / 2; off > 0; off >>= 1) r += __shfl_xor(r, off, kWave);
-  return r;
 }
 
 }  // namespace ts
