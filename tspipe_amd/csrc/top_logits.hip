@@ -501,45 +501,51 @@ __global__ __launch_bounds__(kTeacherBlock) void top_teacher_kernel(const TopDis
   const int64_t row = (int64_t)blockIdx.x * (kTeacherBlock / kWave) + w;
   const bool on = row < a.r.n_rows && !(a.mask && a.mask[row] == 0);
   int idx[NE];
-  double lp[NE];
-  float p[NE];
+  float v[NE], p[NE];
   float m = kVrLowest;
 #pragma unroll
   for (int i = 0; i < NE; ++i) {
     const int at = lane + i * kWave;
     idx[i] = -1;
-    float v = 0.f;
-    if (on && at < k) {
-      const int j = a.t_indices[row * k + at];
-      if (j >= 0 && j < a.r.V) {
-        idx[i] = j;
-        v = top_value(a.t_values, a.t_dtype, row * k + at);
-        m = fmaxf(m, v);
+    v[i] = p[i] = 0.f;
+    if (i * kWave < k) {  // uniform
+      if (on && at < k) {
+        idx[i] = a.t_indices[row * k + at];
+        v[i] = top_value(a.t_values, a.t_dtype, row * k + at);
+        if (idx[i] < 0 || idx[i] >= a.r.V) idx[i] = -1;
+        if (idx[i] >= 0) m = fmaxf(m, v[i]);
       }
     }
-    lp[i] = (double)v;
   }
-  m = wave_max(m);
-  double off = 0.0;
+  // p = e^(v / T - off) / z; without a log-sum-exp z is the entries' own sum
+  double off, z = 1.0;
   if (a.t_lse) {
-    if (on) off = (double)a.t_lse[row];
+    off = on ? (double)a.t_lse[row] : 0.0;
   } else {
-    double z = 0.0;
-#pragma unroll
-    for (int i = 0; i < NE; ++i)
-      if (idx[i] >= 0) z += exp((lp[i] - (double)m) * a.r.inv_T);
-    off = (double)m * a.r.inv_T + log(wave_sum_f64(z));
+    m = wave_max(m);
+    off = (double)m * a.r.inv_T;
+    z = 0.0;
   }
+  double pd[NE];
+#pragma unroll
+  for (int i = 0; i < NE; ++i) {
+    pd[i] = 0.0;
+    if (i * kWave < k && idx[i] >= 0 && v[i] != -__builtin_inff()) {
+      pd[i] = exp((double)v[i] * a.r.inv_T - off);
+      if (!a.t_lse) z += pd[i];
+    }
+  }
+  if (!a.t_lse) z = wave_sum_f64(z);
+  const double rz = z > 0.0 ? 1.0 / z : (z == 0.0 ? 0.0 : z), lz = off + (a.t_lse ? 0.0 : log(z));
   double sum = 0.0, p_ln_p = 0.0;
 #pragma unroll
   for (int i = 0; i < NE; ++i) {
-    const bool none = idx[i] < 0 || lp[i] == -__builtin_inf();
-    lp[i] = lp[i] * a.r.inv_T - off;
-    const double pd = none ? 0.0 : exp(lp[i]);
-    p[i] = (float)pd;
-    sum += pd;
-    // with p as it was rounded, so that p ln p - p ln q keeps its difference's accuracy
-    if (!none && p[i] != 0.f) p_ln_p += (double)p[i] * lp[i];
+    if (i * kWave < k) {
+      p[i] = (float)(pd[i] * rz);
+      sum += pd[i] * rz;
+      // with p as it was rounded, so that p ln p - p ln q keeps its difference's accuracy
+      if (p[i] != 0.f) p_ln_p += (double)p[i] * ((double)v[i] * a.r.inv_T - lz);
+    }
     ent_idx[w][lane + i * kWave] = idx[i];
     ent_p[w][lane + i * kWave] = p[i];
   }
@@ -547,12 +553,12 @@ __global__ __launch_bounds__(kTeacherBlock) void top_teacher_kernel(const TopDis
   p_ln_p = wave_sum_f64(p_ln_p);
   __syncthreads();
   // the same token named twice: the first naming stands for all of them.  Every entry is compared with
-  // all others, four at a read (one at a time this took 21 us for 1024 rows of 128 entries).
+  // all others, four at a read; only a second naming takes the branch.
   float all[NE];
   bool first[NE];
 #pragma unroll
   for (int i = 0; i < NE; ++i) {
-    all[i] = 0.f;
+    all[i] = p[i];
     first[i] = idx[i] >= 0;
   }
 #pragma unroll 4
@@ -562,12 +568,15 @@ __global__ __launch_bounds__(kTeacherBlock) void top_teacher_kernel(const TopDis
 #pragma unroll
     for (int i = 0; i < NE; ++i) {
       if (i * kWave >= k) break;  // uniform
-      const bool any = idx[i] == o[0] || idx[i] == o[1] || idx[i] == o[2] || idx[i] == o[3];
-      if (any && idx[i] >= 0) {
+      const int self = lane + i * kWave - q0;  // (out of 0..3 mostly)
+      bool again = false;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) again = again || (o[q] == idx[i] && q != self);
+      if (again && idx[i] >= 0) {
 #pragma unroll
         for (int q = 0; q < 4; ++q)
-          if (o[q] == idx[i]) {
-            first[i] = first[i] && q0 + q >= lane + i * kWave;
+          if (o[q] == idx[i] && q != self) {
+            first[i] = first[i] && q > self;
             all[i] += ent_p[w][q0 + q];
           }
       }
@@ -594,7 +603,6 @@ struct TopDistilShared {
   RowSum sums[NT / kWave];
   VocabStat stats[NT / kWave];
   double d[NT / kWave];
-  float go;  // factor of the other tokens' probabilities
 };
 
 // Bit of element j in the marks: vector v of the row owns bits 8 + v * VEC on, so
@@ -657,9 +665,16 @@ __global__ __launch_bounds__(NT, (KREG > 8 ? 4 : NT > 256 ? (NT > 512 ? 8 : 6) :
   }
   const TopTeacher t = scalar_load(a.teacher + row);
   const float gs = a.gscale / (float)scalar_load(a.live);
-  // Loss and gradient factor from the student's sums: lq(x) = ln of its probability of a logit x, and
-  // with TAIL the ln of what it leaves to the tokens without an entry, and one over that.
-  auto finish = [&](auto lq, Float2x lq_rest, float inv_q_rest) {
+  // Factor of the other tokens' probabilities in the gradient; inv_q_rest: one over what the student
+  // leaves to the tokens without an entry.
+  auto outside = [&](float inv_q_rest) {
+    float o = t.whole;
+    if (TAIL && t.rest > 0.f && inv_q_rest < __builtin_inff()) o = fmaf(-t.rest, inv_q_rest, o);
+    return gs * o;
+  };
+  // The row's loss, after its gradient (no wavefront waits for it): lq(x) = ln of the student's
+  // probability of a logit x, lq_rest that of all tokens without an entry.
+  auto loss = [&](auto lq, auto lq_rest) {
     double term = 0.0;
 #pragma unroll
     for (int i = 0; i < NE; ++i)
@@ -670,15 +685,12 @@ __global__ __launch_bounds__(NT, (KREG > 8 ? 4 : NT > 256 ? (NT > 512 ? 8 : 6) :
     term = block_sum_f64<NW>(term, sh.d);
     if (tid == 0) {
       term += t.p_ln_p;
-      float outside = t.whole;
       if (TAIL && t.rest > 0.f) {
-        term -= (double)t.rest * ((double)lq_rest.hi + (double)lq_rest.lo);
-        if (inv_q_rest < __builtin_inff()) outside = fmaf(-t.rest, inv_q_rest, outside);
+        const Float2x l = lq_rest();
+        term -= (double)t.rest * ((double)l.hi + (double)l.lo);
       }
       a.row_loss[row] = term;
-      sh.go = gs * outside;
     }
-    __syncthreads();
   };
   auto patch = [&](auto q_of) {  // the kept entries' gradients replace what the walk over the row wrote
     __syncthreads();
@@ -724,12 +736,13 @@ __global__ __launch_bounds__(NT, (KREG > 8 ? 4 : NT > 256 ? (NT > 512 ? 8 : 6) :
     if (s.ok) {
       const float rest_z = s.z;
       if (TAIL) s.z += s.a;
-      finish([&](float xv) { return rowsum_log_prob<false>(a.r, s, xv); },
-             TAIL ? ln_share(log2_2x(rest_z), s.z) : Float2x{0.f, 0.f}, s.z / rest_z);
-      if (!grow) return;
-      const float rz = 1.f / s.z, go = sh.go * rz, c = s.c;
-      regs_map(r, g, x, grow, V, -1, [=](float xv) { return go * fast_exp2(fmaf(xv, kk, c)); }, [](float) { return 0.f; });
-      patch([&](float xv) { return fast_exp2(fmaf(xv, kk, c)) * rz; });
+      if (grow) {
+        const float rz = 1.f / s.z, go = outside(s.z / rest_z) * rz, c = s.c;
+        regs_map(r, g, x, grow, V, -1, [=](float xv) { return go * fast_exp2(fmaf(xv, kk, c)); },
+                 [](float) { return 0.f; });
+        patch([&](float xv) { return fast_exp2(fmaf(xv, kk, c)) * rz; });
+      }
+      loss([&](float xv) { return rowsum_log_prob<false>(a.r, s, xv); }, [&]() { return ln_share(log2_2x(rest_z), s.z); });
       return;
     }
     __syncthreads();
@@ -765,11 +778,12 @@ __global__ __launch_bounds__(NT, (KREG > 8 ? 4 : NT > 256 ? (NT > 512 ? 8 : 6) :
       lq_rest.hi = -__builtin_inff();
     inv_q_rest = fast_exp2(-e.hi) * (all.z / out.z);
   }
-  finish([&](float xv) { return vstat_log_prob(a.r, all, xv); }, lq_rest, inv_q_rest);
-  if (!grow) return;
-  const float rz = 1.f / all.z, go = sh.go * rz, m = all.m;
-  vocab_map_walk<T, NT>(x, grow, V, [=](float xv, int) { return go * fast_exp2((xv - m) * kk); });
-  patch([&](float xv) { return fast_exp2((xv - m) * kk) * rz; });
+  if (grow) {
+    const float rz = 1.f / all.z, go = outside(inv_q_rest) * rz, m = all.m;
+    vocab_map_walk<T, NT>(x, grow, V, [=](float xv, int) { return go * fast_exp2((xv - m) * kk); });
+    patch([&](float xv) { return fast_exp2((xv - m) * kk) * rz; });
+  }
+  loss([&](float xv) { return vstat_log_prob(a.r, all, xv); }, [&]() { return lq_rest; });
 }
 
 __global__ __launch_bounds__(1024) void top_distil_sum_kernel(const double* __restrict__ v, int64_t n,
