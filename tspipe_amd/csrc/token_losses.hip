@@ -352,6 +352,7 @@ template <typename T>
 struct PolicyRow {
   float old_lp, ref_lp, adv, weight;
   T label_logit;
+  __device__ __forceinline__ PolicyRow() {}
   __device__ __forceinline__ PolicyRow(const TokenRows& a, const PolicyArgs& p, int64_t row, const T* srow, int64_t label) {
     const int64_t seq = (uint32_t)row / (uint32_t)a.r.seq_len;
     old_lp = scalar_load(p.old_logp + row);
@@ -362,8 +363,8 @@ struct PolicyRow {
   }
 };
 
-// What one thread of a row's workgroup does with the row's log probability:
-// outputs, and the factor of its gradient.
+// What one thread does with a row's log probability: outputs, and the factor of
+// its gradient.
 template <typename T>
 __device__ __forceinline__ float policy_finish(const TokenRows& a, const PolicyArgs& p, const PolicyRow<T>& r,
                                                int64_t row, Float2x lp) {
@@ -374,8 +375,7 @@ __device__ __forceinline__ float policy_finish(const TokenRows& a, const PolicyA
   return r.weight * slope * (float)a.r.inv_T;
 }
 
-// Rows whose sum needs the true maximum, and rows too long for registers: two
-// walks over the row.
+// Rows whose sum needs the true maximum: two walks over the row.
 template <typename T, int NT>
 __device__ __forceinline__ void policy_row_walked(const TokenRows& a, const PolicyArgs& p, const PolicyRow<T>& pr,
                                                   int64_t row, const T* srow, T* grow, int64_t label, float& coef) {
@@ -390,8 +390,7 @@ __device__ __forceinline__ void policy_row_walked(const TokenRows& a, const Poli
 }
 
 // A row's factor c follows from the row itself, so the row stays in registers
-// between its sum and its gradient and is read once.  KREG = 0: the row is
-// walked twice.
+// between its sum and its gradient and is read once.
 template <typename T, int NT, int KREG>
 __global__ __launch_bounds__(NT) void policy_rows_kernel(const TokenRows a, const PolicyArgs p) {
   __shared__ RowSum lds[NT / kWave];
@@ -409,21 +408,49 @@ __global__ __launch_bounds__(NT) void policy_rows_kernel(const TokenRows a, cons
   }
   const T* srow = vocab_row<T>(a.r, row);
   const PolicyRow<T> pr(a, p, row, srow, label);
-  if constexpr (KREG > 0) {
-    const VocabGeom g = vocab_geom(srow, V);
-    RowRegs<T, NT, KREG> r;
-    regs_load(r, srow, V, g);
-    const RowSum s = regs_sum<T, NT, KREG>(r, g, a.r.k, lds);
-    if (s.ok) {
-      if (threadIdx.x == 0) coef = policy_finish(a, p, pr, row, rowsum_log_prob<false>(a.r, s, to_f32(pr.label_logit)));
-      if (!grow) return;
-      __syncthreads();
-      const TokenGrad f(a.r.k, make_float2(s.c, s.z), coef);
-      regs_map(r, g, srow, grow, V, (int)label, [&](float x) { return f.other(x); }, [&](float x) { return f.label(x); });
-      return;
-    }
+  const VocabGeom g = vocab_geom(srow, V);
+  RowRegs<T, NT, KREG> r;
+  regs_load(r, srow, V, g);
+  const RowSum s = regs_sum(r, g, a.r.k, lds);
+  if (s.ok) {
+    if (threadIdx.x == 0) coef = policy_finish(a, p, pr, row, rowsum_log_prob<false>(a.r, s, to_f32(pr.label_logit)));
+    if (!grow) return;
+    __syncthreads();
+    const TokenGrad f(a.r.k, make_float2(s.c, s.z), coef);
+    regs_map(r, g, srow, grow, V, (int)label, [&](float x) { return f.other(x); }, [&](float x) { return f.label(x); });
+    return;
   }
+  __syncthreads();
   policy_row_walked<T, NT>(a, p, pr, row, srow, grow, label, coef);
+}
+
+// Rows too long for registers go through the kernels of the log probabilities
+// and their gradient, with this one between them: the factor of each row, one
+// thread a row.  (One workgroup that reads its row twice: 332 us for 1900 x
+// 140000 bf16, this way 283.)
+template <typename T>
+__global__ __launch_bounds__(kTokBlock) void policy_coef_kernel(const TokenRows a, const PolicyArgs p,
+                                                                const double* __restrict__ lp, float* __restrict__ coef) {
+  const int64_t row = (int64_t)blockIdx.x * kTokBlock + threadIdx.x;
+  if (row >= a.r.n_rows) return;
+  int64_t label;
+  if (!token_live<false>(a, row, &label)) {
+    if (p.logp) p.logp[row] = 0.f;
+    p.row_loss[row] = 0.0;
+    coef[row] = 0.f;
+    return;
+  }
+  const int64_t seq = row / a.r.seq_len;
+  const double l = lp[row];
+  const float hi = (float)l;
+  PolicyRow<T> r;
+  r.old_lp = p.old_logp[row];
+  r.ref_lp = p.ref_logp ? p.ref_logp[row] : 0.f;
+  r.adv = p.adv[p.adv_per_seq ? seq : row];
+  r.weight = p.seq_weight[seq];
+  // (the gradient kernel takes the temperature itself)
+  coef[row] = policy_finish(a, p, r, row, Float2x{hi, fabsf(hi) < __builtin_inff() ? (float)(l - (double)hi) : 0.f}) /
+              (float)a.r.inv_T;
 }
 
 // ---- host side ------------------------------------------------------------------
@@ -433,13 +460,16 @@ inline size_t pad16(size_t b) { return (b + 15) / 16 * 16; }
 struct TokenWs {
   double* row;     // n_rows: log ratios or loss terms
   float2* stats;   // n_rows
+  double* lp;      // n_rows: log probabilities
+  float* coef;     // n_rows: gradient factors
   double* pair;    // n_seq / 2
   float* seq;      // n_seq: factors or weights
   int* counts;     // 4
 };
 
 inline size_t token_ws_bytes(int64_t n_rows, int64_t n_seq) {
-  return 16 + pad16((size_t)n_rows * 8) * 2 + pad16((size_t)(n_seq / 2) * 8) + pad16((size_t)n_seq * 4);
+  return 16 + pad16((size_t)n_rows * 8) * 3 + pad16((size_t)n_rows * 4) + pad16((size_t)(n_seq / 2) * 8) +
+         pad16((size_t)n_seq * 4);
 }
 
 inline TokenWs token_carve(void* ws, int64_t n_rows, int64_t n_seq) {
@@ -451,6 +481,10 @@ inline TokenWs token_carve(void* ws, int64_t n_rows, int64_t n_seq) {
   b += pad16((size_t)n_rows * 8);
   w.stats = reinterpret_cast<float2*>(b);
   b += pad16((size_t)n_rows * 8);
+  w.lp = reinterpret_cast<double*>(b);
+  b += pad16((size_t)n_rows * 8);
+  w.coef = reinterpret_cast<float*>(b);
+  b += pad16((size_t)n_rows * 4);
   w.pair = reinterpret_cast<double*>(b);
   b += pad16((size_t)(n_seq / 2) * 8);
   w.seq = reinterpret_cast<float*>(b);
@@ -466,8 +500,10 @@ int launch_token_stat(const TokenRows& a, int64_t row0, int64_t rows, const floa
                      log_ratio, stats, ticket)
   if (sh.nt == 64)
     TS_STAT(64, 4);
-  else if (sh.nt == 256)
+  else if (sh.nt == 256 && sh.kreg == 4)
     TS_STAT(256, 4);
+  else if (sh.nt == 256)
+    TS_STAT(256, 8);
   else
     TS_STAT(512, 8);
 #undef TS_STAT
@@ -532,18 +568,30 @@ int launch_policy(const TokenRows& a, const PolicyArgs& p, const TokenWs& w, int
   if (rc) return rc;
   const dim3 grid((unsigned)a.r.n_rows);
   const RowShape sh = row_shape<T>(a.r.V);
+#define TS_POLICY(NT, KREG) hipLaunchKernelGGL((policy_rows_kernel<T, NT, KREG>), grid, dim3(NT), 0, st, a, p)
   if (sh.nt == 64)
-    hipLaunchKernelGGL((policy_rows_kernel<T, 64, 4>), grid, dim3(64), 0, st, a, p);
+    TS_POLICY(64, 4);
+  else if (sh.nt == 256 && sh.kreg == 4)
+    TS_POLICY(256, 4);
   else if (sh.nt == 256)
-    hipLaunchKernelGGL((policy_rows_kernel<T, 256, 4>), grid, dim3(256), 0, st, a, p);
+    TS_POLICY(256, 8);
   else if (sh.nt == 512)
-    hipLaunchKernelGGL((policy_rows_kernel<T, 512, 8>), grid, dim3(512), 0, st, a, p);
+    TS_POLICY(512, 8);
   else if (sh.kreg == 8)
-    hipLaunchKernelGGL((policy_rows_kernel<T, 1024, 8>), grid, dim3(1024), 0, st, a, p);
+    TS_POLICY(1024, 8);
   else if (sh.kreg == 16)
-    hipLaunchKernelGGL((policy_rows_kernel<T, 1024, 16>), grid, dim3(1024), 0, st, a, p);
-  else
-    hipLaunchKernelGGL((policy_rows_kernel<T, 1024, 0>), grid, dim3(1024), 0, st, a, p);
+    TS_POLICY(1024, 16);
+  else {
+    rc = launch_token_stat<T>(a, 0, a.r.n_rows, nullptr, nullptr, w.lp, w.stats, nullptr, st);
+    if (rc) return rc;
+    hipLaunchKernelGGL((policy_coef_kernel<T>), dim3((unsigned)((a.r.n_rows + kTokBlock - 1) / kTokBlock)),
+                       dim3(kTokBlock), 0, st, a, p, w.lp, w.coef);
+    rc = check_launch();
+    if (rc) return rc;
+    if (p.grad) rc = launch_token_grad<T>(a, 0, a.r.n_rows, w.stats, w.coef, 0, p.grad, st);
+    if (rc) return rc;
+  }
+#undef TS_POLICY
   rc = check_launch();
   if (rc) return rc;
   hipLaunchKernelGGL(policy_sum_kernel, dim3(1), dim3(1024), 0, st, w.row, a.r.n_rows, (const int*)w.counts, loss_out);

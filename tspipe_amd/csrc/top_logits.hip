@@ -45,10 +45,16 @@ constexpr int top_hit_cap() { return NT == 64 ? 288 : NT == 256 ? 512 : 1024; }
 template <int NT>
 constexpr int top_cand_cap() { return NT == 64 ? 2304 : 1536; }
 
+// Groups per thread when k is large: short rows have few vectors per thread, and
+// a group each gives the bar they need (1000 bf16, k = 64, one group per thread:
+// 64 groups, 600 candidates, 456 us for 8192 rows).
+template <int NT>
+constexpr int top_groups() { return NT <= 256 ? 4 : 2; }
+
 template <int NT>
 struct TopShared {
   union {
-    uint32_t group[2 * NT];  // order numbers of the groups' maxima
+    uint32_t group[top_groups<NT>() * NT];  // order numbers of the groups' maxima
     uint64_t kept[kTopMax];
     u32x4 hit[top_hit_cap<NT>()];  // vectors with a candidate
   };
@@ -276,16 +282,18 @@ __device__ __forceinline__ bool top_expand(TopShared<NT>& sh, int k) {
   __syncthreads();
   const int n = sh.n;
   if (n > kCap) return false;
-  if (LAST && n <= 2 * kTopMax) return true;
+  // (a single wavefront ranks slowly: it narrows its candidates down sooner)
+  const bool narrow = n > 2 * kTopMax || (NT == kWave && n > 192 && n > k + k / 4);
+  if (LAST && !narrow) return true;
   __syncthreads();  // (nobody changes it before everybody has read it)
   if (threadIdx.x == 0) sh.n_hit = 0;
-  if (n > 2 * kTopMax) top_refine<NT>(sh, n, k);
+  if (narrow) top_refine<NT>(sh, n, k);
   __syncthreads();
   return true;
 }
 
 // One pass over a row by one workgroup, in pieces of NT * KREG vectors.  The
-// first piece gives a bar: the threads' maxima (two each when k is large) are
+// first piece gives a bar: the threads' maxima (several each when k is large) are
 // elements of disjoint groups, so the k-th largest of them is reached by at
 // least k elements.  Every element that reaches the bar is a candidate -- few
 // more than k, since the best k mostly lie in different groups (k = 64 of 512
@@ -313,7 +321,8 @@ __global__ __launch_bounds__(NT, NT > 256 ? 8 : 1) void top_logits_kernel(const 
   const VocabGeom g = vocab_geom(x, V);
   const float kk = a.k;
   const int tid = threadIdx.x;
-  const bool two = k > NT / 4;  // two groups per thread
+  constexpr int G = top_groups<NT>();
+  const bool many = k > NT / 4;  // G groups per thread, else one
   RowRegs<T, NT, KREG> r;
   regs_load(r, x, V, g);
   if (tid == 0) sh.n = sh.n_hit = 0;
@@ -327,48 +336,47 @@ __global__ __launch_bounds__(NT, NT > 256 ? 8 : 1) void top_logits_kernel(const 
   }
   // the first piece: its sum, the groups' maxima, the bar
   const int n0 = g.nvec < NT * KREG ? (int)g.nvec : NT * KREG;
-  int32_t m0 = Raw::kNone, m1 = Raw::kNone;
+  int32_t mx[G];
+#pragma unroll
+  for (int q = 0; q < G; ++q) mx[q] = Raw::kNone;
 #pragma unroll
   for (int j = 0; j < KREG; ++j) {
     if (tid + j * NT < n0) {
       forget(r.v[j]);
-      if (j < KREG / 2)
-        m0 = Raw::max2(m0, Raw::of(r.v[j]));
-      else
-        m1 = Raw::max2(m1, Raw::of(r.v[j]));
+      mx[j * G / KREG] = Raw::max2(mx[j * G / KREG], Raw::of(r.v[j]));
 #pragma unroll
       for (int i = 0; i < VEC; ++i) add(to_f32(r.v[j].v[i]));
     }
     __builtin_amdgcn_sched_barrier(0);
   }
   {
-    float f0 = fmaxf(r.h(), r.t()), f1 = -__builtin_inff();
-    bool has0 = r.has_h || r.has_t;
-    if (tid < n0) {
-      f0 = fmaxf(f0, Raw::value(m0));
-      has0 = true;
+    uint32_t whole = r.has_h || r.has_t ? top_key(fmaxf(r.h(), r.t())) : 0u;
+#pragma unroll
+    for (int q = 0; q < G; ++q) {
+      uint32_t key = 0u;
+      if (tid + q * (KREG / G) * NT < n0) {  // (a NaN sets no bar)
+        const float f = Raw::value(mx[q]);
+        key = f == f ? top_key(f) : 0u;
+      }
+      if (many && q > 0) sh.group[q * NT + tid] = key;
+      if (!many || q == 0) whole = key > whole ? key : whole;
     }
-    const bool has1 = tid + KREG / 2 * NT < n0;
-    if (has1) f1 = Raw::value(m1);
-    if (!two) f0 = fmaxf(f0, f1);
-    sh.group[tid] = has0 ? top_key(f0) : 0u;
-    if (two) sh.group[NT + tid] = has1 ? top_key(f1) : 0u;
+    sh.group[tid] = whole;
   }
   __syncthreads();
   if (tid < kWave) {
     // in registers: read from LDS for every bit, 4096 rows of 30522 took 76 us instead of 57
-    constexpr int kKeys = 2 * NT / kWave;
-    uint32_t key[kKeys];
+    constexpr int kOne = NT / kWave, kAll = G * NT / kWave;
+    uint32_t one[kOne], t;
 #pragma unroll
-    for (int i = 0; i < kKeys; ++i) key[i] = two || i < NT / kWave ? sh.group[i * kWave + tid] : 0u;
-    uint32_t t;
-    if (two) {  // uniform
-      t = top_bar<kKeys>(key, k);
+    for (int i = 0; i < kOne; ++i) one[i] = sh.group[i * kWave + tid];
+    if (many) {  // uniform
+      uint32_t all[kAll];
+#pragma unroll
+      for (int i = 0; i < kAll; ++i) all[i] = i < kOne ? one[i] : sh.group[i * kWave + tid];
+      t = top_bar<kAll>(all, k);
     } else {
-      uint32_t half[NT / kWave];
-#pragma unroll
-      for (int i = 0; i < NT / kWave; ++i) half[i] = key[i];
-      t = top_bar<NT / kWave>(half, k);
+      t = top_bar<kOne>(one, k);
     }
     if (tid == 0) sh.bar = top_unkey(t);
   }
@@ -609,13 +617,13 @@ struct TopDistilShared {
 // that a vector's marks are one byte (or half of one).
 __device__ __forceinline__ uint32_t top_mark_bit(int j, const VocabGeom& g) { return (uint32_t)(j - g.head + 8); }
 
-// KREG = 0: the row is walked for its sums and again for its gradient.
+// LONG rows do not fit the registers and are read twice.
 //
 // 64 registers a thread for up to eight vectors of a row, but for the 512-thread
 // arrangement, which would spill there: with six wavefronts a SIMD instead of
 // eight 4096 x 30522 bf16 takes 88 us instead of 99.
-template <typename T, int NT, int KREG, bool TAIL>
-__global__ __launch_bounds__(NT, (KREG > 8 ? 4 : NT > 256 ? (NT > 512 ? 8 : 6) : 1)) void top_distil_kernel(
+template <typename T, int NT, int KREG, bool LONG, bool TAIL>
+__global__ __launch_bounds__(NT, (KREG > 8 || LONG ? 4 : NT > 256 ? (NT > 512 ? 8 : 6) : 1)) void top_distil_kernel(
     const TopDistilArgs a) {
   constexpr int NW = NT / kWave, NE = (kTopMax + NT - 1) / NT, VEC = Vec16<T>::N;
   extern __shared__ uint32_t marks[];  // TAIL: a bit per vocabulary entry
@@ -631,7 +639,7 @@ __global__ __launch_bounds__(NT, (KREG > 8 ? 4 : NT > 256 ? (NT > 512 ? 8 : 6) :
   const T* x = vocab_row<T>(a.r, row);
   const VocabGeom g = vocab_geom(x, V);
   const float kk = a.r.k;
-  RowRegs<T, NT, KREG ? KREG : 1> r;
+  RowRegs<T, NT, KREG> r;
   int idx[NE];
   float p[NE];  // the teacher's probability of the token
   T xe[NE];     // the student's logit
@@ -646,7 +654,7 @@ __global__ __launch_bounds__(NT, (KREG > 8 ? 4 : NT > 256 ? (NT > 512 ? 8 : 6) :
       idx[i] = a.t_indices[row * k + at];
     }
   }
-  if constexpr (KREG > 0) regs_load(r, x, V, g);
+  regs_load(r, x, V, g);
 #pragma unroll
   for (int i = 0; i < NE; ++i)
     if (p[i] < 0.f) idx[i] = -1;
@@ -699,54 +707,63 @@ __global__ __launch_bounds__(NT, (KREG > 8 ? 4 : NT > 256 ? (NT > 512 ? 8 : 6) :
       if (idx[i] >= 0) grow[idx[i]] = from_f32<T>(gs * fmaf(q_of(ex(i)), t.whole, -p[i]));
   };
 
-  if constexpr (KREG > 0) {
-    RowSum s;
-    if (TAIL) {
-      const float c = regs_anchor(r, g, kk);
-      float out = 0.f, in = 0.f;
-      const uint8_t* mark8 = reinterpret_cast<const uint8_t*>(marks);
-      auto marked = [&](uint32_t bit) { return ((marks[bit >> 5] >> (bit & 31)) & 1u) != 0; };
-      if (tid < g.head && !marked(top_mark_bit(tid, g))) out += fast_exp2(fmaf(r.h(), kk, c));
-      if (g.tail0 + tid < V && !marked(top_mark_bit((int)g.tail0 + tid, g))) out += fast_exp2(fmaf(r.t(), kk, c));
+  RowSum s;
+  if (TAIL) {
+    const float c = regs_anchor(r, g, kk);
+    float out = 0.f, in = 0.f;
+    const uint8_t* mark8 = reinterpret_cast<const uint8_t*>(marks);
+    auto marked = [&](uint32_t bit) { return ((marks[bit >> 5] >> (bit & 31)) & 1u) != 0; };
+    if (tid < g.head && !marked(top_mark_bit(tid, g))) out += fast_exp2(fmaf(r.h(), kk, c));
+    if (g.tail0 + tid < V && !marked(top_mark_bit((int)g.tail0 + tid, g))) out += fast_exp2(fmaf(r.t(), kk, c));
+    auto add = [&](const Vec16<T>& v, uint32_t at) {
+      const uint32_t bit0 = 8u + at * VEC;
+      const uint32_t m = mark8[bit0 >> 3] >> (bit0 & 7u);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        const float e = fast_exp2(fmaf(to_f32(v.v[i]), kk, c));
+        out += (m >> i) & 1u ? 0.f : e;
+      }
+    };
+    if (LONG) {
+      long_each(r, x, g, [&](const Vec16<T>& v, int64_t at) { add(v, (uint32_t)at); });
+    } else {
 #pragma unroll
       for (int j = 0; j < KREG; ++j) {
-        const int vv = tid + j * NT;
-        if (vv < (int)g.nvec) {
+        if (tid + j * NT < (int)g.nvec) {
           forget(r.v[j]);
-          const uint32_t bit0 = 8u + (uint32_t)vv * VEC;
-          const uint32_t m = mark8[bit0 >> 3] >> (bit0 & 7u);
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) {
-            const float e = fast_exp2(fmaf(to_f32(r.v[j].v[i]), kk, c));
-            out += (m >> i) & 1u ? 0.f : e;
-          }
+          add(r.v[j], (uint32_t)(tid + j * NT));
         }
         __builtin_amdgcn_sched_barrier(0);
       }
+    }
 #pragma unroll
-      for (int i = 0; i < NE; ++i)
-        if (idx[i] >= 0) in += fast_exp2(fmaf(ex(i), kk, c));
-      // (a wavefront of nothing but -inf has no exponent of its own to take entries by)
-      if (!(c < kVrNoTerm) && in > 0.f) in = __builtin_inff();
-      s = rowsum_block<NW, kSumSecond>(c, out, in, sh.sums);
-      s.ok = s.ok && (t.rest == 0.f || s.z > 1e-30f);
-    } else {
-      s = regs_sum<T, NT, KREG>(r, g, kk, sh.sums);
-    }
-    if (s.ok) {
-      const float rest_z = s.z;
-      if (TAIL) s.z += s.a;
-      if (grow) {
-        const float rz = 1.f / s.z, go = outside(s.z / rest_z) * rz, c = s.c;
-        regs_map(r, g, x, grow, V, -1, [=](float xv) { return go * fast_exp2(fmaf(xv, kk, c)); },
-                 [](float) { return 0.f; });
-        patch([&](float xv) { return fast_exp2(fmaf(xv, kk, c)) * rz; });
-      }
-      loss([&](float xv) { return rowsum_log_prob<false>(a.r, s, xv); }, [&]() { return ln_share(log2_2x(rest_z), s.z); });
-      return;
-    }
-    __syncthreads();
+    for (int i = 0; i < NE; ++i)
+      if (idx[i] >= 0) in += fast_exp2(fmaf(ex(i), kk, c));
+    // (a wavefront of nothing but -inf has no exponent of its own to take entries by)
+    if (!(c < kVrNoTerm) && in > 0.f) in = __builtin_inff();
+    s = rowsum_block<NW, kSumSecond>(c, out, in, sh.sums);
+    s.ok = s.ok && (t.rest == 0.f || s.z > 1e-30f);
+  } else {
+    s = LONG ? long_sum(r, x, g, kk, sh.sums) : regs_sum(r, g, kk, sh.sums);
   }
+  if (s.ok) {
+    const float rest_z = s.z;
+    if (TAIL) s.z += s.a;
+    if (grow) {
+      const float rz = 1.f / s.z, go = outside(s.z / rest_z) * rz, c = s.c;
+      auto other = [=](float xv) { return go * fast_exp2(fmaf(xv, kk, c)); };
+      auto none = [](float) { return 0.f; };
+      if (LONG)
+        long_map(r, g, x, grow, V, -1, other, none);
+      else
+        regs_map(r, g, x, grow, V, -1, other, none);
+      patch([&](float xv) { return fast_exp2(fmaf(xv, kk, c)) * rz; });
+    }
+    loss([&](float xv) { return rowsum_log_prob<false>(a.r, s, xv); }, [&]() { return ln_share(log2_2x(rest_z), s.z); });
+    return;
+  }
+  __syncthreads();
+  // Rows whose sums need the true maximum: walked.
   VocabStat out = vstat_init(), all;
   if (TAIL) {
     for (int64_t i = tid; i < V; i += NT) {
@@ -801,8 +818,10 @@ int launch_top_logits(const VocabRows& a, int k, void* values, int32_t* indices,
   const dim3 grid((unsigned)a.n_rows);
   if (sh.nt == 64)
     hipLaunchKernelGGL((top_logits_kernel<T, 64, 4, false>), grid, dim3(64), 0, st, a, k, out, indices, lse);
-  else if (sh.nt == 256)
+  else if (sh.nt == 256 && sh.kreg == 4)
     hipLaunchKernelGGL((top_logits_kernel<T, 256, 4, false>), grid, dim3(256), 0, st, a, k, out, indices, lse);
+  else if (sh.nt == 256)
+    hipLaunchKernelGGL((top_logits_kernel<T, 256, 8, false>), grid, dim3(256), 0, st, a, k, out, indices, lse);
   else if (sh.nt == 512)
     hipLaunchKernelGGL((top_logits_kernel<T, 512, 8, false>), grid, dim3(512), 0, st, a, k, out, indices, lse);
   else
@@ -810,30 +829,31 @@ int launch_top_logits(const VocabRows& a, int k, void* values, int32_t* indices,
   return check_launch();
 }
 
-template <typename T, int NT, int KREG, bool TAIL>
+template <typename T, int NT, int KREG, bool LONG, bool TAIL>
 int launch_top_distil_rows(const TopDistilArgs& a, hipStream_t st) {
   const size_t marks = TAIL ? (size_t)((a.r.V + 8 + 31) / 32) * 4 : 0;
   if (marks > 32768) {
-    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&top_distil_kernel<T, NT, KREG, TAIL>),
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&top_distil_kernel<T, NT, KREG, LONG, TAIL>),
                                              hipFuncAttributeMaxDynamicSharedMemorySize, (int)marks);
     if (e != hipSuccess) {
       set_last_hip_error((int)e);
       return TS_ERR_LAUNCH;
     }
   }
-  hipLaunchKernelGGL((top_distil_kernel<T, NT, KREG, TAIL>), dim3((unsigned)a.r.n_rows), dim3(NT), marks, st, a);
+  hipLaunchKernelGGL((top_distil_kernel<T, NT, KREG, LONG, TAIL>), dim3((unsigned)a.r.n_rows), dim3(NT), marks, st, a);
   return check_launch();
 }
 
 template <typename T, bool TAIL>
 int launch_top_distil_shape(const TopDistilArgs& a, hipStream_t st) {
   const RowShape sh = row_shape<T>(a.r.V);
-  if (sh.nt == 64) return launch_top_distil_rows<T, 64, 4, TAIL>(a, st);
-  if (sh.nt == 256) return launch_top_distil_rows<T, 256, 4, TAIL>(a, st);
-  if (sh.nt == 512) return launch_top_distil_rows<T, 512, 8, TAIL>(a, st);
-  if (sh.kreg == 8) return launch_top_distil_rows<T, 1024, 8, TAIL>(a, st);
-  if (sh.kreg == 16) return launch_top_distil_rows<T, 1024, 16, TAIL>(a, st);
-  return launch_top_distil_rows<T, 1024, 0, TAIL>(a, st);
+  if (sh.nt == 64) return launch_top_distil_rows<T, 64, 4, false, TAIL>(a, st);
+  if (sh.nt == 256 && sh.kreg == 4) return launch_top_distil_rows<T, 256, 4, false, TAIL>(a, st);
+  if (sh.nt == 256) return launch_top_distil_rows<T, 256, 8, false, TAIL>(a, st);
+  if (sh.nt == 512) return launch_top_distil_rows<T, 512, 8, false, TAIL>(a, st);
+  if (sh.kreg == 8) return launch_top_distil_rows<T, 1024, 8, false, TAIL>(a, st);
+  if (sh.kreg == 16) return launch_top_distil_rows<T, 1024, 16, false, TAIL>(a, st);
+  return launch_top_distil_rows<T, 512, 8, true, TAIL>(a, st);
 }
 
 template <typename T>

@@ -524,6 +524,78 @@ __device__ __forceinline__ double block_sum_f64(double v, double* lds) {
   return r;
 }
 
+// Rows longer than the registers hold, in pieces of NT * KREG vectors: f(vector,
+// its place) for each.  The first piece is in r; a register that is done with
+// takes the next piece's vector at once, so that loads are always under way.
+template <typename T, int NT, int KREG, typename F>
+__device__ __forceinline__ void long_each(RowRegs<T, NT, KREG>& r, const T* row, const VocabGeom& g, F f) {
+  constexpr int VEC = Vec16<T>::N;
+  for (int64_t v0 = 0;; v0 += NT * KREG) {
+    const int left = g.nvec - v0 < NT * KREG ? (int)(g.nvec - v0) : NT * KREG;
+    const int64_t after = g.nvec - v0 - left;
+    const VecBuffer next = vec_buffer(row + g.head + (v0 + left) * VEC, after < NT * KREG ? (int)after : NT * KREG);
+#pragma unroll
+    for (int j = 0; j < KREG; ++j) {
+      if ((int)threadIdx.x + j * NT < left) {
+        forget(r.v[j]);
+        f(r.v[j], v0 + threadIdx.x + j * NT);
+      }
+      if (after > 0) r.v[j] = vec_load<T>(next, threadIdx.x + j * NT);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if (after == 0) return;
+  }
+}
+
+// regs_sum and regs_map of such rows.
+template <typename T, int NT, int KREG>
+__device__ __forceinline__ RowSum long_sum(RowRegs<T, NT, KREG>& r, const T* row, const VocabGeom& g, float k, RowSum* lds) {
+  constexpr int VEC = Vec16<T>::N;
+  const float c = regs_anchor(r, g, k);
+  float z = 0.f;
+  auto add = [&](float x) { z += fast_exp2(fmaf(x, k, c)); };
+  if (threadIdx.x < kWave) {
+    add(r.h());
+    add(r.t());
+  }
+  long_each(r, row, g, [&](const Vec16<T>& v, int64_t) {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) add(to_f32(v.v[i]));
+  });
+  return rowsum_block<NT / kWave, kSumOnly>(c, z, 0.f, lds);
+}
+
+template <typename T, int NT, int KREG, typename F, typename G>
+__device__ __forceinline__ void long_map(RowRegs<T, NT, KREG>& r, const VocabGeom& g, const T* row, T* grow, int64_t V,
+                                         int special, F f, G f_special) {
+  constexpr int VEC = Vec16<T>::N;
+  regs_load(r, row, V, g);  // the second reading
+  if ((int)threadIdx.x < g.head)
+    grow[threadIdx.x] = from_f32<T>((int)threadIdx.x == special ? f_special(r.h()) : f(r.h()));
+  const int64_t t = g.tail0 + threadIdx.x;
+  if (t < V) grow[t] = from_f32<T>((int)t == special ? f_special(r.t()) : f(r.t()));
+  const bool gvec = (((uintptr_t)grow ^ (uintptr_t)row) & 15u) == 0;
+  const int64_t sv = special >= g.head ? (special - g.head) / VEC : -1;
+  const int si = special - g.head - (int)sv * VEC;
+  long_each(r, row, g, [&](const Vec16<T>& x, int64_t v) {
+    Vec16<T> o;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) o.v[i] = from_f32<T>(f(to_f32(x.v[i])));
+    if (v == sv) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i)
+        if (i == si) o.v[i] = from_f32<T>(f_special(to_f32(x.v[i])));
+    }
+    T* p = grow + g.head + v * VEC;
+    if (gvec) {
+      store16_stream(p, o);
+    } else {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) p[i] = o.v[i];
+    }
+  });
+}
+
 // This thread's share of sum(v[0..n)) when NT threads walk the array together, in
 // a fixed order, eight loads in flight each.
 template <int NT>
@@ -590,6 +662,7 @@ inline RowShape row_shape(int64_t V) {
   const int64_t vecs = V / Vec16<T>::N;
   if (vecs <= 64 * 4) return RowShape{64, 4};
   if (vecs <= 256 * 4) return RowShape{256, 4};
+  if (vecs <= 256 * 8) return RowShape{256, 8};
   if (vecs <= 512 * 8) return RowShape{512, 8};
   if (vecs <= 1024 * 8) return RowShape{1024, 8};
   if (vecs <= 1024 * 16) return RowShape{1024, 16};
