@@ -560,10 +560,12 @@ def test_both_refuse_alike(device, monkeypatch):
         with pytest.raises(RuntimeError):
             lp.backward()
         # a second derivative is refused
-        lp = ta.token_log_probs(leaf, lab).sum()
-        with pytest.raises(RuntimeError):
-            g, = torch.autograd.grad(lp, leaf, create_graph=True)
-            g.sum().backward()
+        for make_loss in (lambda: ta.token_log_probs(leaf, lab).sum(), lambda: ta.preference_loss(leaf, lab, ref),
+                          lambda: ta.clipped_policy_loss(leaf, lab, ref, ref),
+                          lambda: ta.top_logits_distil_loss(leaf, *ta.top_logits(leaf, 3)[:2], 1.0)):
+            with pytest.raises(RuntimeError):
+                g, = torch.autograd.grad(make_loss(), leaf, create_graph=True)
+                g.sum().backward()
         for call in (lambda: ta.preference_loss(leaf, lab[:, :4], ref), lambda: ta.preference_loss(leaf, lab, ref[:, :4]),
                      lambda: ta.clipped_policy_loss(leaf, lab, ref, ref[:1, 0]),
                      lambda: ta.token_log_probs(leaf, lab.cpu()),
@@ -626,3 +628,57 @@ def test_two_threads_on_two_streams(device):
     for w, h in zip(want, got):
         for a, b in zip(w, h):
             assert bits_equal(a, b)
+
+
+@pytest.mark.parametrize("V", [700, 9000, 40000, 90000, 150001])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_masked_stretches_and_lone_peaks(device, V, dtype):
+    # stretches of vocabulary masked with -1e4, -1e9, -inf or the type's lowest value, wherever they fall among
+    # the wavefronts' vectors; whole rows far from zero; one logit far above all others, at temperatures down to 0.2
+    g = seeded(140 + V)
+    fi = torch.finfo(dtype)
+    fills = [-1e4, -6e4 if dtype == torch.float16 else -1e9, float("-inf"), fi.min]
+    rows = []
+    for fill in fills:
+        for lo, hi in ((0, V // 2), (V // 2, V - 3), (5, V - 5)):
+            r = torch.randn(V, generator=g) * 2
+            r[lo:hi] = fill
+            rows.append(r)
+    for shift in (-3e4, 3e4):
+        rows.append(torch.randn(V, generator=g) * 50 + shift)
+    for at in (0, V // 3, V - 1):
+        r = torch.randn(V, generator=g)
+        r[at] = 60.0
+        rows.append(r)
+    x = torch.stack(rows).to(dtype)[None]
+    n = x.shape[1]
+    labels = torch.tensor([[int(x[0, i].float().argmax()) if i % 2 else V - 1 for i in range(n)]])
+    go = torch.randn(1, n, generator=g)
+    for T in (1.0, 0.2):
+        x64 = x.double().requires_grad_()
+        want, _ = ref64.log_probs(x64, labels, T)
+        want.backward(go.double())
+        xd = x.to(device).requires_grad_()
+        got = ta.token_log_probs(xd, labels.to(device), T)
+        got.backward(go.to(device))
+        finite = torch.isfinite(want) & (want.abs() < 1e30)
+        # exponents of rows far from zero carry the fp32 rounding of x k, at most 2^-24 |x| / T each way
+        extra = 2.0 ** -23 * (x.double().abs().amin(-1) / T)
+        err = (got.cpu().double() - want).abs()
+        assert (err <= LOGP_ABS + extra + 2.0 ** -24 * want.abs())[finite].all()
+        same = torch.isinf(want) & (got.cpu().double() == want)
+        assert (finite | same | (want.abs() >= 1e30)).all()
+        check_grad(xd.grad, x64.grad, dtype, coef=(go.abs() / T)[..., None] * (1 + extra[..., None] * 2 ** 22))
+    adv, old = torch.randn(1, n, generator=g), want.float().clamp(-50, 0).detach()
+    ok = (want > -50) & torch.isfinite(want)
+    lab2 = labels.masked_fill(~ok, -100)
+    x64 = x.double().requires_grad_()
+    wl, wlp = ref64.policy(x64, lab2, old.double(), adv.double(), T=0.2, lo=10.0, hi=10.0)
+    wl.backward()
+    xd = x.to(device).requires_grad_()
+    loss, lp = ta.clipped_policy_loss(xd, lab2.to(device), old.to(device), adv.to(device), temperature=0.2, clip_low=10.0,
+                                      clip_high=10.0, return_log_probs=True)
+    loss.backward()
+    assert ((lp.cpu().double() - wlp).abs() <= LOGP_ABS + extra + 2.0 ** -24 * wlp.abs()).all()
+    c = adv.abs()[..., None] / 0.2 / int(ok.sum())
+    check_grad(xd.grad, x64.grad, dtype, coef=c * (1 + extra[..., None] * 2 ** 22 + LOGP_ABS * 2 ** 22))

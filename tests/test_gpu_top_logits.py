@@ -329,3 +329,38 @@ def test_graph_capture_replays(device):
         torch.cuda.synchronize()
         for a, b in zip(outs, step(fresh.requires_grad_())):
             assert bits_equal(a, b), trial
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("V", [700, 9000, 40000, 150001])
+def test_masked_stretches(device, V, dtype):
+    g = seeded(33 + V)
+    rows = []
+    for fill in (-1e4, float("-inf"), torch.finfo(dtype).min):
+        for lo, hi in ((0, V // 2), (V // 2, V - 3)):
+            r = torch.randn(V, generator=g) * 3
+            r[lo:hi] = fill
+            rows.append(r)
+    rows.append(torch.randn(V, generator=g).abs() * -3 - 1)     # no logit above zero
+    rows.append(torch.randn(V, generator=g).abs() * -3 - 1e4)
+    x = torch.stack(rows).to(dtype)
+    k = 50
+    top = check_top(x, k, device)
+    # the student is masked the same way, the teacher's kept entries are not among the masked
+    s = x.float().clone()
+    live = s > -9e3
+    live[-1] = True
+    s = torch.where(live, s + torch.randn(s.shape, generator=g) * 0.5, s).to(dtype)
+    for lse in (None, top.logsumexp.cpu()):
+        run_case(device, s, top.values.cpu(), top.indices.cpu(), 1.0, 64.0 * len(rows), None, lse)
+
+
+@pytest.mark.parametrize("rows", [1, 300])
+@pytest.mark.parametrize("V,k", [(150, 150), (900, 256), (2062, 256), (2063, 256), (4100, 200), (8200, 256), (16390, 256),
+                                 (32790, 256), (70000, 256), (300000, 256)])
+def test_top_logits_many_entries(device, V, k, rows):
+    if rows * V > 10 ** 7:
+        rows = 3
+    g = seeded(V - k)
+    for dtype in DTYPES:
+        check_top((torch.randn(rows, V, generator=g) * 2).to(dtype), min(k, V), device)

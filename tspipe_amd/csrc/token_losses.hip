@@ -78,7 +78,7 @@ __global__ __launch_bounds__(NT) void token_stat_kernel(const TokenRows a, int64
   const T label_logit = srow[label];
   RowRegs<T, NT, KREG> r;
   regs_load(r, srow, V, g);
-  const float c = regs_anchor(r, g, k);
+  const float c = regs_anchor<true>(r, g, k);
   float z = 0.f, s_a = 0.f;
   auto add = [&](float x) {
     const float d = fmaf(x, k, c), e = fast_exp2(d);

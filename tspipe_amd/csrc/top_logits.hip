@@ -68,46 +68,6 @@ struct TopShared {
   float bar;
 };
 
-// The largest of a vector's elements by their bits as signed numbers: two
-// sixteen-bit maxima, or one of 32 bits.  For logits above zero that is their
-// order; of a vector without such a one it is just one of its elements.
-template <typename T>
-struct RawMax {
-  int32_t m;
-  static constexpr int32_t kNone = sizeof(T) == 4 ? (int32_t)0x80000000 : (int32_t)0x80008000;
-  __device__ __forceinline__ static int32_t max2(int32_t a, int32_t b) {
-    if constexpr (sizeof(T) == 4) {
-      return a > b ? a : b;
-    } else {
-      typedef int16_t s16x2 __attribute__((ext_vector_type(2)));
-      s16x2 x, y;
-      __builtin_memcpy(&x, &a, 4);
-      __builtin_memcpy(&y, &b, 4);
-      const s16x2 z = __builtin_elementwise_max(x, y);
-      int32_t r;
-      __builtin_memcpy(&r, &z, 4);
-      return r;
-    }
-  }
-  __device__ __forceinline__ static int32_t of(const Vec16<T>& v) {
-    int32_t w[4];
-    __builtin_memcpy(w, &v, 16);
-    return max2(max2(w[0], w[1]), max2(w[2], w[3]));
-  }
-  // the element that `m` stands for, as fp32
-  __device__ __forceinline__ static float value(int32_t m) {
-    if constexpr (sizeof(T) == 4) {
-      return __int_as_float(m);
-    } else {
-      const int16_t lo = (int16_t)(m & 0xffff), hi = (int16_t)(m >> 16);
-      const int16_t top = lo > hi ? lo : hi;
-      T t;
-      __builtin_memcpy(&t, &top, 2);
-      return to_f32(t);
-    }
-  }
-};
-
 // Ranks the n candidates by counting, for each one, those that are larger; the
 // first k leave.  With fewer candidates than threads several threads count for
 // each.  sh.rank is 0 on entry.
@@ -327,7 +287,7 @@ __global__ __launch_bounds__(NT, NT > 256 ? 8 : 1) void top_logits_kernel(const 
   regs_load(r, x, V, g);
   if (tid == 0) sh.n = sh.n_hit = 0;
   for (int i = tid; i < 2 * kTopMax; i += NT) sh.rank[i] = 0;
-  const float c = regs_anchor(r, g, kk);
+  const float c = regs_anchor<false>(r, g, kk);
   float z = 0.f;
   auto add = [&](float xv) { z += fast_exp2(fmaf(xv, kk, c)); };
   if (tid < kWave) {
@@ -709,7 +669,7 @@ __global__ __launch_bounds__(NT, (KREG > 8 || LONG ? 4 : NT > 256 ? (NT > 512 ? 
 
   RowSum s;
   if (TAIL) {
-    const float c = regs_anchor(r, g, kk);
+    const float c = regs_anchor<true>(r, g, kk);
     float out = 0.f, in = 0.f;
     const uint8_t* mark8 = reinterpret_cast<const uint8_t*>(marks);
     auto marked = [&](uint32_t bit) { return ((marks[bit >> 5] >> (bit & 31)) & 1u) != 0; };

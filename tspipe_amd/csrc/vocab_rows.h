@@ -267,15 +267,20 @@ __device__ __forceinline__ void vocab_zero_row(T* grow, int64_t V) {
 // wavefront.
 //
 // Sums are taken of 2^(x k + c) with an integer c per wavefront, so that
-// moving a sum from one c to another is exact and no row maximum is needed in
-// front: c = -rint(k x_0) with x_0 the largest of the wavefront's first
-// vectors.  Elements may exceed x_0; a sum that overflows for it (or one that
-// comes out 0 or NaN) is not ok, and the caller walks the row again with its
-// true maximum.  That drops a third of the vector instructions of a
-// maximum-first pass, and the first exponential waits for one vector instead of
-// for the whole row.
+// moving a sum from one c to another is exact and no maximum of the whole row is
+// needed in front: c = -rint(k x_0) with x_0 an element of the wavefront near its
+// largest.  Elements may exceed x_0; a sum that overflows for it (or comes out 0
+// or NaN) is not ok, and the caller walks the row again with its true maximum.
+// How near x_0 is decides the rounding of the exponents: the gradient of a row
+// whose probability is nearly all in one token shows it, so there x_0 is taken
+// over all of the wavefront's vectors, by their raw bits (an instruction for two
+// 16-bit logits); a log-sum-exp does with the first vectors' maximum, and its
+// first exponential then waits for one vector instead of for all.
 // ---------------------------------------------------------------------------
-constexpr float kVrNoTerm = 1e9f;  // c of a wavefront without a finite element: its factor 2^(C - c) is 0
+// c of a wavefront without an element above -1e7 / k (masked vocabulary): with it such an element's
+// term is 0, so that the others' sum stands alone, or infinite, and the row is walked.
+constexpr float kVrNoTerm = 1e9f;
+constexpr float kVrLeast = -1e7f;
 
 // `count` 16-byte vectors behind a 16-byte aligned address, the same in every
 // lane.  Loads beyond them return 0 and stores beyond them do nothing (the
@@ -354,29 +359,79 @@ __device__ __forceinline__ void forget(Vec16<T>& v) {
   __builtin_memcpy(&v, &b, 16);
 }
 
-// Largest of the wavefront's first vectors and end elements, of all of its
-// vectors if those hold nothing finite.
-template <typename T, int NT, int KREG>
+// The largest of a vector's elements by their bits as signed numbers: two
+// sixteen-bit maxima, or one of 32 bits.  For logits above zero that is their
+// order; of a vector without such a one it is just one of its elements.
+template <typename T>
+struct RawMax {
+  int32_t m;
+  static constexpr int32_t kNone = sizeof(T) == 4 ? (int32_t)0x80000000 : (int32_t)0x80008000;
+  __device__ __forceinline__ static int32_t max2(int32_t a, int32_t b) {
+    if constexpr (sizeof(T) == 4) {
+      return a > b ? a : b;
+    } else {
+      typedef int16_t s16x2 __attribute__((ext_vector_type(2)));
+      s16x2 x, y;
+      __builtin_memcpy(&x, &a, 4);
+      __builtin_memcpy(&y, &b, 4);
+      const s16x2 z = __builtin_elementwise_max(x, y);
+      int32_t r;
+      __builtin_memcpy(&r, &z, 4);
+      return r;
+    }
+  }
+  __device__ __forceinline__ static int32_t of(const Vec16<T>& v) {
+    int32_t w[4];
+    __builtin_memcpy(w, &v, 16);
+    return max2(max2(w[0], w[1]), max2(w[2], w[3]));
+  }
+  // the element that `m` stands for, as fp32
+  __device__ __forceinline__ static float value(int32_t m) {
+    if constexpr (sizeof(T) == 4) {
+      return __int_as_float(m);
+    } else {
+      const int16_t lo = (int16_t)(m & 0xffff), hi = (int16_t)(m >> 16);
+      const int16_t top = lo > hi ? lo : hi;
+      T t;
+      __builtin_memcpy(&t, &top, 2);
+      return to_f32(t);
+    }
+  }
+};
+
+// c of the wavefront.  ALL: by all of its vectors, else by its first ones and, if
+// those are masked, by all.
+template <bool ALL, typename T, int NT, int KREG>
 __device__ __forceinline__ float regs_anchor(const RowRegs<T, NT, KREG>& r, const VocabGeom& g, float k) {
   constexpr int VEC = Vec16<T>::N;
+  typedef RawMax<T> Raw;
   float m = fmaxf(r.h(), r.t());
-  if ((int)threadIdx.x < (int)g.nvec) {
+  if (ALL) {
+    int32_t raw = Raw::kNone;
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) m = fmaxf(m, to_f32(r.v[0].v[i]));
+    for (int j = 0; j < KREG; ++j)
+      if ((int)threadIdx.x + j * NT < (int)g.nvec) raw = Raw::max2(raw, Raw::of(r.v[j]));
+    if ((int)threadIdx.x < (int)g.nvec) m = fmaxf(m, Raw::value(raw));
+  } else {
+    if ((int)threadIdx.x < (int)g.nvec) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) m = fmaxf(m, to_f32(r.v[0].v[i]));
+    }
   }
   m = wave_max(m);
-  if (!(m > -1e30f)) {
+  if (!(m * k > (ALL ? 0.f : kVrLeast))) {  // (masked, or, by raw bits, nothing above zero: the true maximum)
 #pragma unroll
-    for (int j = 1; j < KREG; ++j) {
+    for (int j = 0; j < KREG; ++j) {
       if ((int)threadIdx.x + j * NT < (int)g.nvec) {
 #pragma unroll
         for (int i = 0; i < VEC; ++i) m = fmaxf(m, to_f32(r.v[j].v[i]));
       }
     }
     m = wave_max(m);
-    if (!(m > -1e30f)) return kVrNoTerm;
+    if (!(m * k > kVrLeast)) return kVrNoTerm;
   }
-  return m < 1e30f ? -rintf(m * k) : 0.f;  // (an infinite logit makes the sum overflow whatever c is)
+  const float e = m * k;
+  return e < 1e30f ? -rintf(e) : 0.f;  // (an infinite logit makes the sum overflow whatever c is)
 }
 
 struct RowSum {  // z = sum 2^(x k + c), a: nothing, or one of the two below
@@ -408,8 +463,12 @@ __device__ __forceinline__ RowSum rowsum_get(RowSum r, const RowSum* lds) {
     float C = w.c;
 #pragma unroll
     for (int off = NW / 2; off > 0; off >>= 1) C = fminf(C, __shfl_xor(C, off, kWave));
-    const float d = C - w.c, f = fast_exp2(d);
-    r = RowSum{C, w.z * f, KIND == kSumMean ? f * fmaf(w.z, d, w.a) : KIND == kSumSecond ? f * w.a : 0.f, true};
+    // (by the exponent: 2^d itself may underflow where the sum times it does not)
+    const float d = C - w.c;
+    const int shift = (int)fmaxf(d, -1000.f);
+    r = RowSum{C, __builtin_amdgcn_ldexpf(w.z, shift), 0.f, true};
+    if (KIND == kSumMean) r.a = __builtin_amdgcn_ldexpf(fmaf(w.z, d, w.a), shift);
+    if (KIND == kSumSecond) r.a = __builtin_amdgcn_ldexpf(w.a, shift);
 #pragma unroll
     for (int off = NW / 2; off > 0; off >>= 1) {
       r.z += __shfl_xor(r.z, off, kWave);
@@ -458,7 +517,7 @@ __device__ __forceinline__ void regs_each(RowRegs<T, NT, KREG>& r, const VocabGe
 
 template <typename T, int NT, int KREG>
 __device__ __forceinline__ RowSum regs_sum(RowRegs<T, NT, KREG>& r, const VocabGeom& g, float k, RowSum* lds) {
-  const float c = regs_anchor(r, g, k);
+  const float c = regs_anchor<true>(r, g, k);
   float z = 0.f;
   auto add = [&](float x) { z += fast_exp2(fmaf(x, k, c)); };
   if (threadIdx.x < kWave) {  // the end elements
@@ -551,7 +610,7 @@ __device__ __forceinline__ void long_each(RowRegs<T, NT, KREG>& r, const T* row,
 template <typename T, int NT, int KREG>
 __device__ __forceinline__ RowSum long_sum(RowRegs<T, NT, KREG>& r, const T* row, const VocabGeom& g, float k, RowSum* lds) {
   constexpr int VEC = Vec16<T>::N;
-  const float c = regs_anchor(r, g, k);
+  const float c = regs_anchor<true>(r, g, k);
   float z = 0.f;
   auto add = [&](float x) { z += fast_exp2(fmaf(x, k, c)); };
   if (threadIdx.x < kWave) {

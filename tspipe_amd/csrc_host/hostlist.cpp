@@ -589,6 +589,7 @@ struct ReadyGradNode : public torch::autograd::Node {
   bool done = false;
   torch::autograd::variable_list apply(torch::autograd::variable_list&& grad_out) override {
     TORCH_CHECK(!done, "the fused loss keeps one gradient buffer: backward can run once per forward");
+    TORCH_CHECK(!at::GradMode::is_enabled(), "the fused loss cannot be differentiated twice (create_graph)");
     done = true;
     at::Tensor g = std::move(grad);  // autograd can adopt it as .grad instead of copying
     grad = at::Tensor();

@@ -106,6 +106,7 @@ class _PreferenceFn(torch.autograd.Function):
         return loss, rewards
 
     @staticmethod
+    @torch.autograd.function.once_differentiable
     def backward(ctx, grad_output: Tensor, _):
         return (_take_grad(ctx, grad_output),) + (None,) * 9
 
@@ -197,6 +198,7 @@ class _PolicyFn(torch.autograd.Function):
         return loss, logp
 
     @staticmethod
+    @torch.autograd.function.once_differentiable
     def backward(ctx, grad_output: Tensor, _):
         return (_take_grad(ctx, grad_output),) + (None,) * 12
 

@@ -88,6 +88,7 @@ class _TopDistilFn(torch.autograd.Function):
         return loss
 
     @staticmethod
+    @torch.autograd.function.once_differentiable
     def backward(ctx, grad_output: Tensor):
         if not ctx.needs_input_grad[0]:
             return (None,) * 7
