@@ -331,8 +331,8 @@ int ts_mse_pieces_fwd_bwd(const void* const* s_pieces, const void* const* t_piec
 /* ------------------------------------------------------------------------ */
 
 /* logp[r] = ln softmax(s_r / T)[labels[r]], 0 for rows that do not count.
- * stats (2 floats per row, 8-byte aligned, may be NULL): the row's maximum and
- * sum, what the backward pass takes. */
+ * stats (2 floats per row, 8-byte aligned, may be NULL): the row's sum and what
+ * its terms are relative to, which the backward pass takes. */
 int ts_token_logp_fwd(const void* s, int64_t n_seq, int64_t seq_len, int64_t V, int64_t ld_seq,
                       int64_t ld_tok, const int64_t* labels, const uint8_t* row_mask,
                       int64_t ignore_index, double temperature, float* logp, float* stats, int dtype,

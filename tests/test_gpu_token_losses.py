@@ -682,3 +682,102 @@ def test_masked_stretches_and_lone_peaks(device, V, dtype):
     assert ((lp.cpu().double() - wlp).abs() <= LOGP_ABS + extra + 2.0 ** -24 * wlp.abs()).all()
     c = adv.abs()[..., None] / 0.2 / int(ok.sum())
     check_grad(xd.grad, x64.grad, dtype, coef=c * (1 + extra[..., None] * 2 ** 22 + LOGP_ABS * 2 ** 22))
+
+
+# ---- where a loss is NaN, so is its gradient ---------------------------------------------------
+
+def test_nan_losses_have_nan_gradients(device):
+    x, labels, _ = make((2, 4, 600), torch.float32, 151)
+    lab = labels.to(device)
+    old = torch.full((2, 4), -5.0, device=device)
+    adv = torch.ones(2, 4, device=device)
+    adv[0, 1] = float("nan")
+    leaf = x.to(device).requires_grad_()
+    loss = ta.clipped_policy_loss(leaf, lab, old, adv)
+    loss.backward()
+    assert loss.isnan() and leaf.grad[0, 1].isnan().all() and leaf.grad[0, 0].isfinite().all()
+    # an infinite ratio of no advantage: inf * 0
+    old[1, 2], adv[0, 1], adv[1, 2] = float("-inf"), 1.0, 0.0
+    leaf = x.to(device).requires_grad_()
+    loss = ta.clipped_policy_loss(leaf, lab, old, adv)
+    loss.backward()
+    assert loss.isnan() and leaf.grad[1, 2].isnan().all() and leaf.grad[1, 1].isfinite().all()
+    for kind in ("sigmoid", "hinge", "ipo"):
+        ref = torch.zeros(2, device=device)
+        ref[1] = float("nan")
+        leaf = x.to(device).requires_grad_()
+        loss = ta.preference_loss(leaf, lab, ref, loss_type=kind)
+        loss.backward()
+        assert loss.isnan() and leaf.grad.isnan().all(), kind
+
+
+# ---- many short answers ------------------------------------------------------------------------
+
+@pytest.mark.parametrize("reduction", ["token", "sequence"])
+@pytest.mark.parametrize("n,L", [(5000, 1), (4099, 2), (1300, 3), (700, 17), (257, 33), (9, 64), (3, 65), (2, 1500)])
+def test_policy_many_short_answers(device, n, L, reduction):
+    x, labels, g = make((n, L, 11), torch.float32, 160 + n + L)
+    labels[torch.rand(n, L, generator=g) < 0.4] = -100
+    labels[n // 2] = -100
+    adv = torch.randn(n, generator=g)
+    x64 = x.double().requires_grad_()
+    lp, live = ref64.log_probs(x64, labels)
+    old = (lp.detach() + torch.randn(n, L, generator=g) * 0.05).float()
+    want, _ = ref64.policy(x64, labels, old.double(), adv.double(), lo=0.5, hi=0.5, reduction=reduction, weight=n * L)
+    want.backward()
+    xd = x.to(device).requires_grad_()
+    loss = ta.clipped_policy_loss(xd, labels.to(device), old.to(device), adv.to(device), clip_low=0.5, clip_high=0.5,
+                                  reduction=reduction, weight=n * L)
+    loss.backward()
+    # a term is off by 1e-5 of itself at most (the ratio's exponential of a log probability), and the terms add up in 64 bits
+    size = (n * L) * adv.abs().max().item() * 1.5
+    assert abs(loss.item() - want.item()) <= 1e-5 * size + 2.0 ** -24 * abs(want.item())
+    per = live.sum(-1)
+    count = per.sum() if reduction == "token" else (per > 0).sum() * per.clamp_min(1)
+    c = (adv.abs() * 1.5 * n * L / count).double()[:, None, None].expand(n, L, 1)
+    check_grad(xd.grad, x64.grad, torch.float32, coef=c * (1 + 1e-5 * 2 ** 22))
+
+
+# ---- a near-certain token behind the first piece of a long row ---------------------------------
+
+@pytest.mark.parametrize("V", [50257, 150001])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_log_probs_of_near_certain_tokens(device, V, dtype):
+    # Sums are taken relative to an integer near the row's largest exponent, so that the exponent of a token
+    # that holds nearly all of the probability is exact but for its last half unit below one: its log
+    # probability carries an exponential's and a logarithm's errors, 1.2e-7 and 2e-7, and is within 1e-6.
+    g = seeded(170 + V)
+    peaks = torch.arange(24, 88).to(dtype) * 0.75
+    x = torch.randn(1, peaks.numel(), V, generator=g).to(dtype)
+    at = torch.randint(V * 3 // 4, V, (1, peaks.numel()), generator=g)
+    x.scatter_(-1, at[..., None], peaks[None, :, None])
+    want, _ = ref64.log_probs(x.double(), at)
+    xd = x.to(device)
+    got = ta.token_log_probs(xd, at.to(device))
+    assert ((got.cpu().double() - want).abs() <= 1e-6 + 2.0 ** -24 * want.abs()).all()
+    zero = torch.zeros(1, peaks.numel(), device=device)
+    _, lp = ta.clipped_policy_loss(xd, at.to(device), zero, zero[:, 0] + 1, return_log_probs=True)
+    assert ((lp.cpu().double() - want).abs() <= 1e-6 + 2.0 ** -24 * want.abs()).all()
+    # one entry that the teacher is sure of: the row's loss is minus the student's log probability of it
+    values = torch.zeros(1, peaks.numel(), 1, device=device)
+    for lse in (None, zero):
+        loss = ta.top_logits_distil_loss(xd, values, at[..., None].to(device).int(), 1.0, t_logsumexp=lse)
+        assert abs(loss.item() + want.mean().item()) <= 1e-6
+
+
+def test_forward_mode_is_refused(device, monkeypatch):
+    import torch.autograd.forward_ad as fw
+    x, labels, _ = make((2, 3, 40), torch.float32, 181)
+    xd, lab, ref = x.to(device), labels.to(device), torch.zeros(2, 3, device=device)
+
+    def refused():
+        with fw.dual_level():
+            dual = fw.make_dual(xd, torch.ones_like(xd))
+            for call in (lambda: ta.token_log_probs(dual, lab), lambda: ta.preference_loss(dual, lab, ref),
+                         lambda: ta.clipped_policy_loss(dual, lab, ref, ref),
+                         lambda: ta.top_logits_distil_loss(dual, *ta.top_logits(xd, 3)[:2], 1.0)):
+                with pytest.raises((RuntimeError, NotImplementedError)):
+                    call()
+        return True
+
+    assert _both_ways(monkeypatch, refused) == (True, True)

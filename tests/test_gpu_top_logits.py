@@ -364,3 +364,24 @@ def test_top_logits_many_entries(device, V, k, rows):
     g = seeded(V - k)
     for dtype in DTYPES:
         check_top((torch.randn(rows, V, generator=g) * 2).to(dtype), min(k, V), device)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("V,k", [(200, 64), (2500, 64), (12000, 200), (30522, 64), (140001, 64)])
+def test_top_logits_fewer_left_than_asked_for(device, V, k, dtype):
+    # the vocabulary masked but for fewer than k tokens (or for just k, or one more): the masked ones follow by place
+    g = seeded(41 + V)
+    fi = torch.finfo(dtype)
+    rows = []
+    for fill in (float("-inf"), fi.min, -1e4, 0.0):
+        for live in (0, 1, 2, k - 1, k, k + 1):
+            r = torch.full((V,), fill)
+            r[torch.randperm(V, generator=g)[:live]] = torch.randn(live, generator=g) * 3
+            rows.append(r)
+    x = torch.stack(rows).to(dtype)
+    check_top(x, k, device)
+    x[:, V // 2] = float("nan")  # with a NaN in every row: the largest, and the others in their order
+    top = ta.top_logits(x.to(device), k)
+    assert (top.indices[:, 0] == V // 2).all() and top.logsumexp.isnan().all()
+    x[:, V // 2] = float("inf")
+    assert torch.equal(top.indices.cpu().long(), ref64.top(x.float(), k)[1])

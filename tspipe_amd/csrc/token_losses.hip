@@ -78,8 +78,7 @@ __global__ __launch_bounds__(NT) void token_stat_kernel(const TokenRows a, int64
   const T label_logit = srow[label];
   RowRegs<T, NT, KREG> r;
   regs_load(r, srow, V, g);
-  const float c = regs_anchor<true>(r, g, k);
-  float z = 0.f, s_a = 0.f;
+  float c = regs_anchor<true>(r, g, k), z = 0.f, s_a = 0.f;
   auto add = [&](float x) {
     const float d = fmaf(x, k, c), e = fast_exp2(d);
     z += e;
@@ -95,6 +94,9 @@ __global__ __launch_bounds__(NT) void token_stat_kernel(const TokenRows a, int64
     const VecBuffer piece = vec_buffer(srow + g.head + v0 * VEC, left);
 #pragma unroll
     for (int j = 0; j < KREG; ++j) r.v[j] = vec_load<T>(piece, threadIdx.x + j * NT);
+    const float shift = regs_raise(r, left, k, c);
+    s_a = __builtin_amdgcn_ldexpf(fmaf(z, shift, s_a), (int)shift);
+    z = __builtin_amdgcn_ldexpf(z, (int)shift);
 #pragma unroll
     for (int j = 0; j < KREG; ++j) {
       if ((int)threadIdx.x + j * NT < left) {
@@ -246,7 +248,7 @@ __global__ __launch_bounds__(kTokBlock) void pref_join_kernel(const TokenRows a,
       slope = p.beta * (p.smoothing - 1.0 / (1.0 + exp(bh)));
     } else if (p.kind == kPrefHinge) {
       loss = bh < 1.0 ? 1.0 - bh : (bh >= 1.0 ? 0.0 : bh);  // (a NaN stays one)
-      slope = bh < 1.0 ? -p.beta : 0.0;
+      slope = bh < 1.0 ? -p.beta : (bh >= 1.0 ? 0.0 : bh);
     } else {
       const double e = h - 0.5 / p.beta;
       loss = e * e;
@@ -295,34 +297,75 @@ struct PolicyArgs {
 
 // Weight of every sequence's tokens: weight / (live rows), or with per_seq
 // weight / (sequences with a live row) / (live rows of this one).
-// counts[0] = live rows.
-__global__ __launch_bounds__(1024) void policy_weight_kernel(const TokenRows a, int64_t n_seq, int per_seq, float weight,
-                                                             float* __restrict__ seq_weight, int* __restrict__ counts) {
+// counts[0] = live rows.  One workgroup; the smallest power of two of lanes that
+// is no smaller than a sequence takes it, up to a wavefront (4096 sequences of one
+// token, a wavefront each: 175 us), with eight loads in flight, of that sequence
+// or of eight sequences.
+constexpr int kWeightBlock = 1024;
+
+__global__ __launch_bounds__(kWeightBlock) void policy_weight_kernel(const TokenRows a, int64_t n_seq, int per_seq,
+                                                                     float weight, float* __restrict__ seq_weight,
+                                                                     int* __restrict__ counts) {
+  constexpr int kInFlight = 8;
   __shared__ int total, full;
-  const int lane = threadIdx.x % kWave, w = threadIdx.x / kWave;
   if (threadIdx.x == 0) total = full = 0;
-  __syncthreads();
-  const int64_t L = a.r.seq_len;
-  for (int64_t q = w; q < n_seq; q += 1024 / kWave) {
-    int c = 0;
-    for (int64_t i = lane; i < L; i += kWave) {
-      int64_t label;
-      c += token_live<false>(a, q * L + i, &label);
+  const int L = (int)a.r.seq_len, n = (int)n_seq;  // (their product is below 2^22)
+  int lanes = kWave;
+  while (lanes / 2 >= L) lanes /= 2;
+  const int sub = (int)threadIdx.x & (lanes - 1), first = (int)threadIdx.x / lanes, step = kWeightBlock / lanes;
+  int rows = 0, some = 0;
+  auto finish = [&](int q, int c) {  // c: of this lane
+    for (int off = lanes / 2; off > 0; off >>= 1) c += __shfl_xor(c, off, kWave);
+    if (sub != 0 || q >= n) return;
+    seq_weight[q] = (float)c;  // exact: fewer than 2^24 rows
+    rows += c;
+    some += c > 0;
+  };
+  // rows at + u * stride, as far as place + u * by lies below end
+  auto count = [&](int at, int stride, int place, int by, int end, int (&c)[kInFlight]) {
+    int64_t label[kInFlight];
+    bool on[kInFlight];
+#pragma unroll
+    for (int u = 0; u < kInFlight; ++u) {  // (all loads before the first use; out of range, row 0's)
+      const bool in = place + u * by < end;
+      const int row = in ? at + u * stride : 0;
+      label[u] = a.labels[row];
+      on[u] = in && (!a.mask || a.mask[row] != 0);
     }
 #pragma unroll
-    for (int off = kWave / 2; off > 0; off >>= 1) c += __shfl_xor(c, off, kWave);
-    if (lane == 0) {
-      seq_weight[q] = (float)c;  // exact: fewer than 2^24 rows
-      atomicAdd(&total, c);
-      if (c) atomicAdd(&full, 1);
+    for (int u = 0; u < kInFlight; ++u)
+      c[u] += on[u] && label[u] != a.ignore_index && label[u] >= 0 && label[u] < a.r.V;
+  };
+  if (L > kWave) {
+    for (int q = first; q < n; q += step) {
+      int c[kInFlight] = {}, sum = 0;
+      for (int i = sub; i < L; i += kWave * kInFlight) count(q * L + i, kWave, i, kWave, L, c);
+#pragma unroll
+      for (int u = 0; u < kInFlight; ++u) sum += c[u];
+      finish(q, sum);
+    }
+  } else {
+    for (int q0 = first; q0 - first < n; q0 += step * kInFlight) {  // uniform
+      int c[kInFlight] = {};
+      if (sub < L) count(q0 * L + sub, step * L, q0, step, n, c);
+#pragma unroll
+      for (int u = 0; u < kInFlight; ++u) finish(q0 + u * step, c[u]);
     }
   }
+#pragma unroll
+  for (int off = kWave / 2; off > 0; off >>= 1) {
+    rows += __shfl_xor(rows, off, kWave);
+    some += __shfl_xor(some, off, kWave);
+  }
   __syncthreads();
-  for (int64_t q = w; q < n_seq; q += 1024 / kWave) {
-    if (lane == 0) {
-      const float c = seq_weight[q];
-      seq_weight[q] = per_seq ? weight / ((float)full * fmaxf(c, 1.f)) : weight / (float)total;
-    }
+  if (threadIdx.x % kWave == 0) {
+    atomicAdd(&total, rows);
+    atomicAdd(&full, some);
+  }
+  __syncthreads();
+  for (int q = threadIdx.x; q < n; q += kWeightBlock) {
+    const float c = seq_weight[q];
+    seq_weight[q] = per_seq ? weight / ((float)full * fmaxf(c, 1.f)) : weight / (float)total;
   }
   if (threadIdx.x == 0) counts[0] = total;
 }
@@ -333,9 +376,9 @@ __device__ __forceinline__ void policy_term(const PolicyArgs& p, Float2x lp, flo
   const float r = expf((lp.hi - old_lp) + lp.lo);
   const float held = r < p.clip_lo ? p.clip_lo : (r > p.clip_hi ? p.clip_hi : r);
   const float f = r * A, h = held * A;
-  // min(f, h): the gradient flows where the ratio itself decides
+  // min(f, h): the gradient flows where the ratio itself decides (f + h: one of them is NaN, and so is all)
   *term = f <= h ? -f : (h < f ? -h : f + h);
-  *slope = f <= h ? -f : 0.f;
+  *slope = f <= h ? -f : (h < f ? 0.f : f + h);
   if (p.kl_weight != 0.f) {
     const float d = (ref_lp - lp.hi) - lp.lo;
     const float em1 = expm1f(d);
@@ -563,7 +606,7 @@ template <typename T>
 int launch_policy(const TokenRows& a, const PolicyArgs& p, const TokenWs& w, int64_t n_seq, int per_seq, float weight,
                   float* loss_out, hipStream_t st) {
   if (a.r.n_rows == 0) return launch_nan(loss_out, st);
-  hipLaunchKernelGGL(policy_weight_kernel, dim3(1), dim3(1024), 0, st, a, n_seq, per_seq, weight, w.seq, w.counts);
+  hipLaunchKernelGGL(policy_weight_kernel, dim3(1), dim3(kWeightBlock), 0, st, a, n_seq, per_seq, weight, w.seq, w.counts);
   int rc = check_launch();
   if (rc) return rc;
   const dim3 grid((unsigned)a.r.n_rows);

@@ -19,8 +19,19 @@ __device__ __forceinline__ uint32_t top_key(float x) {
 // Number of the row's elements for which f holds.
 template <typename T, int NT, typename F>
 __device__ __forceinline__ int top_count(const T* row, int64_t V, int* lds, F f) {
+  constexpr int VEC = Vec16<T>::N;
+  const VocabGeom g = vocab_geom(row, V);
   int c = 0;
-  for (int64_t i = threadIdx.x; i < V; i += NT) c += f(to_f32(row[i]), (int)i) ? 1 : 0;
+  if ((int)threadIdx.x < g.head) c += f(to_f32(row[threadIdx.x]), (int)threadIdx.x) ? 1 : 0;
+  const int64_t t = g.tail0 + threadIdx.x;
+  if (t < V) c += f(to_f32(row[t]), (int)t) ? 1 : 0;
+#pragma unroll 1
+  for (int64_t v = threadIdx.x; v < g.nvec; v += NT) {
+    const int64_t e0 = g.head + v * VEC;
+    const Vec16<T> r = load16(row + e0);
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) c += f(to_f32(r.v[i]), (int)(e0 + i)) ? 1 : 0;
+  }
 #pragma unroll
   for (int off = kWave / 2; off > 0; off >>= 1) c += __shfl_xor(c, off, kWave);
   __syncthreads();
@@ -106,9 +117,12 @@ __device__ __forceinline__ void top_emit(TopShared<NT>& sh, int n, const T* x, i
 
 // Rows with a NaN, with a sum that needs the true maximum, or with more
 // candidates than fit (thousands of equal logits at the border).  The k-th
-// largest order number is found bit by bit (the largest t such that at least k
-// elements reach it), then the place up to which elements equal to it are
-// taken, likewise; the k elements so defined are collected.
+// largest order number is the bar's, if fewer than k elements exceed the bar (a
+// vocabulary masked but for fewer than k tokens), or found bit by bit (the largest
+// t such that at least k elements reach it); then the place up to which elements
+// equal to it are taken is found likewise, and the k elements so defined are
+// collected.  (4096 x 30522 bf16 with 30 tokens not masked, k = 64: 0.66 ms;
+// all of it bit by bit, an element a thread: 3.3.)
 template <typename T, int NT>
 __device__ __forceinline__ void top_row_walked(const VocabRows& a, int64_t row, const T* x, int k,
                                                T* __restrict__ values, int32_t* __restrict__ indices,
@@ -123,14 +137,19 @@ __device__ __forceinline__ void top_row_walked(const VocabRows& a, int64_t row, 
       l = s.m;
     if (threadIdx.x == 0) lse[row] = l;
   }
-  uint32_t t = 0;
-  for (int bit = 31; bit >= 0; --bit) {
-    const uint32_t c = t | (1u << bit);
-    if (top_count<T, NT>(x, V, sh.counts, [=](float v, int) { return top_key(v) >= c; }) >= k) t = c;
+  const float bar = sh.bar;
+  uint32_t t = top_key(bar);
+  int above = top_count<T, NT>(x, V, sh.counts, [=](float v, int) { return !(v <= bar); });
+  if (above >= k) {  // uniform
+    t = 0;
+    for (int bit = 31; bit >= 0; --bit) {
+      const uint32_t c = t | (1u << bit);
+      if (top_count<T, NT>(x, V, sh.counts, [=](float v, int) { return top_key(v) >= c; }) >= k) t = c;
+    }
+    above = top_count<T, NT>(x, V, sh.counts, [=](float v, int) { return top_key(v) > t; });
   }
-  const int above = top_count<T, NT>(x, V, sh.counts, [=](float v, int) { return top_key(v) > t; });
   int place = 0;  // the largest place such that fewer than k - above elements equal to t lie before it
-  for (int bit = 30; bit >= 0; --bit) {
+  for (int bit = 31 - __builtin_clz((uint32_t)V); bit >= 0; --bit) {
     const int c = place | (1 << bit);
     if (c < V &&
         top_count<T, NT>(x, V, sh.counts, [=](float v, int i) { return i < c && top_key(v) == t; }) < k - above)
@@ -669,8 +688,7 @@ __global__ __launch_bounds__(NT, (KREG > 8 || LONG ? 4 : NT > 256 ? (NT > 512 ? 
 
   RowSum s;
   if (TAIL) {
-    const float c = regs_anchor<true>(r, g, kk);
-    float out = 0.f, in = 0.f;
+    float c = regs_anchor<true>(r, g, kk), out = 0.f, in = 0.f;
     const uint8_t* mark8 = reinterpret_cast<const uint8_t*>(marks);
     auto marked = [&](uint32_t bit) { return ((marks[bit >> 5] >> (bit & 31)) & 1u) != 0; };
     if (tid < g.head && !marked(top_mark_bit(tid, g))) out += fast_exp2(fmaf(r.h(), kk, c));
@@ -685,7 +703,9 @@ __global__ __launch_bounds__(NT, (KREG > 8 || LONG ? 4 : NT > 256 ? (NT > 512 ? 
       }
     };
     if (LONG) {
-      long_each(r, x, g, [&](const Vec16<T>& v, int64_t at) { add(v, (uint32_t)at); });
+      long_each(
+          r, x, g, [&](const Vec16<T>& v, int64_t at) { add(v, (uint32_t)at); },
+          [&](int left) { out = __builtin_amdgcn_ldexpf(out, (int)regs_raise(r, left, kk, c)); });
     } else {
 #pragma unroll
       for (int j = 0; j < KREG; ++j) {

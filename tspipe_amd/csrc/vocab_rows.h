@@ -399,21 +399,20 @@ struct RawMax {
   }
 };
 
-// c of the wavefront.  ALL: by all of its vectors, else by its first ones and, if
-// those are masked, by all.
+// The largest of m and of the wavefront's elements in its first nvec vectors.
+// ALL: of all of them, else of the first ones and, if those are masked, of all.
 template <bool ALL, typename T, int NT, int KREG>
-__device__ __forceinline__ float regs_anchor(const RowRegs<T, NT, KREG>& r, const VocabGeom& g, float k) {
+__device__ __forceinline__ float regs_max(const RowRegs<T, NT, KREG>& r, int nvec, float m, float k) {
   constexpr int VEC = Vec16<T>::N;
   typedef RawMax<T> Raw;
-  float m = fmaxf(r.h(), r.t());
   if (ALL) {
     int32_t raw = Raw::kNone;
 #pragma unroll
     for (int j = 0; j < KREG; ++j)
-      if ((int)threadIdx.x + j * NT < (int)g.nvec) raw = Raw::max2(raw, Raw::of(r.v[j]));
-    if ((int)threadIdx.x < (int)g.nvec) m = fmaxf(m, Raw::value(raw));
+      if ((int)threadIdx.x + j * NT < nvec) raw = Raw::max2(raw, Raw::of(r.v[j]));
+    if ((int)threadIdx.x < nvec) m = fmaxf(m, Raw::value(raw));
   } else {
-    if ((int)threadIdx.x < (int)g.nvec) {
+    if ((int)threadIdx.x < nvec) {
 #pragma unroll
       for (int i = 0; i < VEC; ++i) m = fmaxf(m, to_f32(r.v[0].v[i]));
     }
@@ -422,16 +421,33 @@ __device__ __forceinline__ float regs_anchor(const RowRegs<T, NT, KREG>& r, cons
   if (!(m * k > (ALL ? 0.f : kVrLeast))) {  // (masked, or, by raw bits, nothing above zero: the true maximum)
 #pragma unroll
     for (int j = 0; j < KREG; ++j) {
-      if ((int)threadIdx.x + j * NT < (int)g.nvec) {
+      if ((int)threadIdx.x + j * NT < nvec) {
 #pragma unroll
         for (int i = 0; i < VEC; ++i) m = fmaxf(m, to_f32(r.v[j].v[i]));
       }
     }
     m = wave_max(m);
-    if (!(m * k > kVrLeast)) return kVrNoTerm;
   }
-  const float e = m * k;
+  return m;
+}
+
+// c of the wavefront.
+template <bool ALL, typename T, int NT, int KREG>
+__device__ __forceinline__ float regs_anchor(const RowRegs<T, NT, KREG>& r, const VocabGeom& g, float k) {
+  const float e = regs_max<ALL>(r, (int)g.nvec, fmaxf(r.h(), r.t()), k) * k;
+  if (!(e > kVrLeast)) return kVrNoTerm;
   return e < 1e30f ? -rintf(e) : 0.f;  // (an infinite logit makes the sum overflow whatever c is)
+}
+
+// A later piece of the row, of nvec vectors, in r: where it holds something larger
+// than what c was taken from, c follows it.  Returns the exponent (<= 0) by which
+// sums taken so far have to be moved.
+template <typename T, int NT, int KREG>
+__device__ __forceinline__ float regs_raise(const RowRegs<T, NT, KREG>& r, int nvec, float k, float& c) {
+  const float e = regs_max<true>(r, nvec, -__builtin_inff(), k) * k;
+  const float old = c;
+  if (e > kVrLeast && e < 1e30f) c = fminf(c, -rintf(e));
+  return fmaxf(c - old, -1000.f);
 }
 
 struct RowSum {  // z = sum 2^(x k + c), a: nothing, or one of the two below
@@ -584,14 +600,16 @@ __device__ __forceinline__ double block_sum_f64(double v, double* lds) {
 }
 
 // Rows longer than the registers hold, in pieces of NT * KREG vectors: f(vector,
-// its place) for each.  The first piece is in r; a register that is done with
-// takes the next piece's vector at once, so that loads are always under way.
-template <typename T, int NT, int KREG, typename F>
-__device__ __forceinline__ void long_each(RowRegs<T, NT, KREG>& r, const T* row, const VocabGeom& g, F f) {
+// its place) for each, `later`(its vectors) in front of each piece but the first.
+// The first piece is in r; a register that is done with takes the next piece's
+// vector at once, so that loads are always under way.
+template <typename T, int NT, int KREG, typename F, typename P>
+__device__ __forceinline__ void long_each(RowRegs<T, NT, KREG>& r, const T* row, const VocabGeom& g, F f, P later) {
   constexpr int VEC = Vec16<T>::N;
   for (int64_t v0 = 0;; v0 += NT * KREG) {
     const int left = g.nvec - v0 < NT * KREG ? (int)(g.nvec - v0) : NT * KREG;
     const int64_t after = g.nvec - v0 - left;
+    if (v0 > 0) later(left);
     const VecBuffer next = vec_buffer(row + g.head + (v0 + left) * VEC, after < NT * KREG ? (int)after : NT * KREG);
 #pragma unroll
     for (int j = 0; j < KREG; ++j) {
@@ -610,17 +628,19 @@ __device__ __forceinline__ void long_each(RowRegs<T, NT, KREG>& r, const T* row,
 template <typename T, int NT, int KREG>
 __device__ __forceinline__ RowSum long_sum(RowRegs<T, NT, KREG>& r, const T* row, const VocabGeom& g, float k, RowSum* lds) {
   constexpr int VEC = Vec16<T>::N;
-  const float c = regs_anchor<true>(r, g, k);
-  float z = 0.f;
+  float c = regs_anchor<true>(r, g, k), z = 0.f;
   auto add = [&](float x) { z += fast_exp2(fmaf(x, k, c)); };
   if (threadIdx.x < kWave) {
     add(r.h());
     add(r.t());
   }
-  long_each(r, row, g, [&](const Vec16<T>& v, int64_t) {
+  long_each(
+      r, row, g,
+      [&](const Vec16<T>& v, int64_t) {
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) add(to_f32(v.v[i]));
-  });
+        for (int i = 0; i < VEC; ++i) add(to_f32(v.v[i]));
+      },
+      [&](int left) { z = __builtin_amdgcn_ldexpf(z, (int)regs_raise(r, left, k, c)); });
   return rowsum_block<NT / kWave, kSumOnly>(c, z, 0.f, lds);
 }
 
@@ -652,7 +672,7 @@ __device__ __forceinline__ void long_map(RowRegs<T, NT, KREG>& r, const VocabGeo
 #pragma unroll
       for (int i = 0; i < VEC; ++i) p[i] = o.v[i];
     }
-  });
+  }, [](int) {});
 }
 
 // This thread's share of sum(v[0..n)) when NT threads walk the array together, in

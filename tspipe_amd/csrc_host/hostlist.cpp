@@ -547,9 +547,10 @@ struct VocabView {
   int code;
 };
 
-// False when the logits are not two- or three-dimensional device tensors with a dense last dimension.
+// False when the logits are not two- or three-dimensional device tensors with a dense last dimension, or
+// carry a forward-mode tangent (which the Python functions refuse).
 bool vocab_view(const at::Tensor& x, VocabView* v) {
-  if (!x.is_cuda() || x.layout() != at::kStrided || (x.dim() != 2 && x.dim() != 3)) return false;
+  if (!x.is_cuda() || x.layout() != at::kStrided || (x.dim() != 2 && x.dim() != 3) || x._fw_grad(0).defined()) return false;
   v->code = dtype_code(x.scalar_type());
   v->V = x.size(-1);
   if (v->code < 0 || v->V < 1 || (v->V > 1 && x.stride(-1) != 1)) return false;
