@@ -781,3 +781,46 @@ def test_forward_mode_is_refused(device, monkeypatch):
         return True
 
     assert _both_ways(monkeypatch, refused) == (True, True)
+
+
+def test_capture_while_an_eager_graph_holds_the_leaf(device, monkeypatch):
+    from tspipe_amd import _lib
+    x, labels, _ = make((2, 5, 700), torch.float32, 191)
+    lab, ref = labels.to(device), torch.zeros(2, 5, device=device)
+    leaf = x.to(device).requires_grad_()
+    calls = [lambda: ta.token_log_probs(leaf, lab).sum(), lambda: ta.preference_loss(leaf, lab, ref),
+             lambda: ta.clipped_policy_loss(leaf, lab, ref, ref),
+             lambda: ta.top_logits_distil_loss(leaf, *ta.top_logits(leaf, 3)[:2], 1.0)]
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        calls[1]()  # (workspaces and code are there before the captures)
+    side.synchronize()
+    eager = calls[0]()
+    want, = torch.autograd.grad(eager, leaf, retain_graph=True)
+    host = _lib.host_helper()
+    assert host.leaf_on_default_stream(leaf)
+    with torch.cuda.stream(side):
+        assert host.leaf_on_default_stream(leaf)
+        calls[1]()  # outside a capture there is nothing to refuse
+    side.synchronize()
+
+    def refused():
+        for call in calls:
+            with pytest.raises(RuntimeError, match="captured"):
+                with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                    call()
+        return True
+
+    assert _both_ways(monkeypatch, refused) == (True, True)
+    monkeypatch.undo()
+    del eager
+    assert not torch.cuda.is_current_stream_capturing()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        assert not host.leaf_on_default_stream(leaf)
+        got, = torch.autograd.grad(calls[0](), leaf)
+    for _ in range(3):
+        got.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert bits_equal(got, want)

@@ -165,7 +165,8 @@ def host_helper():
                         mod.bind_vocab(addr(handle.ts_token_logp_fwd), addr(handle.ts_token_logp_bwd),
                                        addr(handle.ts_token_loss_workspace_bytes), addr(handle.ts_preference_fwd_bwd),
                                        addr(handle.ts_policy_fwd_bwd), addr(handle.ts_top_logits),
-                                       addr(handle.ts_top_distil_workspace_bytes), addr(handle.ts_top_distil_fwd_bwd))
+                                       addr(handle.ts_top_distil_workspace_bytes), addr(handle.ts_top_distil_fwd_bwd),
+                                       addr(handle.hipStreamIsCapturing))
                 _host = mod
             _host_tried = True
     return _host

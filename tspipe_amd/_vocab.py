@@ -75,7 +75,13 @@ def rows_of(logits: Tensor, what: str) -> Rows:
 def recorded(logits: Tensor) -> Tensor:
     """The logits as an autograd function should see them: without gradient
     mode nothing is recorded, so no gradient buffer is wanted either."""
-    return logits if torch.is_grad_enabled() else logits.detach()
+    if not torch.is_grad_enabled():
+        return logits.detach()
+    if logits.requires_grad and logits.is_leaf and logits.is_cuda:
+        host = _lib.host_helper()
+        if host is not None and hasattr(host, "check_capture"):
+            host.check_capture(logits, _lib.current_stream_ptr(logits.device))
+    return logits
 
 
 def same_device(device, **tensors: Optional[Tensor]) -> None:

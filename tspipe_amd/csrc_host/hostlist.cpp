@@ -526,10 +526,11 @@ static struct {
   top_fn top = nullptr;
   top_ws_fn top_ws = nullptr;
   top_distil_fn top_distil = nullptr;
+  int (*is_capturing)(void*, int*) = nullptr;  // the HIP runtime's question
 } g_vocab;
 
 void bind_vocab(uintptr_t logp_fwd, uintptr_t logp_bwd, uintptr_t token_ws, uintptr_t pref, uintptr_t policy,
-                uintptr_t top, uintptr_t top_ws, uintptr_t top_distil) {
+                uintptr_t top, uintptr_t top_ws, uintptr_t top_distil, uintptr_t is_capturing) {
   g_vocab.logp_fwd = reinterpret_cast<logp_fwd_fn>(logp_fwd);
   g_vocab.logp_bwd = reinterpret_cast<logp_bwd_fn>(logp_bwd);
   g_vocab.token_ws = reinterpret_cast<token_ws_fn>(token_ws);
@@ -538,6 +539,7 @@ void bind_vocab(uintptr_t logp_fwd, uintptr_t logp_bwd, uintptr_t token_ws, uint
   g_vocab.top = reinterpret_cast<top_fn>(top);
   g_vocab.top_ws = reinterpret_cast<top_ws_fn>(top_ws);
   g_vocab.top_distil = reinterpret_cast<top_distil_fn>(top_distil);
+  g_vocab.is_capturing = reinterpret_cast<int (*)(void*, int*)>(is_capturing);
 }
 
 // Logits as the entry points take them.
@@ -582,6 +584,28 @@ inline at::Tensor like(const at::Tensor& x, at::IntArrayRef sizes, at::ScalarTyp
 }
 
 inline bool records(const at::Tensor& x) { return at::GradMode::is_enabled() && x.requires_grad(); }
+
+// A leaf's gradient is accumulated on the stream on which a graph first met the
+// leaf, for as long as any graph holds its accumulator.
+bool leaf_on_default_stream(const at::Tensor& x) {
+  if (!x.is_leaf() || !x.requires_grad()) return false;
+  const auto edges = torch::autograd::collect_next_edges(x);
+  if (edges.empty() || !edges[0].function) return false;
+  const auto stream = edges[0].function->stream();
+  return stream.has_value() && stream->id() == 0;
+}
+
+// A captured backward pass that reaches an accumulator of the default stream
+// would make that stream part of the capture, which the runtime does not allow
+// and the autograd engine does not survive.
+void check_capture(const at::Tensor& x, int64_t stream) {
+  int status = 0;
+  if (stream == 0 || !g_vocab.is_capturing || !x.is_leaf()) return;
+  if (g_vocab.is_capturing(reinterpret_cast<void*>(stream), &status) != 0 || status == 0) return;
+  TORCH_CHECK(!leaf_on_default_stream(x),
+              "these logits are a leaf of an eager graph that ran on the default stream and is still alive: a backward "
+              "pass captured now would have to add to its gradient there. Drop that graph (its loss) before the capture");
+}
 
 // Hands out a gradient that the forward pass computed, scaled by the incoming one.
 struct ReadyGradNode : public torch::autograd::Node {
@@ -656,6 +680,7 @@ py::object vocab_log_probs(const at::Tensor& x, const at::Tensor& labels, const 
     py::gil_scoped_release no_gil;
     c10::DeviceGuard guard(x.device());
     const bool record = records(x);
+    if (record) check_capture(x, stream);
     out = like(x, labels.sizes(), at::kFloat);
     at::Tensor stats;
     if (record) stats = like(x, {v.n_seq * v.seq_len, 2}, at::kFloat);
@@ -698,6 +723,7 @@ py::object vocab_preference(const at::Tensor& x, const at::Tensor& labels, const
     c10::DeviceGuard guard(x.device());
     void* st = reinterpret_cast<void*>(stream);
     const bool record = records(x);
+    if (record) check_capture(x, stream);
     at::Tensor ws = like(x, {(int64_t)g_vocab.token_ws(v.n_seq, v.seq_len)}, at::kByte), grad;
     loss = like(x, {}, at::kFloat);
     rewards = like(x, {v.n_seq}, at::kFloat);
@@ -732,6 +758,7 @@ py::object vocab_policy(const at::Tensor& x, const at::Tensor& labels, const at:
     c10::DeviceGuard guard(x.device());
     void* st = reinterpret_cast<void*>(stream);
     const bool record = records(x);
+    if (record) check_capture(x, stream);
     at::Tensor ws = like(x, {(int64_t)g_vocab.token_ws(v.n_seq, v.seq_len)}, at::kByte), grad;
     loss = like(x, {}, at::kFloat);
     logp = like(x, labels.sizes(), at::kFloat);
@@ -787,6 +814,7 @@ py::object vocab_top_distil(const at::Tensor& x, const at::Tensor& values, const
     c10::DeviceGuard guard(x.device());
     void* st = reinterpret_cast<void*>(stream);
     const bool record = records(x);
+    if (record) check_capture(x, stream);
     at::Tensor ws = like(x, {(int64_t)g_vocab.top_ws(v.n_seq * v.seq_len, (int)k)}, at::kByte), grad;
     loss = like(x, {}, at::kFloat);
     if (record) grad = like(x, x.sizes(), x.scalar_type());
@@ -818,6 +846,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("bind_losses", &bind_losses);
   m.def("row_loss", &row_loss);
   m.def("bind_vocab", &bind_vocab);
+  m.def("leaf_on_default_stream", &leaf_on_default_stream);
+  m.def("check_capture", &check_capture);
   m.def("vocab_log_probs", &vocab_log_probs);
   m.def("vocab_preference", &vocab_preference);
   m.def("vocab_policy", &vocab_policy);
