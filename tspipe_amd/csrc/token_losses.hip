@@ -51,16 +51,20 @@ struct TokenGrad {
 };
 
 // log_ratio (optional): the log probability minus ref[row] in 64 bits, for the
-// sums over whole sequences.  Rows longer than NT * KREG vectors are walked in
-// pieces of that size.
+// sums over whole sequences.  The threads' sums are joined and the logarithm is
+// taken in 64 bits as well (the row's registers are free by then): a sequence's
+// sum of differences to a reference that nearly agrees shows every unit of fp32.
+// Rows longer than NT * KREG vectors are walked in pieces of that size.
 template <typename T, int NT, int KREG>
 __global__ __launch_bounds__(NT) void token_stat_kernel(const TokenRows a, int64_t row0, const float* __restrict__ ref,
                                                         float* __restrict__ logp, double* __restrict__ log_ratio,
                                                         float2* __restrict__ stats, unsigned* __restrict__ ticket) {
   if (ticket && blockIdx.x == 0 && threadIdx.x == 0) *ticket = 0u;  // of the next kernel
   constexpr int VEC = Vec16<T>::N;
-  __shared__ RowSum lds[NT / kWave];
-  __shared__ VocabStat lds_v[NT / kWave];
+  constexpr int NW = NT / kWave;
+  __shared__ double lds_z[NW];
+  __shared__ float lds_c[NW], lds_a[NW];
+  __shared__ VocabStat lds_v[NW];
   const int64_t row = row0 + blockIdx.x;
   int64_t label;
   if (!token_live<true>(a, row, &label)) {
@@ -107,21 +111,48 @@ __global__ __launch_bounds__(NT) void token_stat_kernel(const TokenRows a, int64
       __builtin_amdgcn_sched_barrier(0);
     }
   }
-  const RowSum s = rowsum_block<NT / kWave, kSumMean>(c, z, s_a, lds);
-  Float2x lp;
+  double sum = wave_sum_f64((double)z);
+  s_a = wave_sum(s_a);
+  if (NW > 1) {  // (as rowsum_put and rowsum_get do it; s_a = sum of terms times their exponents)
+    if (threadIdx.x % kWave == 0) {
+      lds_z[threadIdx.x / kWave] = sum;
+      lds_c[threadIdx.x / kWave] = c;
+      lds_a[threadIdx.x / kWave] = s_a;
+    }
+    __syncthreads();
+    const int w = threadIdx.x % NW;
+    const float wc = lds_c[w], wz = (float)lds_z[w];
+    c = wc;
+#pragma unroll
+    for (int off = NW / 2; off > 0; off >>= 1) c = fminf(c, __shfl_xor(c, off, kWave));
+    const float d = c - wc;
+    const int shift = (int)fmaxf(d, -1000.f);
+    sum = __builtin_amdgcn_ldexp(lds_z[w], shift);
+    s_a = __builtin_amdgcn_ldexpf(fmaf(wz, d, lds_a[w]), shift);
+#pragma unroll
+    for (int off = NW / 2; off > 0; off >>= 1) {
+      sum += __shfl_xor(sum, off, kWave);
+      s_a += __shfl_xor(s_a, off, kWave);
+    }
+  }
+  z = (float)sum;
+  const float x = to_f32(label_logit);
+  double lp;
   float2 st;
-  if (s.ok) {
+  if (z > 1e-30f && z < __builtin_inff() && c < kVrNoTerm) {  // uniform
     if (threadIdx.x != 0) return;
-    lp = rowsum_log_prob<true>(a.r, s, to_f32(label_logit));
-    st = make_float2(s.c, s.z);
+    const double xk = (double)x * (double)k, mean = (double)(s_a / z) - (double)c;  // mean of x k under the soft-max
+    lp = x == -__builtin_inff() ? (double)x : kVrLn2 * (xk + (double)c + (double)a.r.k_rel * (xk - mean)) - log(sum);
+    st = make_float2(c, z);
   } else {
-    const VocabStat sv = vstat_block<NT / kWave>(vocab_stat_walk<T, NT>(srow, V, k), k, lds_v);
+    const VocabStat sv = vstat_block<NW>(vocab_stat_walk<T, NT>(srow, V, k), k, lds_v);
     if (threadIdx.x != 0) return;
-    lp = vstat_log_prob(a.r, sv, to_f32(label_logit));
+    const Float2x l = vstat_log_prob(a.r, sv, x);
+    lp = (double)l.hi + (double)l.lo;
     st = make_float2(sv.m, -sv.z);
   }
-  if (logp) logp[row] = lp.hi;
-  if (log_ratio) log_ratio[row] = ((double)lp.hi - (ref ? (double)ref[row] : 0.0)) + (double)lp.lo;
+  if (logp) logp[row] = (float)lp;
+  if (log_ratio) log_ratio[row] = lp - (ref ? (double)ref[row] : 0.0);
   if (stats) stats[row] = st;
 }
 
@@ -456,7 +487,7 @@ __global__ __launch_bounds__(NT) void policy_rows_kernel(const TokenRows a, cons
   regs_load(r, srow, V, g);
   const RowSum s = regs_sum(r, g, a.r.k, lds);
   if (s.ok) {
-    if (threadIdx.x == 0) coef = policy_finish(a, p, pr, row, rowsum_log_prob<false>(a.r, s, to_f32(pr.label_logit)));
+    if (threadIdx.x == 0) coef = policy_finish(a, p, pr, row, rowsum_log_prob(a.r, s, to_f32(pr.label_logit)));
     if (!grow) return;
     __syncthreads();
     const TokenGrad f(a.r.k, make_float2(s.c, s.z), coef);

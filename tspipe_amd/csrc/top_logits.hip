@@ -417,16 +417,16 @@ __global__ __launch_bounds__(NT, NT > 256 ? 8 : 1) void top_logits_kernel(const 
     if (!MULTI || after == 0) break;
     if ((v0 / (NT * KREG)) % 2 == 1) fits = top_expand<T, NT, false, MULTI>(sh, k);
   }
-  const RowSum mine = rowsum_put<NT / kWave, kSumOnly>(c, z, 0.f, sh.sums);
+  const RowSum mine = rowsum_put<NT / kWave, false>(c, z, 0.f, sh.sums);
   fits = fits && top_expand<T, NT, true, MULTI>(sh, k);
-  const RowSum s = rowsum_get<NT / kWave, kSumOnly>(mine, sh.sums);
+  const RowSum s = rowsum_get<NT / kWave, false>(mine, sh.sums);
   if (!s.ok || !fits) {
     __syncthreads();
     for (int i = tid; i < 2 * kTopMax; i += NT) sh.rank[i] = 0;
     top_row_walked<T, NT>(a, row, x, k, values, indices, lse, sh);
     return;
   }
-  if (tid == 0 && lse) lse[row] = -rowsum_log_prob<false>(a, s, 0.f).hi;  // the log probability of a logit of 0
+  if (tid == 0 && lse) lse[row] = -rowsum_log_prob(a, s, 0.f).hi;  // the log probability of a logit of 0
   top_emit<T, NT>(sh, sh.n, x, row, k, values, indices);
 }
 
@@ -459,12 +459,6 @@ __device__ __forceinline__ float top_value(const void* v, int dtype, int64_t i) 
   if (dtype == TS_F32) return reinterpret_cast<const float*>(v)[i];
   if (dtype == TS_BF16) return to_f32(reinterpret_cast<const bf16_t*>(v)[i]);
   return to_f32(reinterpret_cast<const f16_t*>(v)[i]);
-}
-
-__device__ __forceinline__ double wave_sum_f64(double v) {
-#pragma unroll
-  for (int off = kWave / 2; off > 0; off >>= 1) v += __shfl_xor(v, off, kWave);
-  return v;
 }
 
 // Everything that depends on the teacher alone, in 64 bits (what the teacher
@@ -721,7 +715,7 @@ __global__ __launch_bounds__(NT, (KREG > 8 || LONG ? 4 : NT > 256 ? (NT > 512 ? 
       if (idx[i] >= 0) in += fast_exp2(fmaf(ex(i), kk, c));
     // (a wavefront of nothing but -inf has no exponent of its own to take entries by)
     if (!(c < kVrNoTerm) && in > 0.f) in = __builtin_inff();
-    s = rowsum_block<NW, kSumSecond>(c, out, in, sh.sums);
+    s = rowsum_block<NW, true>(c, out, in, sh.sums);
     s.ok = s.ok && (t.rest == 0.f || s.z > 1e-30f);
   } else {
     s = LONG ? long_sum(r, x, g, kk, sh.sums) : regs_sum(r, g, kk, sh.sums);
@@ -739,7 +733,7 @@ __global__ __launch_bounds__(NT, (KREG > 8 || LONG ? 4 : NT > 256 ? (NT > 512 ? 
         regs_map(r, g, x, grow, V, -1, other, none);
       patch([&](float xv) { return fast_exp2(fmaf(xv, kk, c)) * rz; });
     }
-    loss([&](float xv) { return rowsum_log_prob<false>(a.r, s, xv); }, [&]() { return ln_share(log2_2x(rest_z), s.z); });
+    loss([&](float xv) { return rowsum_log_prob(a.r, s, xv); }, [&]() { return ln_share(log2_2x(rest_z), s.z); });
     return;
   }
   __syncthreads();

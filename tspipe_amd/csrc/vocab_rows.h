@@ -450,28 +450,23 @@ __device__ __forceinline__ float regs_raise(const RowRegs<T, NT, KREG>& r, int n
   return fmaxf(c - old, -1000.f);
 }
 
-struct RowSum {  // z = sum 2^(x k + c), a: nothing, or one of the two below
+struct RowSum {  // z = sum 2^(x k + c); a, with TWO: another such sum, and the row's sum is z + a
   float c, z, a;
   bool ok;
-};
-enum {
-  kSumOnly = 0,
-  kSumMean = 1,   // a = sum 2^(x k + c) (x k + c)
-  kSumSecond = 2  // a = another sum of 2^(x k + c); the row's sum is z + a
 };
 
 // Merged over a workgroup of NW wavefronts: each leaves its sums in `lds` (NW
 // RowSums), and after a barrier every thread gets the whole.
-template <int NW, int KIND>
+template <int NW, bool TWO>
 __device__ __forceinline__ RowSum rowsum_put(float c, float z, float a, RowSum* lds) {
   z = wave_sum(z);
-  if (KIND != kSumOnly) a = wave_sum(a);
+  if (TWO) a = wave_sum(a);
   const RowSum r{c, z, a, true};
   if (NW > 1 && threadIdx.x % kWave == 0) lds[threadIdx.x / kWave] = r;
   return r;
 }
 
-template <int NW, int KIND>
+template <int NW, bool TWO>
 __device__ __forceinline__ RowSum rowsum_get(RowSum r, const RowSum* lds) {
   if (NW > 1) {
     // lane i takes the sum of wavefront i % NW (all NW of them in every lane would need 3 NW registers)
@@ -483,37 +478,33 @@ __device__ __forceinline__ RowSum rowsum_get(RowSum r, const RowSum* lds) {
     const float d = C - w.c;
     const int shift = (int)fmaxf(d, -1000.f);
     r = RowSum{C, __builtin_amdgcn_ldexpf(w.z, shift), 0.f, true};
-    if (KIND == kSumMean) r.a = __builtin_amdgcn_ldexpf(fmaf(w.z, d, w.a), shift);
-    if (KIND == kSumSecond) r.a = __builtin_amdgcn_ldexpf(w.a, shift);
+    if (TWO) r.a = __builtin_amdgcn_ldexpf(w.a, shift);
 #pragma unroll
     for (int off = NW / 2; off > 0; off >>= 1) {
       r.z += __shfl_xor(r.z, off, kWave);
-      if (KIND != kSumOnly) r.a += __shfl_xor(r.a, off, kWave);
+      if (TWO) r.a += __shfl_xor(r.a, off, kWave);
     }
   }
-  const float all = KIND == kSumSecond ? r.z + r.a : r.z;
+  const float all = TWO ? r.z + r.a : r.z;
   r.ok = all > 1e-30f && all < __builtin_inff() && r.c < kVrNoTerm;
   return r;
 }
 
-template <int NW, int KIND>
+template <int NW, bool TWO>
 __device__ __forceinline__ RowSum rowsum_block(float c, float z, float a, RowSum* lds) {
-  const RowSum r = rowsum_put<NW, KIND>(c, z, a, lds);
+  const RowSum r = rowsum_put<NW, TWO>(c, z, a, lds);
   if (NW > 1) __syncthreads();
-  return rowsum_get<NW, KIND>(r, lds);
+  return rowsum_get<NW, TWO>(r, lds);
 }
 
-// ln of the soft-max probability of a logit of the row.  Without the sum a the
-// factor k stays as rounded, in the logit's own exponent too: what the rounding
-// took then counts only for the logit's distance from the row's mean.
-template <bool WITH_MEAN>
+// ln of the soft-max probability of a logit of the row.  The factor k stays as
+// rounded, in the logit's own exponent too: what the rounding took then counts
+// only for the logit's distance from the row's mean.
 __device__ __forceinline__ Float2x rowsum_log_prob(const VocabRows& r, const RowSum& s, float x) {
 #pragma clang fp contract(off)
   const Float2x p = two_mul(x, r.k), q = two_sum(p.hi, s.c);
   if (x < -1e38f && x > -__builtin_inff()) return Float2x{(float)((double)x * r.inv_T), 0.f};  // (x k may overflow)
-  float lo = p.lo + q.lo;
-  if (WITH_MEAN) lo += r.k_rel * (p.hi - (s.a / s.z - s.c));  // a / z - c: mean of x k under the soft-max
-  return ln_share(Float2x{q.hi, lo}, s.z);
+  return ln_share(Float2x{q.hi, p.lo + q.lo}, s.z);
 }
 
 // One thread's terms of its registers: f(x, exponent) per element.
@@ -541,7 +532,7 @@ __device__ __forceinline__ RowSum regs_sum(RowRegs<T, NT, KREG>& r, const VocabG
     add(r.t());
   }
   regs_each(r, g, add);
-  return rowsum_block<NT / kWave, kSumOnly>(c, z, 0.f, lds);
+  return rowsum_block<NT / kWave, false>(c, z, 0.f, lds);
 }
 
 // grow[j] = f(x[j]) from registers, but for element `special` (or -1), which
@@ -583,12 +574,17 @@ __device__ __forceinline__ void regs_map(RowRegs<T, NT, KREG>& r, const VocabGeo
   }
 }
 
+__device__ __forceinline__ double wave_sum_f64(double v) {
+#pragma unroll
+  for (int off = kWave / 2; off > 0; off >>= 1) v += __shfl_xor(v, off, kWave);
+  return v;
+}
+
 // Sum of doubles over a workgroup of NW wavefronts, in a fixed order; every
 // thread gets the result.
 template <int NW>
 __device__ __forceinline__ double block_sum_f64(double v, double* lds) {
-#pragma unroll
-  for (int off = kWave / 2; off > 0; off >>= 1) v += __shfl_xor(v, off, kWave);
+  v = wave_sum_f64(v);
   if (NW == 1) return v;
   __syncthreads();
   if (threadIdx.x % kWave == 0) lds[threadIdx.x / kWave] = v;
@@ -641,7 +637,7 @@ __device__ __forceinline__ RowSum long_sum(RowRegs<T, NT, KREG>& r, const T* row
         for (int i = 0; i < VEC; ++i) add(to_f32(v.v[i]));
       },
       [&](int left) { z = __builtin_amdgcn_ldexpf(z, (int)regs_raise(r, left, k, c)); });
-  return rowsum_block<NT / kWave, kSumOnly>(c, z, 0.f, lds);
+  return rowsum_block<NT / kWave, false>(c, z, 0.f, lds);
 }
 
 template <typename T, int NT, int KREG, typename F, typename G>
