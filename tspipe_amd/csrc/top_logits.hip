@@ -49,41 +49,56 @@ __device__ __forceinline__ float top_unkey(uint32_t key) {
   return __uint_as_float((key & 0x80000000u) ? key & 0x7fffffffu : ~key);
 }
 
-// Vectors with a candidate and candidates a row may have at a time.  64 threads
-// may have to take a whole row of theirs (k close to V).
+// Short rows come in two arrangements.  FEW, one wavefront, for k up to kTopFew:
+// at most 88 of its vectors reach the bar, but for equal logits, and 10 KB of LDS
+// are enough.  For larger k, up to the whole row, 256 threads with a vector each.
+// (One wavefront with the LDS for a whole row, 26 KB: 8192 x 1000 bf16 k = 64
+// takes 63 us instead of 30, k = 128 234 instead of 64.)
+constexpr int kTopFew = 64;
+
+// Vectors with a candidate, candidates, and candidates to rank that a row may
+// have at a time.
+template <int NT, int KREG>
+constexpr int top_hit_cap() { return NT == 64 ? 128 : KREG == 1 ? 256 : NT == 256 ? 512 : 1024; }
+template <int NT, int KREG>
+constexpr int top_cand_cap() { return NT == 64 ? 768 : KREG == 1 ? 2304 : 1536; }
 template <int NT>
-constexpr int top_hit_cap() { return NT == 64 ? 288 : NT == 256 ? 512 : 1024; }
-template <int NT>
-constexpr int top_cand_cap() { return NT == 64 ? 2304 : 1536; }
+constexpr int top_rank_cap() { return NT == 64 ? 256 : 2 * kTopMax; }
 
 // Groups per thread when k is large: short rows have few vectors per thread, and
 // a group each gives the bar they need (1000 bf16, k = 64, one group per thread:
-// 64 groups, 600 candidates, 456 us for 8192 rows).
+// 64 groups, 600 candidates, 456 us for 8192 rows); a thread with one vector makes
+// four groups of that.
 template <int NT>
 constexpr int top_groups() { return NT <= 256 ? 4 : 2; }
 
-template <int NT>
+template <int NT, int KREG>
 struct TopShared {
+  static constexpr int kMost = NT == 64 ? kTopFew : kTopMax;  // k
+  static constexpr int kKept = kMost + kMost / 8 + 4;         // what top_refine leaves
   union {
     uint32_t group[top_groups<NT>() * NT];  // order numbers of the groups' maxima
-    uint64_t kept[kTopMax];
-    u32x4 hit[top_hit_cap<NT>()];  // vectors with a candidate
+    uint64_t kept[kKept];
+    u32x4 hit[top_hit_cap<NT, KREG>()];  // vectors with a candidate
   };
-  int hit_at[top_hit_cap<NT>()];  // their first elements' places
-  uint64_t cand[top_cand_cap<NT>()];  // order number and place, larger for smaller places
+  int hit_at[top_hit_cap<NT, KREG>()];  // their first elements' places
+  alignas(16) uint64_t cand[top_cand_cap<NT, KREG>()];  // order number and place, larger for smaller places
   RowSum sums[NT / kWave];
   VocabStat stats[NT / kWave];
   int counts[NT / kWave];
-  int rank[2 * kTopMax];
+  int rank[top_rank_cap<NT>()];
   int n, n_hit;
   float bar;
 };
 
 // Ranks the n candidates by counting, for each one, those that are larger; the
 // first k leave.  With fewer candidates than threads several threads count for
-// each.  sh.rank is 0 on entry.
-template <typename T, int NT>
-__device__ __forceinline__ void top_emit(TopShared<NT>& sh, int n, const T* x, int64_t row, int k,
+// each.  256 threads with more of them than threads count for two at a reading of
+// two: reading bounds it there (8192 x 4000 bf16, k = 256: 145 us, one by one 185;
+// with fewer candidates that is slower, 8192 x 1000 and k = 128 73 us, one by one
+// 64).  sh.rank is 0 on entry.
+template <typename T, int NT, int KREG>
+__device__ __forceinline__ void top_emit(TopShared<NT, KREG>& sh, int n, const T* x, int64_t row, int k,
                                          T* __restrict__ values, int32_t* __restrict__ indices) {
   constexpr int NW = NT / kWave;
   const int all = __builtin_amdgcn_readfirstlane(n);
@@ -97,12 +112,30 @@ __device__ __forceinline__ void top_emit(TopShared<NT>& sh, int n, const T* x, i
   }
   const int per = (int)(((float)all + (float)parts - 0.5f) / (float)parts);  // all / parts, rounded up
   const int lo = part * per, hi = part < parts ? (lo + per < all ? lo + per : all) : lo;
-  for (int c = first * kWave + (int)threadIdx.x % kWave; c < all; c += NT) {
-    const uint64_t me = sh.cand[c];
-    int rank = 0;
+  if (NT == 256 && all > NT) {  // uniform; at most twice as many
+    const int c0 = (int)threadIdx.x, c1 = c0 + NT;
+    const uint64_t me0 = sh.cand[c0], me1 = c1 < all ? sh.cand[c1] : ~0ull;
+    int rank0 = 0, rank1 = 0, i = 0;
+#pragma unroll 2
+    for (; i + 1 < all; i += 2) {
+      const ulonglong2 two = *reinterpret_cast<const ulonglong2*>(&sh.cand[i]);
+      rank0 += (int)(two.x > me0) + (int)(two.y > me0);
+      rank1 += (int)(two.x > me1) + (int)(two.y > me1);
+    }
+    if (i < all) {
+      rank0 += (int)(sh.cand[i] > me0);
+      rank1 += (int)(sh.cand[i] > me1);
+    }
+    sh.rank[c0] = rank0;
+    if (c1 < all) sh.rank[c1] = rank1;
+  } else {
+    for (int c = first * kWave + (int)threadIdx.x % kWave; c < all; c += NT) {
+      const uint64_t me = sh.cand[c];
+      int rank = 0;
 #pragma unroll 4
-    for (int i = lo; i < hi; ++i) rank += sh.cand[i] > me;
-    if (rank) atomicAdd(&sh.rank[c], rank);
+      for (int i = lo; i < hi; ++i) rank += sh.cand[i] > me;
+      if (rank) atomicAdd(&sh.rank[c], rank);
+    }
   }
   __syncthreads();
   for (int c = threadIdx.x; c < n; c += NT) {
@@ -123,10 +156,10 @@ __device__ __forceinline__ void top_emit(TopShared<NT>& sh, int n, const T* x, i
 // equal to it are taken is found likewise, and the k elements so defined are
 // collected.  (4096 x 30522 bf16 with 30 tokens not masked, k = 64: 0.66 ms;
 // all of it bit by bit, an element a thread: 3.3.)
-template <typename T, int NT>
+template <typename T, int NT, int KREG>
 __device__ __forceinline__ void top_row_walked(const VocabRows& a, int64_t row, const T* x, int k,
                                                T* __restrict__ values, int32_t* __restrict__ indices,
-                                               float* __restrict__ lse, TopShared<NT>& sh) {
+                                               float* __restrict__ lse, TopShared<NT, KREG>& sh) {
   const int64_t V = a.V;
   if (lse) {
     const VocabStat s = vstat_block<NT / kWave>(vocab_stat_walk<T, NT>(x, V, a.k), a.k, sh.stats);
@@ -161,29 +194,43 @@ __device__ __forceinline__ void top_row_walked(const VocabRows& a, int64_t row, 
     const uint32_t key = top_key(to_f32(x[i]));
     if (key > t || (key == t && i <= place)) {
       const int at = atomicAdd(&sh.n, 1);
-      if (at < kTopMax) sh.cand[at] = ((uint64_t)key << 32) | (uint32_t)~(uint32_t)i;
+      if (at < sh.kMost) sh.cand[at] = ((uint64_t)key << 32) | (uint32_t)~(uint32_t)i;
     }
   }
   __syncthreads();
-  top_emit<T, NT>(sh, k, x, row, k, values, indices);
+  top_emit<T>(sh, k, x, row, k, values, indices);
 }
 
-// Reduces n > k candidates to the k largest.
-template <int NT>
-__device__ __forceinline__ void top_refine(TopShared<NT>& sh, int n, int k) {
+// Reduces n > k candidates to the k largest, or some more that can be ranked:
+// the search for the border ends as soon as that is so (to the last bit, a row of
+// 1000 candidates takes twice as long).
+template <int NT, int KREG>
+__device__ __forceinline__ void top_refine(TopShared<NT, KREG>& sh, int n, int k) {
+  static_assert(sizeof(sh.kept) <= sizeof(sh.hit), "no LDS of its own");
   uint64_t t = 0;
+  const int enough = k + k / 8 + 4;
   for (int bit = 63; bit >= 0; --bit) {
     const uint64_t c = t | (1ull << bit);
     int m = 0;
-    for (int i = threadIdx.x; i < n; i += NT) m += sh.cand[i] >= c;
+    if (NT == kWave) {
+      for (int i0 = 0; i0 < n; i0 += kWave) {
+        const int i = i0 + (int)threadIdx.x;
+        m += (int)__popcll(__ballot(i < n && sh.cand[i < n ? i : 0] >= c));
+      }
+    } else {
+      for (int i = threadIdx.x; i < n; i += NT) m += sh.cand[i] >= c;
 #pragma unroll
-    for (int off = kWave / 2; off > 0; off >>= 1) m += __shfl_xor(m, off, kWave);
-    __syncthreads();
-    if (threadIdx.x % kWave == 0) sh.counts[threadIdx.x / kWave] = m;
-    __syncthreads();
-    m = 0;
-    for (int i = 0; i < NT / kWave; ++i) m += sh.counts[i];
-    if (m >= k) t = c;
+      for (int off = kWave / 2; off > 0; off >>= 1) m += __shfl_xor(m, off, kWave);
+      __syncthreads();
+      if (threadIdx.x % kWave == 0) sh.counts[threadIdx.x / kWave] = m;
+      __syncthreads();
+      m = 0;
+      for (int i = 0; i < NT / kWave; ++i) m += sh.counts[i];
+    }
+    if (m >= k) {  // uniform
+      t = c;
+      if (m <= enough) break;
+    }
   }
   __syncthreads();
   if (threadIdx.x == 0) sh.n = 0;
@@ -191,10 +238,11 @@ __device__ __forceinline__ void top_refine(TopShared<NT>& sh, int n, int k) {
   for (int i = threadIdx.x; i < n; i += NT)
     if (sh.cand[i] >= t) {
       const int at = atomicAdd(&sh.n, 1);
-      if (at < kTopMax) sh.kept[at] = sh.cand[i];  // (places differ, so exactly k reach t)
+      if (at < sh.kKept) sh.kept[at] = sh.cand[i];  // (places differ, so that k or at most `enough` reach t)
     }
   __syncthreads();
-  for (int i = threadIdx.x; i < k; i += NT) sh.cand[i] = sh.kept[i];
+  const int left = sh.n;
+  for (int i = threadIdx.x; i < left; i += NT) sh.cand[i] = sh.kept[i];
   __syncthreads();
 }
 
@@ -223,14 +271,14 @@ __device__ __forceinline__ uint32_t top_bar(const uint32_t (&key)[N], int k) {
 // than k the bar first rises to the k-th largest of their maxima: ranking costs
 // the square of the candidates (k = 128 of 131072 in two pieces, 270 of them:
 // 22 of 105 us).
-template <typename T, int NT, bool LAST, bool MULTI>
-__device__ __forceinline__ bool top_expand(TopShared<NT>& sh, int k) {
-  constexpr int VEC = Vec16<T>::N, kCap = top_cand_cap<NT>();
+template <typename T, bool LAST, bool MULTI, int NT, int KREG>
+__device__ __forceinline__ bool top_expand(TopShared<NT, KREG>& sh, int k) {
+  constexpr int VEC = Vec16<T>::N, kCap = top_cand_cap<NT, KREG>(), kHits = top_hit_cap<NT, KREG>();
   __syncthreads();
   const int hits = sh.n_hit;
-  if (hits > top_hit_cap<NT>()) return false;  // uniform
+  if (hits > kHits) return false;  // uniform
   if (MULTI && hits > k + k / 2) {
-    constexpr int N = (top_hit_cap<NT>() + kWave - 1) / kWave / 2;
+    constexpr int N = (kHits + kWave - 1) / kWave / 2;
     if (hits <= N * kWave && threadIdx.x < kWave) {
       uint32_t key[N];
 #pragma unroll
@@ -262,11 +310,11 @@ __device__ __forceinline__ bool top_expand(TopShared<NT>& sh, int k) {
   const int n = sh.n;
   if (n > kCap) return false;
   // (a single wavefront ranks slowly: it narrows its candidates down sooner)
-  const bool narrow = n > 2 * kTopMax || (NT == kWave && n > 192 && n > k + k / 4);
+  const bool narrow = n > top_rank_cap<NT>() || (NT == kWave && n > 192 && n > k + k / 4);
   if (LAST && !narrow) return true;
   __syncthreads();  // (nobody changes it before everybody has read it)
   if (threadIdx.x == 0) sh.n_hit = 0;
-  if (narrow) top_refine<NT>(sh, n, k);
+  if (narrow) top_refine(sh, n, k);
   __syncthreads();
   return true;
 }
@@ -294,7 +342,7 @@ __global__ __launch_bounds__(NT, NT > 256 ? 8 : 1) void top_logits_kernel(const 
                                                                           float* __restrict__ lse) {
   constexpr int VEC = Vec16<T>::N;
   typedef RawMax<T> Raw;
-  __shared__ TopShared<NT> sh;
+  __shared__ TopShared<NT, KREG> sh;
   const int64_t row = blockIdx.x, V = a.V;
   const T* x = vocab_row<T>(a, row);
   const VocabGeom g = vocab_geom(x, V);
@@ -305,7 +353,7 @@ __global__ __launch_bounds__(NT, NT > 256 ? 8 : 1) void top_logits_kernel(const 
   RowRegs<T, NT, KREG> r;
   regs_load(r, x, V, g);
   if (tid == 0) sh.n = sh.n_hit = 0;
-  for (int i = tid; i < 2 * kTopMax; i += NT) sh.rank[i] = 0;
+  for (int i = tid; i < top_rank_cap<NT>(); i += NT) sh.rank[i] = 0;
   const float c = regs_anchor<false>(r, g, kk);
   float z = 0.f;
   auto add = [&](float xv) { z += fast_exp2(fmaf(xv, kk, c)); };
@@ -322,7 +370,10 @@ __global__ __launch_bounds__(NT, NT > 256 ? 8 : 1) void top_logits_kernel(const 
   for (int j = 0; j < KREG; ++j) {
     if (tid + j * NT < n0) {
       forget(r.v[j]);
-      mx[j * G / KREG] = Raw::max2(mx[j * G / KREG], Raw::of(r.v[j]));
+      if (KREG == 1)
+        __builtin_memcpy(mx, &r.v[j], 16);
+      else
+        mx[j * G / KREG] = Raw::max2(mx[j * G / KREG], Raw::of(r.v[j]));
 #pragma unroll
       for (int i = 0; i < VEC; ++i) add(to_f32(r.v[j].v[i]));
     }
@@ -333,7 +384,7 @@ __global__ __launch_bounds__(NT, NT > 256 ? 8 : 1) void top_logits_kernel(const 
 #pragma unroll
     for (int q = 0; q < G; ++q) {
       uint32_t key = 0u;
-      if (tid + q * (KREG / G) * NT < n0) {  // (a NaN sets no bar)
+      if (tid + (KREG == 1 ? 0 : q * (KREG / G) * NT) < n0) {  // (a NaN sets no bar)
         const float f = Raw::value(mx[q]);
         key = f == f ? top_key(f) : 0u;
       }
@@ -376,7 +427,7 @@ __global__ __launch_bounds__(NT, NT > 256 ? 8 : 1) void top_logits_kernel(const 
   auto take = [&](float xv, int i) {
     if (xv >= bar) {
       const int at = atomicAdd(&sh.n, 1);
-      if (at < top_cand_cap<NT>()) sh.cand[at] = ((uint64_t)top_key(xv) << 32) | (uint32_t)~(uint32_t)i;
+      if (at < top_cand_cap<NT, KREG>()) sh.cand[at] = ((uint64_t)top_key(xv) << 32) | (uint32_t)~(uint32_t)i;
     }
   };
   if (tid < g.head) take(r.h(), tid);
@@ -401,7 +452,7 @@ __global__ __launch_bounds__(NT, NT > 256 ? 8 : 1) void top_logits_kernel(const 
         forget(r.v[j]);
         if (reaches(r.v[j])) {
           const int at = atomicAdd(&sh.n_hit, 1);
-          if (at < top_hit_cap<NT>()) {
+          if (at < top_hit_cap<NT, KREG>()) {
             __builtin_memcpy(&sh.hit[at], &r.v[j], 16);
             sh.hit_at[at] = g.head + ((int)v0 + tid + j * NT) * VEC;
           }
@@ -415,19 +466,19 @@ __global__ __launch_bounds__(NT, NT > 256 ? 8 : 1) void top_logits_kernel(const 
       __builtin_amdgcn_sched_barrier(0);
     }
     if (!MULTI || after == 0) break;
-    if ((v0 / (NT * KREG)) % 2 == 1) fits = top_expand<T, NT, false, MULTI>(sh, k);
+    if ((v0 / (NT * KREG)) % 2 == 1) fits = top_expand<T, false, MULTI>(sh, k);
   }
   const RowSum mine = rowsum_put<NT / kWave, false>(c, z, 0.f, sh.sums);
-  fits = fits && top_expand<T, NT, true, MULTI>(sh, k);
+  fits = fits && top_expand<T, true, MULTI>(sh, k);
   const RowSum s = rowsum_get<NT / kWave, false>(mine, sh.sums);
   if (!s.ok || !fits) {
     __syncthreads();
-    for (int i = tid; i < 2 * kTopMax; i += NT) sh.rank[i] = 0;
-    top_row_walked<T, NT>(a, row, x, k, values, indices, lse, sh);
+    for (int i = tid; i < top_rank_cap<NT>(); i += NT) sh.rank[i] = 0;
+    top_row_walked<T>(a, row, x, k, values, indices, lse, sh);
     return;
   }
   if (tid == 0 && lse) lse[row] = -rowsum_log_prob(a, s, 0.f).hi;  // the log probability of a logit of 0
-  top_emit<T, NT>(sh, sh.n, x, row, k, values, indices);
+  top_emit<T>(sh, sh.n, x, row, k, values, indices);
 }
 
 // ---- distillation from a teacher's largest logits ----------------------------------
@@ -790,8 +841,10 @@ int launch_top_logits(const VocabRows& a, int k, void* values, int32_t* indices,
   const RowShape sh = row_shape<T>(a.V);
   T* out = reinterpret_cast<T*>(values);
   const dim3 grid((unsigned)a.n_rows);
-  if (sh.nt == 64)
+  if (sh.nt == 64 && k <= kTopFew)
     hipLaunchKernelGGL((top_logits_kernel<T, 64, 4, false>), grid, dim3(64), 0, st, a, k, out, indices, lse);
+  else if (sh.nt == 64)
+    hipLaunchKernelGGL((top_logits_kernel<T, 256, 1, false>), grid, dim3(256), 0, st, a, k, out, indices, lse);
   else if (sh.nt == 256 && sh.kreg == 4)
     hipLaunchKernelGGL((top_logits_kernel<T, 256, 4, false>), grid, dim3(256), 0, st, a, k, out, indices, lse);
   else if (sh.nt == 256)
