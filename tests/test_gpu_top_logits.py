@@ -385,3 +385,52 @@ def test_top_logits_fewer_left_than_asked_for(device, V, k, dtype):
     assert (top.indices[:, 0] == V // 2).all() and top.logsumexp.isnan().all()
     x[:, V // 2] = float("inf")
     assert torch.equal(top.indices.cpu().long(), ref64.top(x.float(), k)[1])
+
+
+def test_offsets_beyond_32_bits(device):
+    # 2.36e9 logits, 4.7 GB: the last rows against the same rows in a tensor of their own
+    rows, V, n = 36000, 65536, 6
+    x = torch.zeros(rows, V, dtype=torch.bfloat16, device=device)
+    g = seeded(51)
+    own = (torch.randn(n, V, generator=g) * 3).to(torch.bfloat16).to(device)
+    x[-n:] = own
+    live = torch.arange(rows, device=device) >= rows - n
+    labels = torch.full((rows,), -100, device=device)
+    labels[-n:] = torch.randint(0, V, (n,), generator=g).to(device)
+    for a, b in zip(ta.top_logits(x, 20), ta.top_logits(own, 20)):
+        assert bits_equal(a[-n:].contiguous(), b) and (a[0] == a[7]).all()
+    top = ta.top_logits(own, 20)
+    values, indices = torch.zeros(rows, 20, dtype=torch.bfloat16, device=device), torch.zeros(rows, 20, dtype=torch.int32, device=device)
+    lse = torch.zeros(rows, device=device)
+    values[-n:], indices[-n:], lse[-n:] = top.values, top.indices, top.logsumexp + 0.1
+    ref, adv = torch.full((rows,), -9.0, device=device), torch.ones(rows, device=device)
+
+    def losses(t, m):  # m: the rows' part of the inputs
+        two = t.view(2, -1, V)
+        pair = lambda v: v[m].view(2, -1)  # noqa: E731
+        yield lambda: ta.token_log_probs(t, labels[m]).sum()
+        yield lambda: ta.clipped_policy_loss(two, pair(labels), pair(ref), pair(adv), pair(ref), 0.1)
+        yield lambda: ta.top_logits_distil_loss(t, values[m], indices[m], 2.0, row_mask=live[m], t_logsumexp=lse[m])
+
+    every, last = slice(0, rows), slice(rows - n, rows)
+    big, small = x.requires_grad_(), own.clone().requires_grad_()
+    for f, h in zip(losses(big, every), losses(small, last)):
+        a, b = f(), h()
+        assert bits_equal(a.detach(), b.detach())
+        ga, = torch.autograd.grad(a, big)
+        gb, = torch.autograd.grad(b, small)
+        assert bits_equal(ga[-n:].contiguous(), gb)
+        assert not ga[:rows - n].any()
+        del ga, a
+    # the second answer of a pair lies behind the 32 bits
+    big3, small3 = big.detach().view(2, -1, V).requires_grad_(), torch.zeros(2, n, V, dtype=torch.bfloat16, device=device)
+    small3[1] = own
+    small3.requires_grad_()
+    lab3 = torch.full((2, n), -100, device=device)
+    lab3[1] = labels[-n:]
+    a = ta.preference_loss(big3, labels.view(2, -1), torch.zeros(2, device=device))
+    b = ta.preference_loss(small3, lab3, torch.zeros(2, device=device))
+    assert bits_equal(a.detach(), b.detach())
+    ga, = torch.autograd.grad(a, big3)
+    gb, = torch.autograd.grad(b, small3)
+    assert bits_equal(ga[1, -n:].contiguous(), gb[1]) and gb[1].any() and not ga[0].any() and not ga[1, :-n].any()
