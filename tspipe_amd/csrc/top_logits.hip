@@ -110,7 +110,7 @@ __device__ __forceinline__ void top_emit(TopShared<NT, KREG>& sh, int n, const T
     for (int w = waves; w <= NW; w += waves) ++parts;
     for (; first >= waves; first -= waves) ++part;
   }
-  const int per = (int)(((float)all + (float)parts - 0.5f) / (float)parts);  // all / parts, rounded up
+  const int per = ((int)(((float)all + (float)parts - 0.5f) / (float)parts) + 1) & ~1;  // all / parts, rounded up, even
   const int lo = part * per, hi = part < parts ? (lo + per < all ? lo + per : all) : lo;
   if (NT == 256 && all > NT) {  // uniform; at most twice as many
     const int c0 = (int)threadIdx.x, c1 = c0 + NT;
@@ -131,9 +131,13 @@ __device__ __forceinline__ void top_emit(TopShared<NT, KREG>& sh, int n, const T
   } else {
     for (int c = first * kWave + (int)threadIdx.x % kWave; c < all; c += NT) {
       const uint64_t me = sh.cand[c];
-      int rank = 0;
-#pragma unroll 4
-      for (int i = lo; i < hi; ++i) rank += sh.cand[i] > me;
+      int rank = 0, i = lo;
+#pragma unroll 2
+      for (; i + 1 < hi; i += 2) {
+        const ulonglong2 two = *reinterpret_cast<const ulonglong2*>(&sh.cand[i]);
+        rank += (int)(two.x > me) + (int)(two.y > me);
+      }
+      if (i < hi) rank += (int)(sh.cand[i] > me);
       if (rank) atomicAdd(&sh.rank[c], rank);
     }
   }
@@ -141,9 +145,12 @@ __device__ __forceinline__ void top_emit(TopShared<NT, KREG>& sh, int n, const T
   for (int c = threadIdx.x; c < n; c += NT) {
     const int rank = sh.rank[c];
     if (rank < k) {
-      const int32_t i = (int32_t)~(uint32_t)sh.cand[c];
+      const uint64_t me = sh.cand[c];
+      const int32_t i = (int32_t)~(uint32_t)me;
+      const uint32_t key = (uint32_t)(me >> 32);
       indices[row * k + rank] = i;
-      values[row * k + rank] = x[i];
+      // (the order number is the logit but for a zero's sign and a NaN's bits)
+      values[row * k + rank] = key == 0x80000000u || key == 0xffffffffu ? x[i] : from_f32<T>(top_unkey(key));
     }
   }
 }
