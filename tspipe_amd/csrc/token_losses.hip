@@ -165,10 +165,8 @@ __global__ __launch_bounds__(NT) void token_stat_kernel(const TokenRows a, int64
 
 // One workgroup per part of a row: every element depends on its row's two
 // numbers only, so this is a copy with an exponential, bound by memory (8192 x
-// 32000 bf16 with 70 % of the rows counting: 891 MB in 135 us, 6.6 TB/s).  A
-// gradient that fits the last-level cache is stored into it (2044 x 50257 bf16,
-// 205 MB: 70 us, past it 76; 4096 x 8000 fp32, 131 MB: 40 and 47; 524 MB 167 and
-// 136).  The factor c of a row is coef[row] or, with per_seq, coef[row / seq_len].
+// 32000 bf16 with 70 % of the rows counting: 891 MB in 135 us, 6.6 TB/s).  The
+// factor c of a row is coef[row] or, with per_seq, coef[row / seq_len].
 constexpr int kGradVecs = 8;                           // 16-byte vectors per thread, all loads in flight at once
 constexpr int kGradPart = kTokBlock * kGradVecs;       // vectors per workgroup
 
@@ -231,7 +229,7 @@ __global__ __launch_bounds__(kTokBlock) void token_grad_kernel(const TokenRows a
           if (i == li) o.v[i] = from_f32<T>(f.label(to_f32(x[j].v[i])));
       }
       if (gvec) {
-        vec_store(to, (uint32_t)v, o, a.r.keep_grad);
+        vec_store(to, (uint32_t)v, o);
       } else {
         T* p = grow + e0 + v * VEC;
 #pragma unroll
@@ -477,9 +475,7 @@ __device__ __forceinline__ void policy_row_walked(const TokenRows& a, const Poli
 // between its sum and its gradient and is read once.  Bound by memory: 8192 x
 // 65536 bf16 with 70 % of the rows counting, 1826 MB in 316 us (5.8 TB/s, 281 us
 // at best); two workgroups of 1024 threads a CU, one loading while the other
-// stores.  512 threads with 16 vectors each take 321 us.  (Gradients stored into
-// the last-level cache where they fit make no difference on the whole: 8192 x 4000
-// bf16 30 us, past it 28; 4096 x 8000 fp32 43 and 46; 1024 x 100000 bf16 87 both.)
+// stores.  512 threads with 16 vectors each take 321 us.
 template <typename T, int NT, int KREG>
 __global__ __launch_bounds__(NT) void policy_rows_kernel(const TokenRows a, const PolicyArgs p) {
   __shared__ RowSum lds[NT / kWave];
@@ -506,7 +502,7 @@ __global__ __launch_bounds__(NT) void policy_rows_kernel(const TokenRows a, cons
     if (!grow) return;
     __syncthreads();
     const TokenGrad f(a.r.k, make_float2(s.c, s.z), coef);
-    regs_map(r, g, srow, grow, V, false, (int)label, [&](float x) { return f.other(x); }, [&](float x) { return f.label(x); });
+    regs_map(r, g, srow, grow, V, (int)label, [&](float x) { return f.other(x); }, [&](float x) { return f.label(x); });
     return;
   }
   __syncthreads();
@@ -699,10 +695,9 @@ inline int token_status(const void* s, int64_t n_seq, int64_t seq_len, int64_t V
 }
 
 inline TokenRows token_rows(const void* s, int64_t n_seq, int64_t seq_len, int64_t V, int64_t ld_seq, int64_t ld_tok,
-                            const int64_t* labels, const uint8_t* mask, int64_t ignore_index, double temperature,
-                            int dtype) {
+                            const int64_t* labels, const uint8_t* mask, int64_t ignore_index, double temperature) {
   TokenRows a;
-  a.r = vocab_rows(s, n_seq * seq_len, seq_len, V, ld_seq, ld_tok, temperature, dtype == TS_F32 ? 4 : 2);
+  a.r = vocab_rows(s, n_seq * seq_len, seq_len, V, ld_seq, ld_tok, temperature);
   a.labels = labels;
   a.mask = mask;
   a.ignore_index = ignore_index;
@@ -722,7 +717,7 @@ int ts_token_logp_fwd(const void* s, int64_t n_seq, int64_t seq_len, int64_t V, 
   if (!logp) return TS_ERR_ARG;
   if (((uintptr_t)logp & 3u) || ((uintptr_t)stats & 7u)) return TS_ERR_ALIGN;
   const ts::TokenRows a =
-      ts::token_rows(s, n_seq, seq_len, V, ld_seq, ld_tok, labels, row_mask, ignore_index, temperature, dtype);
+      ts::token_rows(s, n_seq, seq_len, V, ld_seq, ld_tok, labels, row_mask, ignore_index, temperature);
   hipStream_t st = (hipStream_t)stream;
   TS_BY_DTYPE(dtype, (ts::launch_token_stat<T>(a, 0, a.r.n_rows, nullptr, logp, nullptr, (float2*)stats, nullptr, st)))
 }
@@ -736,7 +731,7 @@ int ts_token_logp_bwd(const void* s, int64_t n_seq, int64_t seq_len, int64_t V, 
   if (!stats || !grad_logp || !grad) return TS_ERR_ARG;
   if (((uintptr_t)grad_logp & 3u) || ((uintptr_t)stats & 7u)) return TS_ERR_ALIGN;
   const ts::TokenRows a =
-      ts::token_rows(s, n_seq, seq_len, V, ld_seq, ld_tok, labels, row_mask, ignore_index, temperature, dtype);
+      ts::token_rows(s, n_seq, seq_len, V, ld_seq, ld_tok, labels, row_mask, ignore_index, temperature);
   hipStream_t st = (hipStream_t)stream;
   TS_BY_DTYPE(dtype, (ts::launch_token_grad<T>(a, 0, a.r.n_rows, (const float2*)stats, grad_logp, 0, grad, st)))
 }
@@ -760,7 +755,7 @@ int ts_preference_fwd_bwd(const void* s, int64_t n_seq, int64_t seq_len, int64_t
   if (n_seq * (ref_per_token ? seq_len : 1) > 0 && !ref_logp) return TS_ERR_ARG;
   if (((uintptr_t)workspace & 15u) || (((uintptr_t)ref_logp | (uintptr_t)loss_out | (uintptr_t)rewards) & 3u))
     return TS_ERR_ALIGN;
-  const ts::TokenRows a = ts::token_rows(s, n_seq, seq_len, V, ld_seq, ld_tok, labels, row_mask, ignore_index, 1.0, dtype);
+  const ts::TokenRows a = ts::token_rows(s, n_seq, seq_len, V, ld_seq, ld_tok, labels, row_mask, ignore_index, 1.0);
   const ts::TokenWs w = ts::token_carve(workspace, a.r.n_rows, n_seq);
   ts::PrefArgs p;
   p.log_ratio = w.row;
@@ -793,7 +788,7 @@ int ts_policy_fwd_bwd(const void* s, int64_t n_seq, int64_t seq_len, int64_t V, 
                                         (uintptr_t)loss_out | (uintptr_t)logp) & 3u))
     return TS_ERR_ALIGN;
   const ts::TokenRows a =
-      ts::token_rows(s, n_seq, seq_len, V, ld_seq, ld_tok, labels, row_mask, ignore_index, temperature, dtype);
+      ts::token_rows(s, n_seq, seq_len, V, ld_seq, ld_tok, labels, row_mask, ignore_index, temperature);
   const ts::TokenWs w = ts::token_carve(workspace, a.r.n_rows, n_seq);
   ts::PolicyArgs p;
   p.old_logp = old_logp;

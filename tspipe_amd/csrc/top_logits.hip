@@ -652,10 +652,7 @@ __device__ __forceinline__ uint32_t top_mark_bit(int j, const VocabGeom& g) { re
 //
 // 64 registers a thread for up to eight vectors of a row, but for the 512-thread
 // arrangement, which would spill there: with six wavefronts a SIMD instead of
-// eight 4096 x 30522 bf16 takes 88 us instead of 99.  A gradient that fits the
-// last-level cache is stored into it, where the kept entries' lines are completed
-// (4096 x 30522 bf16, 85 % of the rows: 87 us, past it 92; 4096 x 8000 fp32 47 and
-// 51), but from 1024 threads (1024 x 50257 bf16: 54 and 51).
+// eight 4096 x 30522 bf16 takes 88 us instead of 99.
 template <typename T, int NT, int KREG, bool LONG, bool TAIL>
 __global__ __launch_bounds__(NT, (KREG > 8 || LONG ? 4 : NT > 256 ? (NT > 512 ? 8 : 6) : 1)) void top_distil_kernel(
     const TopDistilArgs a) {
@@ -791,7 +788,7 @@ __global__ __launch_bounds__(NT, (KREG > 8 || LONG ? 4 : NT > 256 ? (NT > 512 ? 
       if (LONG)
         long_map(r, g, x, grow, V, -1, other, none);
       else
-        regs_map(r, g, x, grow, V, NT <= 512 && a.r.keep_grad, -1, other, none);
+        regs_map(r, g, x, grow, V, -1, other, none);
       patch([&](float xv) { return fast_exp2(fmaf(xv, kk, c)) * rz; });
     }
     loss([&](float xv) { return rowsum_log_prob(a.r, s, xv); }, [&]() { return ln_share(log2_2x(rest_z), s.z); });
@@ -948,7 +945,7 @@ int ts_top_distil_fwd_bwd(const void* s, int64_t n_seq, int64_t seq_len, int64_t
       (((uintptr_t)t_indices | (uintptr_t)t_logsumexp | (uintptr_t)loss_out) & 3u) || ((uintptr_t)workspace & 15u))
     return TS_ERR_ALIGN;
   ts::TopDistilArgs a;
-  a.r = ts::vocab_rows(s, n_seq * seq_len, seq_len, V, ld_seq, ld_tok, temperature, dtype == TS_F32 ? 4 : 2);
+  a.r = ts::vocab_rows(s, n_seq * seq_len, seq_len, V, ld_seq, ld_tok, temperature);
   a.t_values = t_values;
   a.t_dtype = t_dtype;
   a.t_indices = t_indices;

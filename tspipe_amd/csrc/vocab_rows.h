@@ -23,15 +23,11 @@ struct VocabRows {
   // log-sum-exp is corrected for it to first order.
   float k, k_rel;
   double inv_T;
-  // The gradient is smaller than the last-level cache (256 MB) and may be stored into it, for whoever reads it
-  // next; a larger one would only push the logits out of it.
-  bool keep_grad;
 };
 
 inline VocabRows vocab_rows(const void* s, int64_t n_rows, int64_t seq_len, int64_t V, int64_t ld_seq, int64_t ld_tok,
-                            double temperature, size_t grad_element = 0) {
+                            double temperature) {
   VocabRows a;
-  a.keep_grad = (uint64_t)n_rows * (uint64_t)V * grad_element < 256ull << 20;
   a.s = s;
   a.n_rows = n_rows;
   a.seq_len = seq_len;
@@ -310,15 +306,11 @@ __device__ __forceinline__ Vec16<T> vec_load(const VecBuffer& b, uint32_t v) {
   __builtin_memcpy(&r, &raw, 16);
   return r;
 }
-// `keep` is the same in every lane.
 template <typename T>
-__device__ __forceinline__ void vec_store(const VecBuffer& b, uint32_t v, const Vec16<T>& x, bool keep) {
+__device__ __forceinline__ void vec_store(const VecBuffer& b, uint32_t v, const Vec16<T>& x) {
   u32x4 raw;
   __builtin_memcpy(&raw, &x, 16);
-  if (keep)
-    __builtin_amdgcn_raw_buffer_store_b128(raw, b.rsrc, (int)(v * 16u), 0, 0);
-  else
-    __builtin_amdgcn_raw_buffer_store_b128(raw, b.rsrc, (int)(v * 16u), 0, kNonTemporal);
+  __builtin_amdgcn_raw_buffer_store_b128(raw, b.rsrc, (int)(v * 16u), 0, kNonTemporal);
 }
 
 // Element i of `count` (0 beyond them), as fp32.
@@ -544,10 +536,10 @@ __device__ __forceinline__ RowSum regs_sum(RowRegs<T, NT, KREG>& r, const VocabG
 }
 
 // grow[j] = f(x[j]) from registers, but for element `special` (or -1), which
-// gets f_special(x).  keep: the stores leave the gradient in the last-level cache.
+// gets f_special(x).
 template <typename T, int NT, int KREG, typename F, typename G>
 __device__ __forceinline__ void regs_map(RowRegs<T, NT, KREG>& r, const VocabGeom& g, const T* row, T* grow, int64_t V,
-                                         bool keep, int special, F f, G f_special) {
+                                         int special, F f, G f_special) {
   constexpr int VEC = Vec16<T>::N;
   if ((int)threadIdx.x < g.head)
     grow[threadIdx.x] = from_f32<T>((int)threadIdx.x == special ? f_special(r.h()) : f(r.h()));
@@ -571,7 +563,7 @@ __device__ __forceinline__ void regs_map(RowRegs<T, NT, KREG>& r, const VocabGeo
           if (i == si) o.v[i] = from_f32<T>(f_special(to_f32(r.v[j].v[i])));
       }
       if (gvec) {
-        vec_store(body, (uint32_t)v, o, keep);
+        vec_store(body, (uint32_t)v, o);
       } else {
         T* p = grow + g.head + v * VEC;
 #pragma unroll
