@@ -434,3 +434,42 @@ def test_offsets_beyond_32_bits(device):
     ga, = torch.autograd.grad(a, big3)
     gb, = torch.autograd.grad(b, small3)
     assert bits_equal(ga[1, -n:].contiguous(), gb[1]) and gb[1].any() and not ga[0].any() and not ga[1, :-n].any()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("tail", [False, True])
+@pytest.mark.parametrize("V,k", [(150001, 40), (150001, 256), (262144, 8)])
+def test_distil_rows_too_long_for_registers(device, V, k, tail, dtype):
+    # masked rows, absent and repeated entries, rows of the type's lowest value (uniform) and of -inf but for a few
+    # tokens, rows that start at odd addresses and lie apart, no gradient wanted
+    g = seeded(61 + V + k)
+    n, L, T = 2, 4, 1.5
+    vals, idx, lse = teacher(n * L, V, k, g, dtype, T)
+    lse = lse + 0.7
+    x = (torch.randn(n * L, V, generator=g) * 2).to(dtype)
+    x.scatter_add_(1, idx.long(), (vals.float() * 0.6).to(dtype))
+    idx[0, 1], idx[0, 2], idx[1, 3] = -1, V, idx[1, 0]
+    x[3] = torch.finfo(dtype).min
+    x[4] = float("-inf")
+    x[4, -2:] = 1.0
+    idx[4] = -1
+    idx[4, 0], idx[4, 1] = V - 1, V - 2
+    mask = torch.tensor([1, 1, 0, 1, 1, 0, 1, 1]).bool()
+    lse = lse if tail else None
+    if tail:  # (what the teacher leaves to others, the student of row 4 cannot reach)
+        lse[4] = torch.logsumexp(vals[4, :2].double() / T, -1).float() - 1e-3
+    loss, grad = run_case(device, x, vals, idx, T, 64.0 * n * L, mask, lse)
+    assert (grad[~mask.to(device)] == 0).all()
+    wide = torch.full((n, L + 1, V + 3), float("nan"), dtype=dtype, device=device)
+    view = wide[:, 1:, 1:V + 1]
+    view.copy_(x.view(n, L, V))
+    leaf = view.detach().requires_grad_()
+    three = lambda t: None if t is None else t.to(device).view(n, L, *t.shape[1:])  # noqa: E731
+    again = ta.top_logits_distil_loss(leaf, three(vals), three(idx), T, 64.0 * n * L, three(mask), three(lse))
+    again.backward()
+    assert abs(again.item() - loss.item()) <= 64.0 * n * L * T * T * 4 * LOGP_ABS + 2.0 ** -22 * abs(loss.item())
+    want = grad.view(n, L, V).double()
+    # (a row that starts elsewhere is summed in another order: each of the two within its own bound)
+    check_grad(leaf.grad, want.cpu(), dtype, coef=64.0 * T * n * L / 6 * 2 + 2 ** 22 * torch.finfo(dtype).eps / 2 * want.abs().cpu())
+    with torch.no_grad():
+        assert bits_equal(ta.top_logits_distil_loss(leaf, three(vals), three(idx), T, 64.0 * n * L, three(mask), three(lse)), again.detach())

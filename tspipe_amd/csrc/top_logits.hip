@@ -340,8 +340,8 @@ __device__ __forceinline__ bool top_expand(TopShared<NT, KREG>& sh, int k) {
 // when the noted vectors are spread over all threads.
 //
 // MULTI: the row has more than one piece.  Eight wavefronts a SIMD: 64 registers
-// are enough, and with 80 and six of them 4096 x 30522 bf16 takes 67 us instead
-// of 58, 1024 x 131072 96 instead of 79.
+// are enough, and with 80 and six of them 4096 x 30522 bf16 took 67 us instead
+// of 58 (55 by now), 1024 x 131072 96 instead of 79.
 template <typename T, int NT, int KREG, bool MULTI>
 __global__ __launch_bounds__(NT, NT > 256 ? 8 : 1) void top_logits_kernel(const VocabRows a, int k,
                                                                           T* __restrict__ values,
@@ -510,7 +510,18 @@ struct TopDistilArgs {
   TopTeacher* teacher;  // per row
   float* entry_p;       // per entry: the probability of all the row's entries for its token; -1 if absent or not the first of them
   double* row_loss;
+  struct TopRowGrad* row_grad;  // per row, for rows too long for registers
   void* grad;  // may be null
+};
+
+// The gradient of a row's tokens without an entry: go 2^(x k + off), or go
+// 2^((x - off) k) for walked rows; with rz for go a token's probability.
+struct TopRowGrad {
+  float off, go, rz;
+  int by_max;
+  __device__ __forceinline__ float power(float x, float k) const {
+    return fast_exp2(by_max ? (x - off) * k : fmaf(x, k, off));
+  }
 };
 
 __device__ __forceinline__ float top_value(const void* v, int dtype, int64_t i) {
@@ -648,11 +659,13 @@ struct TopDistilShared {
 // that a vector's marks are one byte (or half of one).
 __device__ __forceinline__ uint32_t top_mark_bit(int j, const VocabGeom& g) { return (uint32_t)(j - g.head + 8); }
 
-// LONG rows do not fit the registers and are read twice.
+// LONG rows do not fit the registers: this kernel then reads them in pieces and
+// leaves the gradient to two others.
 //
 // 64 registers a thread for up to eight vectors of a row, but for the 512-thread
 // arrangement, which would spill there: with six wavefronts a SIMD instead of
-// eight 4096 x 30522 bf16 takes 88 us instead of 99.
+// eight 4096 x 30522 bf16 with 85 % of the rows takes 92 us (505 MB, 5.5 TB/s)
+// instead of 99.
 template <typename T, int NT, int KREG, bool LONG, bool TAIL>
 __global__ __launch_bounds__(NT, (KREG > 8 || LONG ? 4 : NT > 256 ? (NT > 512 ? 8 : 6) : 1)) void top_distil_kernel(
     const TopDistilArgs a) {
@@ -664,7 +677,7 @@ __global__ __launch_bounds__(NT, (KREG > 8 || LONG ? 4 : NT > 256 ? (NT > 512 ? 
   T* grow = a.grad ? reinterpret_cast<T*>(a.grad) + row * V : nullptr;
   if (a.mask && a.mask[row] == 0) {
     if (tid == 0) a.row_loss[row] = 0.0;
-    if (grow) vocab_zero_row<T, NT>(grow, V);
+    if (grow && !LONG) vocab_zero_row<T, NT>(grow, V);
     return;
   }
   const T* x = vocab_row<T>(a.r, row);
@@ -731,6 +744,9 @@ __global__ __launch_bounds__(NT, (KREG > 8 || LONG ? 4 : NT > 256 ? (NT > 512 ? 
       a.row_loss[row] = term;
     }
   };
+  auto leave = [&](float off, float go, float rz, int by_max) {  // LONG
+    if (tid == 0) a.row_grad[row] = TopRowGrad{off, go, rz, by_max};
+  };
   auto patch = [&](auto q_of) {  // the kept entries' gradients replace what the walk over the row wrote
     __syncthreads();
 #pragma unroll
@@ -785,11 +801,12 @@ __global__ __launch_bounds__(NT, (KREG > 8 || LONG ? 4 : NT > 256 ? (NT > 512 ? 
       const float rz = 1.f / s.z, go = outside(s.z / rest_z) * rz, c = s.c;
       auto other = [=](float xv) { return go * fast_exp2(fmaf(xv, kk, c)); };
       auto none = [](float) { return 0.f; };
-      if (LONG)
-        long_map(r, g, x, grow, V, -1, other, none);
-      else
+      if (LONG) {
+        leave(c, go, rz, 0);
+      } else {
         regs_map(r, g, x, grow, V, -1, other, none);
-      patch([&](float xv) { return fast_exp2(fmaf(xv, kk, c)) * rz; });
+        patch([&](float xv) { return fast_exp2(fmaf(xv, kk, c)) * rz; });
+      }
     }
     loss([&](float xv) { return rowsum_log_prob(a.r, s, xv); }, [&]() { return ln_share(log2_2x(rest_z), s.z); });
     return;
@@ -829,10 +846,94 @@ __global__ __launch_bounds__(NT, (KREG > 8 || LONG ? 4 : NT > 256 ? (NT > 512 ? 
   }
   if (grow) {
     const float rz = 1.f / all.z, go = outside(inv_q_rest) * rz, m = all.m;
-    vocab_map_walk<T, NT>(x, grow, V, [=](float xv, int) { return go * fast_exp2((xv - m) * kk); });
-    patch([&](float xv) { return fast_exp2((xv - m) * kk) * rz; });
+    if (LONG) {
+      leave(m, go, rz, 1);
+    } else {
+      vocab_map_walk<T, NT>(x, grow, V, [=](float xv, int) { return go * fast_exp2((xv - m) * kk); });
+      patch([&](float xv) { return fast_exp2((xv - m) * kk) * rz; });
+    }
   }
   loss([&](float xv) { return vstat_log_prob(a.r, all, xv); }, [&]() { return lq_rest; });
+}
+
+// The gradient of rows too long for registers, a workgroup per part of a row (one
+// workgroup that reads its row a second time: 1900 x 140000 bf16 341 us a call
+// instead of 303, fp32 606 instead of 566).
+constexpr int kMapBlock = 256, kMapVecs = 8, kMapPart = kMapBlock * kMapVecs;
+
+template <typename T>
+__global__ __launch_bounds__(kMapBlock) void top_map_kernel(const TopDistilArgs a, int64_t row0, int parts) {
+  constexpr int VEC = Vec16<T>::N;
+  const int64_t local = blockIdx.x / (unsigned)parts, row = row0 + local;
+  const int part = (int)(blockIdx.x - (unsigned)local * (unsigned)parts), tid = threadIdx.x;
+  const int64_t V = a.r.V, v0 = (int64_t)part * kMapPart;
+  T* grow = reinterpret_cast<T*>(a.grad) + row * V;
+  if (a.mask && a.mask[row] == 0) {
+    const VocabGeom g = vocab_geom(grow, V);
+    const T zero = from_f32<T>(0.f);
+    if (part == 0 && tid < g.head) grow[tid] = zero;
+    if (part == parts - 1 && g.tail0 + tid < V) grow[g.tail0 + tid] = zero;
+    Vec16<T> z;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) z.v[i] = zero;
+#pragma unroll
+    for (int j = 0; j < kMapVecs; ++j) {
+      const int64_t v = v0 + tid + j * kMapBlock;
+      if (v < g.nvec) store16(grow + g.head + v * VEC, z);
+    }
+    return;
+  }
+  const T* x = vocab_row<T>(a.r, row);
+  const VocabGeom g = vocab_geom(x, V);
+  RowRegs<T, kMapBlock, kMapVecs> r;
+  const int64_t e0 = g.head + v0 * VEC, some = g.nvec - v0;  // this part's first element and vectors
+  const int left = some < kMapPart ? (int)some : kMapPart;
+  const VecBuffer from = vec_buffer(x + e0, left);
+#pragma unroll
+  for (int j = 0; j < kMapVecs; ++j) r.v[j] = vec_load<T>(from, tid + j * kMapBlock);
+  const TopRowGrad f = scalar_load(a.row_grad + row);
+  const float k = a.r.k;
+  auto other = [&](float xv) { return f.go * f.power(xv, k); };
+  if (part == 0 && tid < g.head) grow[tid] = from_f32<T>(other(to_f32(x[tid])));
+  if (part == parts - 1 && g.tail0 + tid < V) grow[g.tail0 + tid] = from_f32<T>(other(to_f32(x[g.tail0 + tid])));
+  const bool gvec = (((uintptr_t)grow ^ (uintptr_t)x) & 15u) == 0;
+  const VecBuffer to = vec_buffer(grow + e0, gvec ? left : 0);
+#pragma unroll
+  for (int j = 0; j < kMapVecs; ++j) {
+    const int v = tid + j * kMapBlock;
+    if (v < left) {
+      forget(r.v[j]);
+      Vec16<T> o;
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) o.v[i] = from_f32<T>(other(to_f32(r.v[j].v[i])));
+      if (gvec) {
+        vec_store(to, (uint32_t)v, o);
+      } else {
+        T* q = grow + e0 + (int64_t)v * VEC;
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) q[i] = o.v[i];
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  }
+}
+
+// The kept entries' gradients replace what top_map_kernel wrote; one thread an entry.
+template <typename T>
+__global__ __launch_bounds__(kMapBlock) void top_entries_kernel(const TopDistilArgs a) {
+  const int64_t e = (int64_t)blockIdx.x * kMapBlock + threadIdx.x;
+  if (e >= a.r.n_rows * a.k) return;
+  const int64_t row = e / a.k;
+  if (a.mask && a.mask[row] == 0) return;
+  const float p = a.entry_p[e];
+  if (p < 0.f) return;  // absent
+  const int idx = a.t_indices[e];
+  const int64_t q = row / a.r.seq_len;
+  const T* x = reinterpret_cast<const T*>(a.r.s) + q * a.r.ld_seq + (row - q * a.r.seq_len) * a.r.ld_tok;
+  const TopRowGrad f = a.row_grad[row];
+  const float gs = a.gscale / (float)*a.live;
+  reinterpret_cast<T*>(a.grad)[row * a.r.V + idx] =
+      from_f32<T>(gs * fmaf(f.power(to_f32(x[idx]), a.r.k) * f.rz, a.teacher[row].whole, -p));
 }
 
 __global__ __launch_bounds__(1024) void top_distil_sum_kernel(const double* __restrict__ v, int64_t n,
@@ -887,7 +988,22 @@ int launch_top_distil_shape(const TopDistilArgs& a, hipStream_t st) {
   if (sh.nt == 512) return launch_top_distil_rows<T, 512, 8, false, TAIL>(a, st);
   if (sh.kreg == 8) return launch_top_distil_rows<T, 1024, 8, false, TAIL>(a, st);
   if (sh.kreg == 16) return launch_top_distil_rows<T, 1024, 16, false, TAIL>(a, st);
-  return launch_top_distil_rows<T, 512, 8, true, TAIL>(a, st);
+  int rc = launch_top_distil_rows<T, 512, 8, true, TAIL>(a, st);
+  if (rc || !a.grad) return rc;
+  const int64_t vecs = a.r.V / Vec16<T>::N, parts = (vecs + kMapPart - 1) / kMapPart;
+  for (int64_t row0 = 0; row0 < a.r.n_rows;) {  // (the grid counts threads in 32 bits)
+    int64_t n = a.r.n_rows - row0;
+    if (n * parts > (1 << 23)) n = (1 << 23) / parts;
+    if (n < 1) return TS_ERR_RANGE;
+    hipLaunchKernelGGL((top_map_kernel<T>), dim3((unsigned)(n * parts)), dim3(kMapBlock), 0, st, a, row0, (int)parts);
+    rc = check_launch();
+    if (rc) return rc;
+    row0 += n;
+  }
+  const int64_t entries = a.r.n_rows * a.k;
+  hipLaunchKernelGGL((top_entries_kernel<T>), dim3((unsigned)((entries + kMapBlock - 1) / kMapBlock)), dim3(kMapBlock), 0,
+                     st, a);
+  return check_launch();
 }
 
 template <typename T>
@@ -904,8 +1020,8 @@ int launch_top_distil(const TopDistilArgs& a, double loss_scale, float* loss_out
   return check_launch();
 }
 
-// Workspace: live count (16 bytes), loss terms and teacher numbers per row, probabilities per entry.
-inline size_t top_ws_bytes(int64_t n_rows, int64_t k) { return 16 + (size_t)n_rows * (8 + 16) + (size_t)(n_rows * k) * 4; }
+// Workspace: live count (16 bytes), teacher and gradient numbers and loss terms per row, probabilities per entry.
+inline size_t top_ws_bytes(int64_t n_rows, int64_t k) { return 16 + (size_t)n_rows * (16 + 16 + 8) + (size_t)(n_rows * k) * 4; }
 
 }  // namespace ts
 
@@ -956,8 +1072,9 @@ int ts_top_distil_fwd_bwd(const void* s, int64_t n_seq, int64_t seq_len, int64_t
   char* ws = reinterpret_cast<char*>(workspace);
   a.live = reinterpret_cast<int*>(ws);
   a.teacher = reinterpret_cast<ts::TopTeacher*>(ws + 16);
-  a.row_loss = reinterpret_cast<double*>(ws + 16 + a.r.n_rows * 16);
-  a.entry_p = reinterpret_cast<float*>(ws + 16 + a.r.n_rows * 24);
+  a.row_grad = reinterpret_cast<ts::TopRowGrad*>(ws + 16 + a.r.n_rows * 16);
+  a.row_loss = reinterpret_cast<double*>(ws + 16 + a.r.n_rows * 32);
+  a.entry_p = reinterpret_cast<float*>(ws + 16 + a.r.n_rows * 40);
   a.grad = grad;
   hipStream_t st = (hipStream_t)stream;
   TS_BY_DTYPE(dtype, (ts::launch_top_distil<T>(a, weight * temperature * temperature, loss_out, st)))

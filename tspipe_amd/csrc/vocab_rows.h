@@ -620,7 +620,7 @@ __device__ __forceinline__ void long_each(RowRegs<T, NT, KREG>& r, const T* row,
   }
 }
 
-// regs_sum and regs_map of such rows.
+// regs_sum of such rows.
 template <typename T, int NT, int KREG>
 __device__ __forceinline__ RowSum long_sum(RowRegs<T, NT, KREG>& r, const T* row, const VocabGeom& g, float k, RowSum* lds) {
   constexpr int VEC = Vec16<T>::N;
@@ -638,37 +638,6 @@ __device__ __forceinline__ RowSum long_sum(RowRegs<T, NT, KREG>& r, const T* row
       },
       [&](int left) { z = __builtin_amdgcn_ldexpf(z, (int)regs_raise(r, left, k, c)); });
   return rowsum_block<NT / kWave, false>(c, z, 0.f, lds);
-}
-
-template <typename T, int NT, int KREG, typename F, typename G>
-__device__ __forceinline__ void long_map(RowRegs<T, NT, KREG>& r, const VocabGeom& g, const T* row, T* grow, int64_t V,
-                                         int special, F f, G f_special) {
-  constexpr int VEC = Vec16<T>::N;
-  regs_load(r, row, V, g);  // the second reading
-  if ((int)threadIdx.x < g.head)
-    grow[threadIdx.x] = from_f32<T>((int)threadIdx.x == special ? f_special(r.h()) : f(r.h()));
-  const int64_t t = g.tail0 + threadIdx.x;
-  if (t < V) grow[t] = from_f32<T>((int)t == special ? f_special(r.t()) : f(r.t()));
-  const bool gvec = (((uintptr_t)grow ^ (uintptr_t)row) & 15u) == 0;
-  const int64_t sv = special >= g.head ? (special - g.head) / VEC : -1;
-  const int si = special - g.head - (int)sv * VEC;
-  long_each(r, row, g, [&](const Vec16<T>& x, int64_t v) {
-    Vec16<T> o;
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) o.v[i] = from_f32<T>(f(to_f32(x.v[i])));
-    if (v == sv) {
-#pragma unroll
-      for (int i = 0; i < VEC; ++i)
-        if (i == si) o.v[i] = from_f32<T>(f_special(to_f32(x.v[i])));
-    }
-    T* p = grow + g.head + v * VEC;
-    if (gvec) {
-      store16_stream(p, o);
-    } else {
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) p[i] = o.v[i];
-    }
-  }, [](int) {});
 }
 
 // This thread's share of sum(v[0..n)) when NT threads walk the array together, in
