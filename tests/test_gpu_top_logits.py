@@ -473,3 +473,24 @@ def test_distil_rows_too_long_for_registers(device, V, k, tail, dtype):
     check_grad(leaf.grad, want.cpu(), dtype, coef=64.0 * T * n * L / 6 * 2 + 2 ** 22 * torch.finfo(dtype).eps / 2 * want.abs().cpu())
     with torch.no_grad():
         assert bits_equal(ta.top_logits_distil_loss(leaf, three(vals), three(idx), T, 64.0 * n * L, three(mask), three(lse)), again.detach())
+
+
+@pytest.mark.parametrize("tail", [False, True])
+@pytest.mark.parametrize("k", [64, 65, 130, 256])
+def test_distil_tokens_named_again_and_again(device, k, tail):
+    # one token twice, far apart and next to each other; every token twice; one token throughout; none twice;
+    # tokens 512 apart and neighbours
+    g = seeded(71 + k)
+    rows, V, T = 7, 140001, 2.0
+    idx = torch.stack([torch.randperm(V, generator=g)[:k] for _ in range(rows)]).to(torch.int32)
+    idx[0, k - 1] = idx[0, 0]
+    idx[1, 1] = idx[1, 0]
+    idx[2, 1::2] = idx[2, :k - 1:2] if k % 2 else idx[2, ::2]
+    idx[3] = 77
+    idx[5] = torch.arange(k) * 512 % V
+    idx[6] = torch.arange(V - k, V)
+    idx[6, 2] = -1
+    vals = torch.randn(rows, k, generator=g).sort(-1, descending=True).values
+    lse = torch.logsumexp(vals.double() / T, -1).float() + 0.5
+    x = torch.randn(rows, V, generator=g) * 2
+    run_case(device, x, vals, idx, T, 64.0 * rows, None, lse if tail else None)
