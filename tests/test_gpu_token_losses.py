@@ -824,3 +824,27 @@ def test_capture_while_an_eager_graph_holds_the_leaf(device, monkeypatch):
         graph.replay()
         torch.cuda.synchronize()
         assert bits_equal(got, want)
+
+
+@pytest.mark.parametrize("per_token", [True, False])
+@pytest.mark.parametrize("pairs,L", [(3000, 1), (1025, 2), (257, 70), (5, 512), (3, 513), (300, 600)])
+def test_preference_many_pairs(device, pairs, L, per_token):
+    x, labels, g = make((2 * pairs, L, 7), torch.float32, 200 + pairs + L)
+    labels[torch.rand(2 * pairs, L, generator=g) < 0.3] = -100
+    labels[1] = -100
+    lp, _ = ref64.log_probs(x.double(), labels)
+    ref = ((lp if per_token else lp.sum(-1)) + torch.randn(lp.shape if per_token else (2 * pairs,), generator=g) * 0.1).float()
+    for average in ((False, True) if per_token else (False,)):
+        x64 = x.double().requires_grad_()
+        want, wr = ref64.preference(x64, labels, ref.double(), 0.3, average=average, weight=2.0 * pairs)
+        want.backward()
+        xd = x.to(device).requires_grad_()
+        loss, rewards = ta.preference_loss(xd, labels.to(device), ref.to(device), 0.3, length_average=average,
+                                           weight=2.0 * pairs, return_rewards=True)
+        loss.backward()
+        # a sequence's sum is off by LOGP_ABS a token, and 2 sequences by 0.3 of that in a pair's loss, whose slope is below 1
+        off = 2 * L * LOGP_ABS * 0.3
+        assert abs(loss.item() - want.item()) <= 2 * pairs * off + 2.0 ** -23 * want.item()
+        assert ((rewards.cpu().double() - wr).abs() <= off + 2.0 ** -23 * wr.abs()).all()
+        # the factor of a row: 0.3 at most times the pair's weight, 2; off by what the slope's argument is
+        check_grad(xd.grad, x64.grad, torch.float32, coef=0.6 * (1 + off * 2 ** 22))

@@ -258,28 +258,37 @@ struct PrefArgs {
 
 __device__ __forceinline__ double softplus_f64(double x) { return fmax(x, 0.0) + log1p(exp(-fabs(x))); }
 
-// One workgroup per pair: both sequences' sums, the pair's loss and the factors
-// c of its two sequences; the last one takes the mean of all pairs' losses.
+// TEAM threads per pair, a wavefront for short sequences: both sequences' sums,
+// the pair's loss and the factors c of its two sequences; the last workgroup takes
+// the mean of all pairs' losses.  A bounded number of workgroups, because each one
+// draws a ticket (2048 pairs of 2 tokens, a workgroup each: 28 us instead of 10).
+constexpr int kPrefGrid = 256;
+constexpr int64_t kPrefShort = 64;  // tokens (8 pairs of 512, a wavefront each: 11 us instead of 6.5)
+
+template <int TEAM>
 __global__ __launch_bounds__(kTokBlock) void pref_join_kernel(const TokenRows a, const PrefArgs p, int64_t pairs) {
+  constexpr int NW = TEAM / kWave, TEAMS = kTokBlock / TEAM;
   __shared__ double lds[kTokBlock / kWave];
   __shared__ bool last;
-  const int64_t pair = blockIdx.x, L = a.r.seq_len;
-  double R[2], n[2];
-  for (int side = 0; side < 2; ++side) {
-    const int64_t row0 = (2 * pair + side) * L;
-    double s = 0.0, c = 0.0;
-    for (int64_t i = threadIdx.x; i < L; i += kTokBlock) {
-      s += p.log_ratio[row0 + i];
-      if (p.average) {
-        int64_t label;
-        c += token_live<false>(a, row0 + i, &label) ? 1.0 : 0.0;
+  const int lane = threadIdx.x % TEAM;
+  const int64_t L = a.r.seq_len;
+  for (int64_t pair = (int64_t)blockIdx.x * TEAMS + threadIdx.x / TEAM; pair < pairs; pair += (int64_t)gridDim.x * TEAMS) {
+    double R[2], n[2];
+    for (int side = 0; side < 2; ++side) {
+      const int64_t row0 = (2 * pair + side) * L;
+      double s = 0.0, c = 0.0;
+      for (int64_t i = lane; i < L; i += TEAM) {
+        s += p.log_ratio[row0 + i];
+        if (p.average) {
+          int64_t label;
+          c += token_live<false>(a, row0 + i, &label) ? 1.0 : 0.0;
+        }
       }
+      R[side] = block_sum_f64<NW>(s, lds);
+      n[side] = p.average ? fmax(block_sum_f64<NW>(c, lds), 1.0) : 1.0;
+      R[side] = R[side] / n[side] - (p.ref_seq ? (double)p.ref_seq[2 * pair + side] : 0.0);
     }
-    R[side] = block_sum_f64<kTokBlock / kWave>(s, lds);
-    n[side] = p.average ? fmax(block_sum_f64<kTokBlock / kWave>(c, lds), 1.0) : 1.0;
-    R[side] = R[side] / n[side] - (p.ref_seq ? (double)p.ref_seq[2 * pair + side] : 0.0);
-  }
-  if (threadIdx.x == 0) {
+    if (lane != 0) continue;
     const double h = R[0] - R[1], bh = p.beta * h;
     double loss, slope;  // slope = d loss / d h
     if (p.kind == kPrefSigmoid) {
@@ -298,8 +307,10 @@ __global__ __launch_bounds__(kTokBlock) void pref_join_kernel(const TokenRows a,
       p.coef[2 * pair + side] = (float)((side ? -c : c) / n[side]);
       if (p.rewards) p.rewards[2 * pair + side] = (float)(p.beta * R[side]);
     }
-    last = publish_term(p.pair_loss + pair, loss, p.ticket, pairs);
+    publish_term(p.pair_loss + pair, loss);
   }
+  __syncthreads();  // all of this workgroup's terms have arrived
+  if (threadIdx.x == 0) last = draw_ticket(p.ticket) == gridDim.x - 1;
   __syncthreads();
   if (!last) return;
   const double s = sum_terms<kTokBlock>(p.pair_loss, pairs, lds);
@@ -638,7 +649,13 @@ int launch_preference(const TokenRows& a, const float* ref_tok, const PrefArgs& 
     rc = check_launch();
   }
   if (rc) return rc;
-  hipLaunchKernelGGL(pref_join_kernel, dim3((unsigned)pairs), dim3(kTokBlock), 0, st, a, p, pairs);
+  const bool small = a.r.seq_len <= kPrefShort;
+  const int64_t groups = small ? (pairs + kTokBlock / kWave - 1) / (kTokBlock / kWave) : pairs;
+  const dim3 grid((unsigned)(groups < kPrefGrid ? groups : kPrefGrid));
+  if (small)
+    hipLaunchKernelGGL((pref_join_kernel<kWave>), grid, dim3(kTokBlock), 0, st, a, p, pairs);
+  else
+    hipLaunchKernelGGL((pref_join_kernel<kTokBlock>), grid, dim3(kTokBlock), 0, st, a, p, pairs);
   rc = check_launch();
   if (rc || !grad || a.r.n_rows == 0) return rc;
   return launch_token_grad<T>(a, 0, a.r.n_rows, w.stats, w.seq, 1, grad, st);

@@ -660,21 +660,21 @@ __device__ __forceinline__ double thread_share_of_sum_f64(const double* __restri
 }
 
 // ---- sums over workgroups without a launch of their own ------------------------
-// Every workgroup publishes one term and draws a ticket; the one that draws the
+// Every workgroup publishes its terms and draws a ticket; the one that draws the
 // last adds all the terms up, in the order of their places, so that the sum does
 // not depend on who that is.  The ticket counter is 0 when the kernel starts (a
 // kernel in front clears it).  For kernels of few workgroups: two chained
 // atomics in each of 8192 rows cost the policy loss 40 us, the launch it saves 5.
 
-// One thread: true for the last of `total` callers.  The exchange's old value is
-// waited for, so the term has arrived before the ticket is drawn.
-__device__ __forceinline__ bool publish_term(double* at, double term, unsigned* ticket, int64_t total) {
+// The exchange's old value is waited for, so the term has arrived on return.
+__device__ __forceinline__ void publish_term(double* at, double term) {
   unsigned long long* p = reinterpret_cast<unsigned long long*>(at);
   const unsigned long long old = __hip_atomic_exchange(p, (unsigned long long)__double_as_longlong(term),
                                                        __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   asm volatile("" : : "v"((uint32_t)old), "v"((uint32_t)(old >> 32)) : "memory");
-  const unsigned drawn = __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  return drawn == (unsigned)(total - 1);
+}
+__device__ __forceinline__ unsigned draw_ticket(unsigned* ticket) {
+  return __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
 // The workgroup of the last caller: the sum of all terms, in every thread.
