@@ -494,3 +494,55 @@ def test_distil_tokens_named_again_and_again(device, k, tail):
     lse = torch.logsumexp(vals.double() / T, -1).float() + 0.5
     x = torch.randn(rows, V, generator=g) * 2
     run_case(device, x, vals, idx, T, 64.0 * rows, None, lse if tail else None)
+
+
+def test_as_many_rows_as_are_taken(device):
+    n, V, k = 4_194_302, 5, 2
+    g = seeded(81)
+    x = torch.randn(n, V, generator=g) * 2
+    xd = x.to(device)
+    top = ta.top_logits(xd, k)
+    want_v, want_i = torch.sort(x, dim=-1, descending=True, stable=True)
+    assert torch.equal(top.indices.cpu().long(), want_i[:, :k]) and torch.equal(top.values.cpu(), want_v[:, :k])
+    labels = torch.randint(0, V, (n,), generator=g)
+    go = torch.randn(n, generator=g)
+    lp = x.double().log_softmax(-1)
+    at = lp.gather(-1, labels[:, None])[:, 0]
+    leaf, lab = xd.clone().requires_grad_(), labels.to(device)
+    got = ta.token_log_probs(leaf, lab)
+    assert ((got.detach().cpu().double() - at).abs() <= LOGP_ABS + 2.0 ** -24 * at.abs()).all()
+    got.backward(go.to(device))
+    onehot = torch.nn.functional.one_hot(labels, V).double()
+    slope = onehot - lp.exp()
+    check_grad(leaf.grad, go.double()[:, None] * slope, torch.float32, coef=go.abs()[:, None])
+    # one token an answer, weights that make a row's factor of the order of one
+    old, adv = (at + torch.randn(n, generator=g) * 0.05).float(), torch.randn(n, generator=g)
+    ratio = (at - old.double()).exp()
+    leaf = xd.clone().requires_grad_()
+    loss = ta.clipped_policy_loss(leaf.view(n, 1, V), lab.view(n, 1), old.to(device).view(n, 1), adv.to(device), clip_low=0.9,
+                                  clip_high=9.0, reduction="sequence", weight=float(n))
+    loss.backward()
+    terms = -ratio * adv.double()
+    assert abs(loss.item() - terms.sum().item()) <= 1e-5 * terms.abs().sum().item()
+    check_grad(leaf.grad, terms[:, None] * slope, torch.float32, coef=adv.abs()[:, None] * 1.5 * (1 + 1e-5 * 2 ** 22))
+    ref = (at + torch.randn(n, generator=g) * 0.1).float()
+    r = at - ref.double()
+    h = r[0::2] - r[1::2]
+    leaf = xd.clone().requires_grad_()
+    loss, rewards = ta.preference_loss(leaf.view(n, 1, V), lab.view(n, 1), ref.to(device), 0.5, weight=n / 2.0,
+                                       return_rewards=True)
+    loss.backward()
+    pair = torch.nn.functional.softplus(-0.5 * h)
+    assert abs(loss.item() - pair.sum().item()) <= 1e-5 * pair.sum().item()
+    assert ((rewards.cpu().double() - 0.5 * r).abs() <= LOGP_ABS + 2.0 ** -23 * r.abs()).all()
+    c = torch.stack((-0.5 * torch.sigmoid(-0.5 * h), 0.5 * torch.sigmoid(-0.5 * h)), -1).view(-1)
+    check_grad(leaf.grad, c[:, None] * slope, torch.float32, coef=c.abs()[:, None] * (1 + 1e-5 * 2 ** 22))
+    leaf = xd.clone().requires_grad_()
+    loss = ta.top_logits_distil_loss(leaf, top.values, top.indices, 1.0, weight=float(n))
+    loss.backward()
+    p = torch.zeros(n, V, dtype=torch.float64).scatter_(-1, want_i[:, :k], want_v[:, :k].double().softmax(-1))
+    term = (torch.special.xlogy(p, p) - p * lp).sum()
+    assert abs(loss.item() - term.item()) <= 1e-5 * term.item()
+    check_grad(leaf.grad, lp.exp() - p, torch.float32, coef=torch.ones(n, 1))
+    with pytest.raises(Exception):
+        ta.top_logits(torch.zeros(1 << 22, 1, device=device), 1)
