@@ -546,3 +546,40 @@ def test_as_many_rows_as_are_taken(device):
     check_grad(leaf.grad, lp.exp() - p, torch.float32, coef=torch.ones(n, 1))
     with pytest.raises(Exception):
         ta.top_logits(torch.zeros(1 << 22, 1, device=device), 1)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("tail", [False, True])
+@pytest.mark.parametrize("rows", [257, 700])
+def test_distil_wide_rows_by_the_hundred(device, rows, tail, dtype):
+    # more rows than a GPU has compute units, of the widest arrangement: the same bits as a few rows at a time,
+    # whatever rows are masked, need the true maximum or start at odd addresses
+    V, k, T = (33003 if dtype == torch.float32 else 65607), 30, 2.0
+    g = torch.Generator(device=device).manual_seed(91)
+    x = torch.randn(rows, V, generator=g, device=device, dtype=torch.float32).mul_(2).to(dtype)
+    x[5] = torch.finfo(dtype).min
+    x[300:303] = float("-inf")
+    x[300:303, 7] = 1.0
+    mask = torch.rand(rows, generator=g, device=device) < 0.7
+    mask[5] = mask[300:303] = True
+    mask[256:259] = torch.tensor([True, False, True], device=device)[:max(0, rows - 256)]
+    top = ta.top_logits(x.roll(1, 0), k, T)
+    lse = top.logsumexp + 0.5 if tail else None
+
+    def run(part):
+        n = int(mask[part].sum())
+        leaf = x[part].clone().requires_grad_()
+        loss = ta.top_logits_distil_loss(leaf, top.values[part], top.indices[part], T, float(max(n, 1)), row_mask=mask[part],
+                                         t_logsumexp=None if lse is None else lse[part])
+        loss.backward()
+        return loss.detach(), leaf.grad
+
+    _, whole = run(slice(0, rows))
+    for lo in range(0, rows, 8):
+        part = slice(lo, min(lo + 8, rows))
+        _, grad = run(part)
+        for i in range(grad.shape[0]):  # (odd V: every row starts at another address than in the whole only if lo is odd)
+            if mask[lo + i]:
+                assert bits_equal(whole[lo + i], grad[i]), lo + i
+            else:
+                assert not whole[lo + i].any()
