@@ -255,11 +255,15 @@ __device__ __forceinline__ void top_refine(TopShared<NT, KREG>& sh, int n, int k
 
 // The largest order number (to within the `enough` that end the search early)
 // that at least k of a wavefront's numbers reach, N of them a lane; 0 when
-// fewer than k are above 0.  Called by one whole wavefront.
+// fewer than k are above `floor`.  Called by one whole wavefront.
 template <int N>
-__device__ __forceinline__ uint32_t top_bar(const uint32_t (&key)[N], int k) {
+__device__ __forceinline__ uint32_t top_bar(const uint32_t (&key)[N], int k, uint32_t floor) {
   uint32_t t = 0;
   const int enough = k + k / 8 + 4;
+  int some = 0;
+#pragma unroll
+  for (int i = 0; i < N; ++i) some += (int)__popcll(__ballot(key[i] > floor));
+  if (some < k) return 0u;
   for (int bit = 31; bit >= 0; --bit) {
     const uint32_t cnd = t | (1u << bit);
     int cnt = 0;
@@ -281,6 +285,7 @@ __device__ __forceinline__ uint32_t top_bar(const uint32_t (&key)[N], int k) {
 template <typename T, bool LAST, bool MULTI, int NT, int KREG>
 __device__ __forceinline__ bool top_expand(TopShared<NT, KREG>& sh, int k) {
   constexpr int VEC = Vec16<T>::N, kCap = top_cand_cap<NT, KREG>(), kHits = top_hit_cap<NT, KREG>();
+  typedef RawMax<T> Raw;
   __syncthreads();
   const int hits = sh.n_hit;
   if (hits > kHits) return false;  // uniform
@@ -295,11 +300,11 @@ __device__ __forceinline__ bool top_expand(TopShared<NT, KREG>& sh, int k) {
         if (at < hits) {
           Vec16<T> v;
           __builtin_memcpy(&v, &sh.hit[at], 16);
-          key[i] = top_key(RawMax<T>::value(RawMax<T>::of(v)));
+          key[i] = top_key(Raw::value(Raw::of(v), Raw::least(v)));
           if (key[i] == 0xffffffffu) key[i] = 0u;  // a NaN sets no bar
         }
       }
-      const uint32_t t = top_bar<N>(key, k);
+      const uint32_t t = top_bar<N>(key, k, 0u);
       if (threadIdx.x == 0 && t) sh.bar = fmaxf(sh.bar, top_unkey(t));
     }
     __syncthreads();
@@ -386,50 +391,84 @@ __global__ __launch_bounds__(NT, NT > 256 ? 8 : 1) void top_logits_kernel(const 
     }
     __builtin_amdgcn_sched_barrier(0);
   }
-  {
+  auto publish = [&](auto group_max) {
     uint32_t whole = r.has_h || r.has_t ? top_key(fmaxf(r.h(), r.t())) : 0u;
 #pragma unroll
     for (int q = 0; q < G; ++q) {
       uint32_t key = 0u;
       if (tid + (KREG == 1 ? 0 : q * (KREG / G) * NT) < n0) {  // (a NaN sets no bar)
-        const float f = Raw::value(mx[q]);
+        const float f = group_max(q);
         key = f == f ? top_key(f) : 0u;
       }
       if (many && q > 0) sh.group[q * NT + tid] = key;
       if (!many || q == 0) whole = key > whole ? key : whole;
     }
     sh.group[tid] = whole;
-  }
-  __syncthreads();
-  if (tid < kWave) {
-    // in registers: read from LDS for every bit, 4096 rows of 30522 took 76 us instead of 57
-    constexpr int kOne = NT / kWave, kAll = G * NT / kWave;
-    uint32_t one[kOne], t;
+  };
+  auto search = [&](uint32_t floor) {
+    __syncthreads();
+    if (tid < kWave) {
+      // in registers: read from LDS for every bit, 4096 rows of 30522 took 76 us instead of 57
+      constexpr int kOne = NT / kWave, kAll = G * NT / kWave;
+      uint32_t one[kOne], t;
 #pragma unroll
-    for (int i = 0; i < kOne; ++i) one[i] = sh.group[i * kWave + tid];
-    if (many) {  // uniform
-      uint32_t all[kAll];
+      for (int i = 0; i < kOne; ++i) one[i] = sh.group[i * kWave + tid];
+      if (many) {  // uniform
+        uint32_t all[kAll];
 #pragma unroll
-      for (int i = 0; i < kAll; ++i) all[i] = i < kOne ? one[i] : sh.group[i * kWave + tid];
-      t = top_bar<kAll>(all, k);
-    } else {
-      t = top_bar<kOne>(one, k);
+        for (int i = 0; i < kAll; ++i) all[i] = i < kOne ? one[i] : sh.group[i * kWave + tid];
+        t = top_bar<kAll>(all, k, floor);
+      } else {
+        t = top_bar<kOne>(one, k, floor);
+      }
+      if (tid == 0) sh.bar = top_unkey(t);
     }
-    if (tid == 0) sh.bar = top_unkey(t);
+    __syncthreads();
+  };
+  publish([&](int q) { return Raw::value(mx[q]); });
+  search(top_key(0.f));
+  // By raw bits a group has its own maximum if it has a logit above zero, and its smallest logit if not.  With
+  // k such groups that makes no difference: the others are below the bar.  Else no bar was found, and the
+  // maxima are taken again, of the groups without such a logit by the smallest raw bits.  (With a bar from the
+  // first maxima nearly every vector reaches it: 4096 x 30522 bf16, k = 64, logits about -40 took 1740 us; now
+  // 62, and 57 where they are about 0.)
+  if (!(sh.bar > 0.f)) {  // uniform
+    int32_t mn[G];
+#pragma unroll
+    for (int q = 0; q < G; ++q) mx[q] = Raw::kNone, mn[q] = -1;
+    if (KREG == 1) {
+      __builtin_memcpy(mx, &r.v[0], 16);
+      __builtin_memcpy(mn, &r.v[0], 16);
+    } else {
+#pragma unroll
+      for (int j = 0; j < KREG; ++j) {
+        if (tid + j * NT < n0) {
+          mx[j * G / KREG] = Raw::max2(mx[j * G / KREG], Raw::of(r.v[j]));
+          mn[j * G / KREG] = Raw::min2(mn[j * G / KREG], Raw::least(r.v[j]));
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    publish([&](int q) { return Raw::value(mx[q], mn[q]); });
+    search(top_key(-__builtin_inff()));
   }
-  __syncthreads();
   const float bar = sh.bar;
-  const bool raw = bar > 0.f;  // raw bits order the logits from there up
-  int32_t below = 0;  // raw bits (twice, for 16-bit types) that a logit which reaches the bar exceeds
+  // A logit that reaches a bar above zero exceeds `limit` by its raw bits as a signed number; one that reaches
+  // another bar lies below `limit` by them as an unsigned number (so do all above zero).
+  const bool raw = bar > 0.f;
+  int32_t limit;  // (twice, for 16-bit types)
   if constexpr (sizeof(T) == 4) {
-    below = __float_as_int(bar) - 1;
+    limit = raw ? __float_as_int(bar) - 1 : __float_as_int(bar == 0.f ? -0.f : bar) + 1;
   } else {
-    // (two steps below the rounded bar: rounding may have gone up; the elements are compared exactly later)
-    const T t = from_f32<T>(bar);
+    const T t = from_f32<T>(bar == 0.f ? -0.f : bar);
     uint16_t bits;
     __builtin_memcpy(&bits, &t, 2);
-    const int32_t b = bits > 1 ? bits - 2 : 0;
-    below = (b << 16) | b;
+    uint32_t b;
+    if (raw)  // two steps below the rounded bar: rounding may have gone up; the elements are compared exactly later
+      b = bits > 1 ? bits - 2u : 0u;
+    else  // the least logit that reaches the bar, and one: a step of 16-bit logits far below zero holds many of them
+      b = bits + (to_f32(t) < bar ? 0u : 1u);
+    limit = (int32_t)(b * 0x10001u);
   }
   auto take = [&](float xv, int i) {
     if (xv >= bar) {
@@ -440,11 +479,7 @@ __global__ __launch_bounds__(NT, NT > 256 ? 8 : 1) void top_logits_kernel(const 
   if (tid < g.head) take(r.h(), tid);
   if (g.tail0 + tid < V) take(r.t(), (int)g.tail0 + tid);
   auto reaches = [&](const Vec16<T>& v) {
-    if (raw) return Raw::max2(Raw::of(v), below) != below;
-    float m = -__builtin_inff();
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) m = fmaxf(m, to_f32(v.v[i]));
-    return m >= bar;
+    return raw ? Raw::max2(Raw::of(v), limit) != limit : Raw::min2(Raw::least(v), limit) != limit;
   };
   // Candidates, piece by piece.  A register that is done with takes the next piece's vector at once, so
   // that loads are always under way; later pieces are summed in this walk.

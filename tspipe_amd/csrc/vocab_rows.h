@@ -397,6 +397,39 @@ struct RawMax {
       return to_f32(t);
     }
   }
+  // The smallest by their bits as unsigned numbers: of a vector without a logit above zero, its largest logit.
+  __device__ __forceinline__ static int32_t min2(int32_t a, int32_t b) {
+    if constexpr (sizeof(T) == 4) {
+      return (int32_t)((uint32_t)a < (uint32_t)b ? (uint32_t)a : (uint32_t)b);
+    } else {
+      typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+      u16x2 x, y;
+      __builtin_memcpy(&x, &a, 4);
+      __builtin_memcpy(&y, &b, 4);
+      const u16x2 z = __builtin_elementwise_min(x, y);
+      int32_t r;
+      __builtin_memcpy(&r, &z, 4);
+      return r;
+    }
+  }
+  __device__ __forceinline__ static int32_t least(const Vec16<T>& v) {
+    int32_t w[4];
+    __builtin_memcpy(w, &v, 16);
+    return min2(min2(w[0], w[1]), min2(w[2], w[3]));
+  }
+  // The largest logit of elements whose raw maximum and minimum are m and l.
+  __device__ __forceinline__ static float value(int32_t m, int32_t l) {
+    if constexpr (sizeof(T) == 4) {
+      return __int_as_float(m >= 0 ? m : l);
+    } else {
+      const int32_t lo = (int16_t)(m & 0xffff) >= 0 ? m : l, hi = m >= 0 ? m : l;
+      const uint16_t a = (uint16_t)(lo & 0xffff), b = (uint16_t)((uint32_t)hi >> 16);
+      T x, y;
+      __builtin_memcpy(&x, &a, 2);
+      __builtin_memcpy(&y, &b, 2);
+      return fmaxf(to_f32(x), to_f32(y));
+    }
+  }
 };
 
 // The largest of m and of the wavefront's elements in its first nvec vectors.
