@@ -258,14 +258,16 @@ def preference_loss_fn(student_outputs, teacher_outputs, labels, tspipe_args, pa
     """``loss_fn`` plug-in: ``preference_loss`` of a causal student against the
     frozen teacher.  ``labels`` is ``(tokens, answer_mask)``, both ``[2 pairs,
     tokens]``; ``params`` carries ``beta`` and optionally ``preference_type``,
-    ``label_smoothing`` and ``length_average``."""
+    ``label_smoothing``, ``length_average`` and ``weight`` (a half precision
+    gradient's loss scale)."""
     targets = _next_tokens(*labels)
     with torch.no_grad():
         ref = token_log_probs(teacher_outputs["logits"].detach(), targets)
     return preference_loss(student_outputs["logits"], targets, ref, beta=params.beta,
                            loss_type=getattr(params, "preference_type", "sigmoid"),
                            label_smoothing=getattr(params, "label_smoothing", 0.0),
-                           length_average=getattr(params, "length_average", False))
+                           length_average=getattr(params, "length_average", False),
+                           weight=getattr(params, "weight", 1.0))
 
 
 def policy_loss_fn(student_outputs, teacher_outputs, labels, tspipe_args, params, epoch: int) -> Tensor:
@@ -273,7 +275,8 @@ def policy_loss_fn(student_outputs, teacher_outputs, labels, tspipe_args, params
     teacher as the reference of the KL term.  ``labels`` is ``(tokens,
     answer_mask, old_log_probs, advantages)``, ``old_log_probs`` at the position
     whose logits gave them; ``params`` carries ``kl_weight``, ``clip_low``,
-    ``clip_high`` and optionally ``temperature`` and ``reduction``."""
+    ``clip_high`` and optionally ``temperature``, ``reduction`` and ``weight`` (a
+    half precision gradient's loss scale)."""
     tokens, answer_mask, old, adv = labels
     targets = _next_tokens(tokens, answer_mask)
     temperature = getattr(params, "temperature", 1.0)
@@ -282,4 +285,5 @@ def policy_loss_fn(student_outputs, teacher_outputs, labels, tspipe_args, params
         with torch.no_grad():
             ref = token_log_probs(teacher_outputs["logits"].detach(), targets, temperature)
     return clipped_policy_loss(student_outputs["logits"], targets, old, adv, ref, params.kl_weight, params.clip_low,
-                               params.clip_high, temperature, getattr(params, "reduction", "token"))
+                               params.clip_high, temperature, getattr(params, "reduction", "token"),
+                               weight=getattr(params, "weight", 1.0))
