@@ -1,4 +1,5 @@
 """Argument handling shared by the losses on rows of vocabulary logits."""
+import math
 from typing import NamedTuple, Optional
 
 import torch
@@ -64,7 +65,7 @@ def rows_of(logits: Tensor, what: str) -> Rows:
     if x.dim() == 1:
         x = x[None]
     elif x.dim() > 3:
-        x = x.reshape(-1, x.shape[-2], V)
+        x = x.reshape(math.prod(x.shape[:-2]), x.shape[-2], V)  # (-1 is ambiguous where there is nothing)
         if V > 1 and x.stride(-1) != 1:
             x = x.contiguous()
     if x.dim() == 2:
