@@ -1018,12 +1018,18 @@ int launch_top_logits(const VocabRows& a, int k, void* values, int32_t* indices,
   return check_launch();
 }
 
+// Bytes of the marks: a bit per vocabulary entry and eight in front.
+inline size_t top_marks_bytes(int64_t V) { return (size_t)((V + 8 + 31) / 32) * 4; }
+
 template <typename T, int NT, int KREG, bool LONG, bool TAIL>
 int launch_top_distil_rows(const TopDistilArgs& a, hipStream_t st) {
-  const size_t marks = TAIL ? (size_t)((a.r.V + 8 + 31) / 32) * 4 : 0;
+  const size_t marks = TAIL ? top_marks_bytes(a.r.V) : 0;
   if (marks > 32768) {
+    // (the largest there is, whatever this call takes: the bound is the function's, and another thread may set
+    // it between this call's setting and its launch)
     const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&top_distil_kernel<T, NT, KREG, LONG, TAIL>),
-                                             hipFuncAttributeMaxDynamicSharedMemorySize, (int)marks);
+                                             hipFuncAttributeMaxDynamicSharedMemorySize,
+                                             (int)top_marks_bytes(kTopTailVocab));
     if (e != hipSuccess) {
       set_last_hip_error((int)e);
       return TS_ERR_LAUNCH;
