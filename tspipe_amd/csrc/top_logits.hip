@@ -519,7 +519,11 @@ __global__ __launch_bounds__(NT, NT > 256 ? 8 : 1) void top_logits_kernel(const 
     top_row_walked<T>(a, row, x, k, values, indices, lse, sh);
     return;
   }
-  if (tid == 0 && lse) lse[row] = -rowsum_log_prob(a, s, 0.f).hi;  // the log probability of a logit of 0
+  if (tid == 0 && lse) {
+    const Float2x l = rowsum_log_prob(a, s, 0.f);  // the log probability of a logit of 0
+    // What k's rounding took is that much of the row's mean; the log-sum-exp stands in for it, a few units away.
+    lse[row] = -(l.hi + fmaf(l.hi, a.k_rel, l.lo));
+  }
   top_emit<T>(sh, sh.n, x, row, k, values, indices);
 }
 
