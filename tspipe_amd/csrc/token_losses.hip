@@ -63,7 +63,7 @@ struct TokenGrad {
 // sum of differences to a reference that nearly agrees shows every unit of fp32.
 // Rows longer than NT * KREG vectors are walked in pieces of that size.
 template <typename T, int NT, int KREG>
-__global__ __launch_bounds__(NT) void token_stat_kernel(const TokenRows a, int64_t row0, const float* __restrict__ ref,
+__global__ __launch_bounds__(NT) void token_stat_kernel(const TokenRows a, const float* __restrict__ ref,
                                                         float* __restrict__ logp, double* __restrict__ log_ratio,
                                                         float2* __restrict__ stats, unsigned* __restrict__ ticket) {
   if (ticket && blockIdx.x == 0 && threadIdx.x == 0) *ticket = 0u;  // of the next kernel
@@ -72,7 +72,7 @@ __global__ __launch_bounds__(NT) void token_stat_kernel(const TokenRows a, int64
   __shared__ double lds_z[NW];
   __shared__ float lds_c[NW], lds_a[NW];
   __shared__ VocabStat lds_v[NW];
-  const int64_t row = row0 + blockIdx.x;
+  const int64_t row = blockIdx.x;
   int64_t label;
   if (!token_live<true>(a, row, &label)) {
     if (threadIdx.x == 0) {
@@ -588,11 +588,11 @@ inline TokenWs token_carve(void* ws, int64_t n_rows, int64_t n_seq) {
 }
 
 template <typename T>
-int launch_token_stat(const TokenRows& a, int64_t row0, int64_t rows, const float* ref, float* logp, double* log_ratio,
-                      float2* stats, unsigned* ticket, hipStream_t st) {
+int launch_token_stat(const TokenRows& a, const float* ref, float* logp, double* log_ratio, float2* stats,
+                      unsigned* ticket, hipStream_t st) {
   const RowShape sh = row_shape<T>(a.r.V);
-#define TS_STAT(NT, KREG)                                                                                        \
-  hipLaunchKernelGGL((token_stat_kernel<T, NT, KREG>), dim3((unsigned)rows), dim3(NT), 0, st, a, row0, ref, logp, \
+#define TS_STAT(NT, KREG)                                                                                         \
+  hipLaunchKernelGGL((token_stat_kernel<T, NT, KREG>), dim3((unsigned)a.r.n_rows), dim3(NT), 0, st, a, ref, logp, \
                      log_ratio, stats, ticket)
   if (sh.nt == 64)
     TS_STAT(64, 4);
@@ -607,20 +607,20 @@ int launch_token_stat(const TokenRows& a, int64_t row0, int64_t rows, const floa
 }
 
 template <typename T>
-int launch_token_grad(const TokenRows& a, int64_t row0, int64_t rows, const float2* stats, const float* coef,
-                      int per_seq, void* grad, hipStream_t st) {
+int launch_token_grad(const TokenRows& a, const float2* stats, const float* coef, int per_seq, void* grad,
+                      hipStream_t st) {
   const int64_t vecs = a.r.V / Vec16<T>::N;
   const int64_t parts = vecs <= kGradPart ? 1 : (vecs + kGradPart - 1) / kGradPart;
   // (the grid counts threads in 32 bits)
-  for (int64_t done = 0; done < rows;) {
-    int64_t n = rows - done;
+  for (int64_t row0 = 0; row0 < a.r.n_rows;) {
+    int64_t n = a.r.n_rows - row0;
     if (n * parts > (1 << 23)) n = (1 << 23) / parts;
     if (n < 1) return TS_ERR_RANGE;
-    hipLaunchKernelGGL((token_grad_kernel<T>), dim3((unsigned)(n * parts)), dim3(kTokBlock), 0, st, a, row0 + done,
+    hipLaunchKernelGGL((token_grad_kernel<T>), dim3((unsigned)(n * parts)), dim3(kTokBlock), 0, st, a, row0,
                        (int)parts, stats, coef, per_seq, reinterpret_cast<T*>(grad));
     const int rc = check_launch();
     if (rc) return rc;
-    done += n;
+    row0 += n;
   }
   return TS_OK;
 }
@@ -643,7 +643,7 @@ int launch_preference(const TokenRows& a, const float* ref_tok, const PrefArgs& 
   if (pairs == 0) return launch_nan(p.loss, st);
   int rc;
   if (a.r.n_rows > 0) {
-    rc = launch_token_stat<T>(a, 0, a.r.n_rows, ref_tok, nullptr, w.row, w.stats, p.ticket, st);
+    rc = launch_token_stat<T>(a, ref_tok, nullptr, w.row, w.stats, p.ticket, st);
   } else {
     hipLaunchKernelGGL(clear_ticket_kernel, dim3(1), dim3(1), 0, st, p.ticket);
     rc = check_launch();
@@ -658,7 +658,7 @@ int launch_preference(const TokenRows& a, const float* ref_tok, const PrefArgs& 
     hipLaunchKernelGGL((pref_join_kernel<kTokBlock>), grid, dim3(kTokBlock), 0, st, a, p, pairs);
   rc = check_launch();
   if (rc || !grad || a.r.n_rows == 0) return rc;
-  return launch_token_grad<T>(a, 0, a.r.n_rows, w.stats, w.seq, 1, grad, st);
+  return launch_token_grad<T>(a, w.stats, w.seq, 1, grad, st);
 }
 
 template <typename T>
@@ -684,13 +684,13 @@ int launch_policy(const TokenRows& a, const PolicyArgs& p, const TokenWs& w, int
   else if (sh.kreg == 16)
     TS_POLICY(1024, 16);
   else {
-    rc = launch_token_stat<T>(a, 0, a.r.n_rows, nullptr, nullptr, w.lp, w.stats, nullptr, st);
+    rc = launch_token_stat<T>(a, nullptr, nullptr, w.lp, w.stats, nullptr, st);
     if (rc) return rc;
     hipLaunchKernelGGL((policy_coef_kernel<T>), dim3((unsigned)((a.r.n_rows + kTokBlock - 1) / kTokBlock)),
                        dim3(kTokBlock), 0, st, a, p, w.lp, w.coef);
     rc = check_launch();
     if (rc) return rc;
-    if (p.grad) rc = launch_token_grad<T>(a, 0, a.r.n_rows, w.stats, w.coef, 0, p.grad, st);
+    if (p.grad) rc = launch_token_grad<T>(a, w.stats, w.coef, 0, p.grad, st);
     if (rc) return rc;
   }
 #undef TS_POLICY
@@ -736,7 +736,7 @@ int ts_token_logp_fwd(const void* s, int64_t n_seq, int64_t seq_len, int64_t V, 
   const ts::TokenRows a =
       ts::token_rows(s, n_seq, seq_len, V, ld_seq, ld_tok, labels, row_mask, ignore_index, temperature);
   hipStream_t st = (hipStream_t)stream;
-  TS_BY_DTYPE(dtype, (ts::launch_token_stat<T>(a, 0, a.r.n_rows, nullptr, logp, nullptr, (float2*)stats, nullptr, st)))
+  TS_BY_DTYPE(dtype, (ts::launch_token_stat<T>(a, nullptr, logp, nullptr, (float2*)stats, nullptr, st)))
 }
 
 int ts_token_logp_bwd(const void* s, int64_t n_seq, int64_t seq_len, int64_t V, int64_t ld_seq, int64_t ld_tok,
@@ -750,7 +750,7 @@ int ts_token_logp_bwd(const void* s, int64_t n_seq, int64_t seq_len, int64_t V, 
   const ts::TokenRows a =
       ts::token_rows(s, n_seq, seq_len, V, ld_seq, ld_tok, labels, row_mask, ignore_index, temperature);
   hipStream_t st = (hipStream_t)stream;
-  TS_BY_DTYPE(dtype, (ts::launch_token_grad<T>(a, 0, a.r.n_rows, (const float2*)stats, grad_logp, 0, grad, st)))
+  TS_BY_DTYPE(dtype, (ts::launch_token_grad<T>(a, (const float2*)stats, grad_logp, 0, grad, st)))
 }
 
 size_t ts_token_loss_workspace_bytes(int64_t n_seq, int64_t seq_len) {
