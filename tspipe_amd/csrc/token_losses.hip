@@ -420,7 +420,10 @@ __global__ __launch_bounds__(kWeightBlock) void policy_weight_kernel(const Token
   if (threadIdx.x == 0) counts[0] = total;
 }
 
-// loss term and d loss / d logp of one token
+// Loss term and d loss / d logp of one token, in fp32: the log probability comes
+// as two floats, so that differences to the other models' keep their accuracy, and
+// each part of the term is off by about 2^-22 of itself.  64-bit exponentials would
+// take registers from the row.
 __device__ __forceinline__ void policy_term(const PolicyArgs& p, Float2x lp, float old_lp, float ref_lp, float A,
                                             float* term, float* slope) {
   const float r = expf((lp.hi - old_lp) + lp.lo);
@@ -544,7 +547,8 @@ __global__ __launch_bounds__(kTokBlock) void policy_coef_kernel(const TokenRows 
   r.ref_lp = p.ref_logp ? p.ref_logp[row] : 0.f;
   r.adv = p.adv[p.adv_per_seq ? seq : row];
   r.weight = p.seq_weight[seq];
-  // (the gradient kernel takes the temperature itself)
+  // (the gradient kernel takes the temperature itself; divided out and multiplied in again
+  // the factor is the same, but for one tie in forty million)
   coef[row] = policy_finish(a, p, r, row, Float2x{hi, fabsf(hi) < __builtin_inff() ? (float)(l - (double)hi) : 0.f}) /
               (float)a.r.inv_T;
 }

@@ -155,8 +155,10 @@ __device__ __forceinline__ void top_emit(TopShared<NT, KREG>& sh, int n, const T
   }
 }
 
-// Rows with a NaN, with a sum that needs the true maximum, or with more
-// candidates than fit (thousands of equal logits at the border).  The k-th
+// Rows with a NaN, with a sum that needs the true maximum, or of which more
+// vectors or candidates reach the bar than fit: thousands of equal logits at the
+// border, fewer than k logits above -inf or the type's lowest value, the best
+// behind the first piece (2048 x 30522 fp32 in rising order: 1.8 ms).  The k-th
 // largest order number is the bar's, if fewer than k elements exceed the bar (a
 // vocabulary masked but for fewer than k tokens), or found bit by bit (the largest
 // t such that at least k elements reach it); then the place up to which elements
@@ -344,9 +346,11 @@ __device__ __forceinline__ bool top_expand(TopShared<NT, KREG>& sh, int k) {
 // and a vector that reaches the bar is only noted; its elements are looked at
 // when the noted vectors are spread over all threads.
 //
-// MULTI: the row has more than one piece.  Eight wavefronts a SIMD: 64 registers
-// are enough, and with 80 and six of them 4096 x 30522 bf16 took 67 us instead
-// of 58 (55 by now), 1024 x 131072 96 instead of 79.
+// MULTI: the row has more than one piece.  Eight wavefronts a SIMD, so 64
+// registers, which the forms of one piece fit; that of several leaves five in
+// scratch memory (24 bytes a thread), and is faster so than without: with 80 and
+// six wavefronts 4096 x 30522 bf16 took 67 us instead of 58 (55 by now), 1024 x
+// 131072 96 instead of 79.
 template <typename T, int NT, int KREG, bool MULTI>
 __global__ __launch_bounds__(NT, NT > 256 ? 8 : 1) void top_logits_kernel(const VocabRows a, int k,
                                                                           T* __restrict__ values,
@@ -720,10 +724,13 @@ __device__ __forceinline__ uint32_t top_mark_bit(int j, const VocabGeom& g) { re
 // LONG rows do not fit the registers: this kernel then reads them in pieces and
 // leaves the gradient to two others.
 //
-// 64 registers a thread for up to eight vectors of a row, but for the 512-thread
-// arrangement, which would spill there: with six wavefronts a SIMD instead of
-// eight 4096 x 30522 bf16 with 85 % of the rows takes 92 us (505 MB, 5.5 TB/s)
-// instead of 99.
+// Registers: 80 in the 512-thread arrangement, of which six wavefronts a SIMD
+// are resident instead of eight (4096 x 30522 bf16 with 85 % of the rows, other
+// classes as one outcome: 92 us (505 MB, 5.5 TB/s) instead of 99 with 64).  Two
+// rows of 1024 threads with eight vectors each share a CU at 64 registers; the
+// form without the other classes leaves one or two of them in scratch memory,
+// that with them 13 (fp16: 19), 48 to 56 bytes a thread: 2044 x 50257 bf16 takes
+// 98 and 104 us a call.
 template <typename T, int NT, int KREG, bool LONG, bool TAIL>
 __global__ __launch_bounds__(NT, (KREG > 8 || LONG ? 4 : NT > 256 ? (NT > 512 ? 8 : 6) : 1)) void top_distil_kernel(
     const TopDistilArgs a) {

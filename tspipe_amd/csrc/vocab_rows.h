@@ -18,9 +18,12 @@ struct VocabRows {
   const void* s;
   int64_t n_rows, seq_len, V, ld_seq, ld_tok;
   // 2^(x k) = e^(x / T); k is log2(e) / T rounded to fp32 and k_rel what the
-  // rounding took, relative: (log2(e) / T - k) / k.  Every exponent of a row is
-  // off by that same factor, which would add up over a sequence of rows, so the
-  // log-sum-exp is corrected for it to first order.
+  // rounding took, relative: (log2(e) / T - k) / k, at most 2^-24.  Every exponent
+  // of a row is off by that same factor, which would add up over a sequence of
+  // rows and show in the log-sum-exp of a row far from zero: token_stat_kernel and
+  // top_logits_kernel correct for it to first order.  The policy loss and the
+  // distillation, which add up no sequence's log probabilities, leave it in them,
+  // times their distance from the row's mean (16: 1e-6).
   float k, k_rel;
   double inv_T;
 };
