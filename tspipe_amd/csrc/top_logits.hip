@@ -306,7 +306,7 @@ __device__ __forceinline__ bool top_expand(TopShared<NT, KREG>& sh, int k) {
           if (key[i] == 0xffffffffu) key[i] = 0u;  // a NaN sets no bar
         }
       }
-      const uint32_t t = top_bar<N>(key, k, 0u);
+      const uint32_t t = top_bar<N>(key, k, top_key(sh.bar));
       if (threadIdx.x == 0 && t) sh.bar = fmaxf(sh.bar, top_unkey(t));
     }
     __syncthreads();
@@ -347,10 +347,10 @@ __device__ __forceinline__ bool top_expand(TopShared<NT, KREG>& sh, int k) {
 // when the noted vectors are spread over all threads.
 //
 // MULTI: the row has more than one piece.  Eight wavefronts a SIMD, so 64
-// registers, which the forms of one piece fit; that of several leaves five in
-// scratch memory (24 bytes a thread), and is faster so than without: with 80 and
-// six wavefronts 4096 x 30522 bf16 took 67 us instead of 58 (55 by now), 1024 x
-// 131072 96 instead of 79.
+// registers, which the forms of one piece fit; that of several leaves four or five
+// in scratch memory (20 to 24 bytes a thread).  With 80 and six wavefronts 4096 x
+// 30522 bf16 took 67 us instead of 58 (55 by now), 1024 x 131072 96 instead of 79
+// (75 by now).
 template <typename T, int NT, int KREG, bool MULTI>
 __global__ __launch_bounds__(NT, NT > 256 ? 8 : 1) void top_logits_kernel(const VocabRows a, int k,
                                                                           T* __restrict__ values,
