@@ -557,13 +557,17 @@ struct TopDistilArgs {
   void* grad;  // may be null
 };
 
-// The gradient of a row's tokens without an entry: go 2^(x k + off), or go
-// 2^((x - off) k) for walked rows; with rz for go a token's probability.
+// A row's gradient: go 2^(x k + off) of the tokens without an entry, and rz times
+// that power a token's probability; of walked rows go 2^((x - off) k), off the
+// largest of these tokens' logits, and with off_all, the row's, a probability.
 struct TopRowGrad {
-  float off, go, rz;
-  int by_max;
-  __device__ __forceinline__ float power(float x, float k) const {
-    return fast_exp2(by_max ? (x - off) * k : fmaf(x, k, off));
+  float off, go, rz, off_all;
+  int by_max, unused;  // (a multiple of 8 bytes)
+  __device__ __forceinline__ float other(float x, float k) const {
+    return go * fast_exp2(by_max ? (x - off) * k : fmaf(x, k, off));
+  }
+  __device__ __forceinline__ float prob(float x, float k) const {
+    return rz * fast_exp2(by_max ? (x - off_all) * k : fmaf(x, k, off));
   }
 };
 
@@ -729,8 +733,8 @@ __device__ __forceinline__ uint32_t top_mark_bit(int j, const VocabGeom& g) { re
 // classes as one outcome: 92 us (505 MB, 5.5 TB/s) instead of 99 with 64).  Two
 // rows of 1024 threads with eight vectors each share a CU at 64 registers; the
 // form without the other classes leaves one or two of them in scratch memory,
-// that with them 13 (fp16: 19), 48 to 56 bytes a thread: 2044 x 50257 bf16 takes
-// 98 and 104 us a call.
+// that with them 13, 48 bytes a thread: 2044 x 50257 bf16 takes 98 and 104 us a
+// call.
 template <typename T, int NT, int KREG, bool LONG, bool TAIL>
 __global__ __launch_bounds__(NT, (KREG > 8 || LONG ? 4 : NT > 256 ? (NT > 512 ? 8 : 6) : 1)) void top_distil_kernel(
     const TopDistilArgs a) {
@@ -782,13 +786,6 @@ __global__ __launch_bounds__(NT, (KREG > 8 || LONG ? 4 : NT > 256 ? (NT > 512 ? 
   }
   const TopTeacher t = scalar_load(a.teacher + row);
   const float gs = a.gscale / (float)scalar_load(a.live);
-  // Factor of the other tokens' probabilities in the gradient; inv_q_rest: one over what the student
-  // leaves to the tokens without an entry.
-  auto outside = [&](float inv_q_rest) {
-    float o = t.whole;
-    if (TAIL && t.rest > 0.f && inv_q_rest < __builtin_inff()) o = fmaf(-t.rest, inv_q_rest, o);
-    return gs * o;
-  };
   // The row's loss, after its gradient (no wavefront waits for it): lq(x) = ln of the student's
   // probability of a logit x, lq_rest that of all tokens without an entry.
   auto loss = [&](auto lq, auto lq_rest) {
@@ -809,8 +806,8 @@ __global__ __launch_bounds__(NT, (KREG > 8 || LONG ? 4 : NT > 256 ? (NT > 512 ? 
       a.row_loss[row] = term;
     }
   };
-  auto leave = [&](float off, float go, float rz, int by_max) {  // LONG
-    if (tid == 0) a.row_grad[row] = TopRowGrad{off, go, rz, by_max};
+  auto leave = [&](float off, float go, float rz, float off_all, int by_max) {  // LONG
+    if (tid == 0) a.row_grad[row] = TopRowGrad{off, go, rz, off_all, by_max, 0};
   };
   auto patch = [&](auto q_of) {  // the kept entries' gradients replace what the walk over the row wrote
     __syncthreads();
@@ -863,11 +860,13 @@ __global__ __launch_bounds__(NT, (KREG > 8 || LONG ? 4 : NT > 256 ? (NT > 512 ? 
     const float rest_z = s.z;
     if (TAIL) s.z += s.a;
     if (grow) {
-      const float rz = 1.f / s.z, go = outside(s.z / rest_z) * rz, c = s.c;
+      // the other tokens' q (P - r / q_r), q_r what the student leaves to them
+      const float rz = 1.f / s.z, c = s.c;
+      const float go = gs * (TAIL && t.rest > 0.f ? fmaf(-t.rest, s.z / rest_z, t.whole) : t.whole) * rz;
       auto other = [=](float xv) { return go * fast_exp2(fmaf(xv, kk, c)); };
       auto none = [](float) { return 0.f; };
       if (LONG) {
-        leave(c, go, rz, 0);
+        leave(c, go, rz, c, 0);
       } else {
         regs_map(r, g, x, grow, V, -1, other, none);
         patch([&](float xv) { return fast_exp2(fmaf(xv, kk, c)) * rz; });
@@ -900,21 +899,26 @@ __global__ __launch_bounds__(NT, (KREG > 8 || LONG ? 4 : NT > 256 ? (NT > 512 ? 
   }
   // the rest's share: its sum, moved to the row's maximum, which may underflow where its logarithm does not
   Float2x lq_rest{0.f, 0.f};
-  float inv_q_rest = 0.f;
   if (TAIL) {
     const Float2x d = two_sum(out.m, -all.m), e = two_mul(d.hi, kk), l = log2_2x(out.z), h = two_sum(e.hi, l.hi);
     if (out.z > 0.f || out.z != out.z)
       lq_rest = ln_share(Float2x{h.hi, h.lo + (l.lo + (e.lo + d.lo * kk))}, all.z);
     else
       lq_rest.hi = -__builtin_inff();
-    inv_q_rest = fast_exp2(-e.hi) * (all.z / out.z);
   }
   if (grow) {
-    const float rz = 1.f / all.z, go = outside(inv_q_rest) * rz, m = all.m;
+    // The other tokens' q P - r q / q_r by their own maximum: q_r, and with it all of their q, may underflow
+    // where q / q_r does not (where their sum is 0 none of them can be reached, and r / q_r is left out).
+    // (As scalars: in vector registers 17 instead of 13 are spilled in the 1024 x 8 form, 4096 x 30522 fp32 226
+    // instead of 208 us a call.)
+    const float rz = same_in_wave(1.f / all.z), m = same_in_wave(all.m), off = same_in_wave(TAIL ? out.m : all.m);
+    float go = t.whole * rz;
+    if (TAIL) go = go * fast_exp2((off - m) * kk) - (t.rest > 0.f && out.z != 0.f ? t.rest / out.z : 0.f);
+    go = same_in_wave(gs * go);
     if (LONG) {
-      leave(m, go, rz, 1);
+      leave(off, go, rz, m, 1);
     } else {
-      vocab_map_walk<T, NT>(x, grow, V, [=](float xv, int) { return go * fast_exp2((xv - m) * kk); });
+      vocab_map_walk<T, NT>(x, grow, V, [=](float xv, int) { return go * fast_exp2((xv - off) * kk); });
       patch([&](float xv) { return fast_exp2((xv - m) * kk) * rz; });
     }
   }
@@ -958,7 +962,7 @@ __global__ __launch_bounds__(kMapBlock) void top_map_kernel(const TopDistilArgs 
   for (int j = 0; j < kMapVecs; ++j) r.v[j] = vec_load<T>(from, tid + j * kMapBlock);
   const TopRowGrad f = scalar_load(a.row_grad + row);
   const float k = a.r.k;
-  auto other = [&](float xv) { return f.go * f.power(xv, k); };
+  auto other = [&](float xv) { return f.other(xv, k); };
   if (part == 0 && tid < g.head) grow[tid] = from_f32<T>(other(to_f32(x[tid])));
   if (part == parts - 1 && g.tail0 + tid < V) grow[g.tail0 + tid] = from_f32<T>(other(to_f32(x[g.tail0 + tid])));
   const bool gvec = (((uintptr_t)grow ^ (uintptr_t)x) & 15u) == 0;
@@ -998,7 +1002,7 @@ __global__ __launch_bounds__(kMapBlock) void top_entries_kernel(const TopDistilA
   const TopRowGrad f = a.row_grad[row];
   const float gs = a.gscale / (float)*a.live;
   reinterpret_cast<T*>(a.grad)[row * a.r.V + idx] =
-      from_f32<T>(gs * fmaf(f.power(to_f32(x[idx]), a.r.k) * f.rz, a.teacher[row].whole, -p));
+      from_f32<T>(gs * fmaf(f.prob(to_f32(x[idx]), a.r.k), a.teacher[row].whole, -p));
 }
 
 __global__ __launch_bounds__(1024) void top_distil_sum_kernel(const double* __restrict__ v, int64_t n,
@@ -1092,7 +1096,7 @@ int launch_top_distil(const TopDistilArgs& a, double loss_scale, float* loss_out
 }
 
 // Workspace: live count (16 bytes), teacher and gradient numbers and loss terms per row, probabilities per entry.
-inline size_t top_ws_bytes(int64_t n_rows, int64_t k) { return 16 + (size_t)n_rows * (16 + 16 + 8) + (size_t)(n_rows * k) * 4; }
+inline size_t top_ws_bytes(int64_t n_rows, int64_t k) { return 16 + (size_t)n_rows * (16 + 24 + 8) + (size_t)(n_rows * k) * 4; }
 
 }  // namespace ts
 
@@ -1144,8 +1148,8 @@ int ts_top_distil_fwd_bwd(const void* s, int64_t n_seq, int64_t seq_len, int64_t
   a.live = reinterpret_cast<int*>(ws);
   a.teacher = reinterpret_cast<ts::TopTeacher*>(ws + 16);
   a.row_grad = reinterpret_cast<ts::TopRowGrad*>(ws + 16 + a.r.n_rows * 16);
-  a.row_loss = reinterpret_cast<double*>(ws + 16 + a.r.n_rows * 32);
-  a.entry_p = reinterpret_cast<float*>(ws + 16 + a.r.n_rows * 40);
+  a.row_loss = reinterpret_cast<double*>(ws + 16 + a.r.n_rows * 40);
+  a.entry_p = reinterpret_cast<float*>(ws + 16 + a.r.n_rows * 48);
   a.grad = grad;
   hipStream_t st = (hipStream_t)stream;
   TS_BY_DTYPE(dtype, (ts::launch_top_distil<T>(a, weight * temperature * temperature, loss_out, st)))

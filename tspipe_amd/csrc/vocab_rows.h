@@ -72,6 +72,11 @@ __device__ __forceinline__ const T* vocab_row(const VocabRows& a, int64_t row) {
   return reinterpret_cast<const T*>(((uint64_t)hi << 32) | lo);
 }
 
+// A number that is the same in every lane, said to the compiler as the address above.
+__device__ __forceinline__ float same_in_wave(float x) {
+  return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(x)));
+}
+
 // An fp32 number and what its rounding left out.  The log probabilities of a row
 // are formed in this type: a sum over a sequence of them, or the difference of
 // two that nearly agree, would show the last bits of fp32, and 64-bit
