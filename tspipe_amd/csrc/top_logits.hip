@@ -730,11 +730,10 @@ __device__ __forceinline__ uint32_t top_mark_bit(int j, const VocabGeom& g) { re
 //
 // Registers: 80 in the 512-thread arrangement, of which six wavefronts a SIMD
 // are resident instead of eight (4096 x 30522 bf16 with 85 % of the rows, other
-// classes as one outcome: 92 us (505 MB, 5.5 TB/s) instead of 99 with 64).  Two
-// rows of 1024 threads with eight vectors each share a CU at 64 registers; the
-// form without the other classes leaves one or two of them in scratch memory,
-// that with them 13, 48 bytes a thread: 2044 x 50257 bf16 takes 98 and 104 us a
-// call.
+// classes as one outcome: 88 us, 505 MB at 5.7 TB/s; when 80 took 92, 64 took 99).
+// Two rows of 1024 threads with eight vectors each share a CU at 64 registers; the
+// form without the other classes leaves one or two of them in scratch memory, that
+// with them 13, 48 bytes a thread: 2044 x 50257 bf16 takes 98 and 104 us a call.
 template <typename T, int NT, int KREG, bool LONG, bool TAIL>
 __global__ __launch_bounds__(NT, (KREG > 8 || LONG ? 4 : NT > 256 ? (NT > 512 ? 8 : 6) : 1)) void top_distil_kernel(
     const TopDistilArgs a) {
