@@ -714,6 +714,11 @@ __global__ __launch_bounds__(kTeacherBlock) void top_teacher_kernel(const TopDis
   a.teacher[row] = TopTeacher{p_ln_p, (float)(sum + (double)rest), rest};
 }
 
+// Error of a log-sum-exp: that of one of top_logits before its rounding, and of the rounding, a step of fp32.
+constexpr float kTopLseError = 4e-6f, kTopLseRounding = 1.1920929e-07f;
+// ln of a share of the student's probability, 1e-30, below which a remainder no larger than that is none.
+constexpr float kTopOutOfReach = -69.f;
+
 template <int NT>
 struct TopDistilShared {
   RowSum sums[NT / kWave];
@@ -731,9 +736,10 @@ __device__ __forceinline__ uint32_t top_mark_bit(int j, const VocabGeom& g) { re
 // Registers: 80 in the 512-thread arrangement, of which six wavefronts a SIMD
 // are resident instead of eight (4096 x 30522 bf16 with 85 % of the rows, other
 // classes as one outcome: 88 us, 505 MB at 5.7 TB/s; when 80 took 92, 64 took 99).
-// Two rows of 1024 threads with eight vectors each share a CU at 64 registers; the
-// form without the other classes leaves one or two of them in scratch memory, that
-// with them 13, 48 bytes a thread: 2044 x 50257 bf16 takes 98 and 104 us a call.
+// Two rows of 1024 threads with eight vectors each share a CU at 64 registers; one
+// or two of them are in scratch memory, four in the bf16 form with the other classes
+// (13 with a row's sums in vector registers: 2044 x 50257 bf16 108 instead of 106 us a
+// call, 4096 x 30522 fp32 208 instead of 204).
 template <typename T, int NT, int KREG, bool LONG, bool TAIL>
 __global__ __launch_bounds__(NT, (KREG > 8 || LONG ? 4 : NT > 256 ? (NT > 512 ? 8 : 6) : 1)) void top_distil_kernel(
     const TopDistilArgs a) {
@@ -787,7 +793,7 @@ __global__ __launch_bounds__(NT, (KREG > 8 || LONG ? 4 : NT > 256 ? (NT > 512 ? 
   const float gs = a.gscale / (float)scalar_load(a.live);
   // The row's loss, after its gradient (no wavefront waits for it): lq(x) = ln of the student's
   // probability of a logit x, lq_rest that of all tokens without an entry.
-  auto loss = [&](auto lq, auto lq_rest) {
+  auto loss = [&](auto lq, auto lq_rest, float rest, float p_ln_p_off) {
     double term = 0.0;
 #pragma unroll
     for (int i = 0; i < NE; ++i)
@@ -797,10 +803,10 @@ __global__ __launch_bounds__(NT, (KREG > 8 || LONG ? 4 : NT > 256 ? (NT > 512 ? 
       }
     term = block_sum_f64<NW>(term, sh.d);
     if (tid == 0) {
-      term += t.p_ln_p;
-      if (TAIL && t.rest > 0.f) {
+      term += t.p_ln_p - (double)p_ln_p_off;
+      if (TAIL && rest > 0.f) {
         const Float2x l = lq_rest();
-        term -= (double)t.rest * ((double)l.hi + (double)l.lo);
+        term -= (double)rest * ((double)l.hi + (double)l.lo);
       }
       a.row_loss[row] = term;
     }
@@ -852,6 +858,8 @@ __global__ __launch_bounds__(NT, (KREG > 8 || LONG ? 4 : NT > 256 ? (NT > 512 ? 
     if (!(c < kVrNoTerm) && in > 0.f) in = __builtin_inff();
     s = rowsum_block<NW, true>(c, out, in, sh.sums);
     s.ok = s.ok && (t.rest == 0.f || s.z > 1e-30f);
+    // (as scalars: no register of every thread for the length of the row)
+    s = RowSum{same_in_wave(s.c), same_in_wave(s.z), same_in_wave(s.a), s.ok};
   } else {
     s = LONG ? long_sum(r, x, g, kk, sh.sums) : regs_sum(r, g, kk, sh.sums);
   }
@@ -871,7 +879,8 @@ __global__ __launch_bounds__(NT, (KREG > 8 || LONG ? 4 : NT > 256 ? (NT > 512 ? 
         patch([&](float xv) { return fast_exp2(fmaf(xv, kk, c)) * rz; });
       }
     }
-    loss([&](float xv) { return rowsum_log_prob(a.r, s, xv); }, [&]() { return ln_share(log2_2x(rest_z), s.z); });
+    loss([&](float xv) { return rowsum_log_prob(a.r, s, xv); }, [&]() { return ln_share(log2_2x(rest_z), s.z); }, t.rest,
+         0.f);
     return;
   }
   __syncthreads();
@@ -898,21 +907,29 @@ __global__ __launch_bounds__(NT, (KREG > 8 || LONG ? 4 : NT > 256 ? (NT > 512 ? 
   }
   // the rest's share: its sum, moved to the row's maximum, which may underflow where its logarithm does not
   Float2x lq_rest{0.f, 0.f};
+  float rest = t.rest, r_ln_r = 0.f;
   if (TAIL) {
     const Float2x d = two_sum(out.m, -all.m), e = two_mul(d.hi, kk), l = log2_2x(out.z), h = two_sum(e.hi, l.hi);
     if (out.z > 0.f || out.z != out.z)
       lq_rest = ln_share(Float2x{h.hi, h.lo + (l.lo + (e.lo + d.lo * kk))}, all.z);
     else
       lq_rest.hi = -__builtin_inff();
+    // What the teacher leaves to the others is one minus a sum that its log-sum-exp's error moves by as much.
+    // Where it is no more than that, and the student leaves them next to nothing, all there is lies in the
+    // entries (a vocabulary masked to fewer tokens than entries): no r, rather than an r ln(r / q_r) of noise,
+    // infinite where both models cannot reach the others.
+    if (rest > 0.f && rest <= kTopLseError + kTopLseRounding * __builtin_fabsf(scalar_load(a.t_lse + row)) &&
+        lq_rest.hi < kTopOutOfReach) {
+      r_ln_r = rest * (0.69314718f * __builtin_amdgcn_logf(rest));
+      rest = 0.f;
+    }
   }
   if (grow) {
     // The other tokens' q P - r q / q_r by their own maximum: q_r, and with it all of their q, may underflow
     // where q / q_r does not (where their sum is 0 none of them can be reached, and r / q_r is left out).
-    // (As scalars: in vector registers 17 instead of 13 are spilled in the 1024 x 8 form, 4096 x 30522 fp32 226
-    // instead of 208 us a call.)
     const float rz = same_in_wave(1.f / all.z), m = same_in_wave(all.m), off = same_in_wave(TAIL ? out.m : all.m);
     float go = t.whole * rz;
-    if (TAIL) go = go * fast_exp2((off - m) * kk) - (t.rest > 0.f && out.z != 0.f ? t.rest / out.z : 0.f);
+    if (TAIL) go = go * fast_exp2((off - m) * kk) - (rest > 0.f && out.z != 0.f ? rest / out.z : 0.f);
     go = same_in_wave(gs * go);
     if (LONG) {
       leave(off, go, rz, m, 1);
@@ -921,7 +938,7 @@ __global__ __launch_bounds__(NT, (KREG > 8 || LONG ? 4 : NT > 256 ? (NT > 512 ? 
       patch([&](float xv) { return fast_exp2((xv - m) * kk) * rz; });
     }
   }
-  loss([&](float xv) { return vstat_log_prob(a.r, all, xv); }, [&]() { return lq_rest; });
+  loss([&](float xv) { return vstat_log_prob(a.r, all, xv); }, [&]() { return lq_rest; }, rest, r_ln_r);
 }
 
 // The gradient of rows too long for registers, a workgroup per part of a row (one

@@ -108,7 +108,10 @@ def top_logits_distil_loss(s_logits: Tensor, t_values: Tensor, t_indices: Tensor
     kept entries.  With it (of the teacher's ``logits / T``, as ``top_logits``
     returns it) they are the full softmax's, and all other classes form one
     more outcome: what the teacher leaves to them against what the student
-    does (up to 2^20 classes).
+    does (up to 2^20 classes).  What is left over by no more than
+    ``t_logsumexp``'s error, 4e-6 and a rounding, is nothing where the student
+    leaves them less than e^-69 (a vocabulary masked to fewer tokens than
+    entries), and an infinite loss if more is left where it leaves them nothing.
 
     Entries with an index outside the classes are absent and those of value
     -inf weigh nothing; a token named twice counts with both its entries.  Up
