@@ -61,9 +61,11 @@ struct TokenGrad {
 // sums over whole sequences.  The threads' sums are joined and the logarithm is
 // taken in 64 bits as well (the row's registers are free by then): a sequence's
 // sum of differences to a reference that nearly agrees shows every unit of fp32.
-// Rows longer than NT * KREG vectors are walked in pieces of that size.
+// Rows longer than NT * KREG vectors are walked in pieces of that size.  Eight
+// wavefronts a SIMD: 64 registers, which fit (without the bound one type or the
+// other takes 67 to 71, and one workgroup fewer is resident).
 template <typename T, int NT, int KREG>
-__global__ __launch_bounds__(NT) void token_stat_kernel(const TokenRows a, const float* __restrict__ ref,
+__global__ __launch_bounds__(NT, KREG > 4 ? 8 : 1) void token_stat_kernel(const TokenRows a, const float* __restrict__ ref,
                                                         float* __restrict__ logp, double* __restrict__ log_ratio,
                                                         float2* __restrict__ stats, unsigned* __restrict__ ticket) {
   if (ticket && blockIdx.x == 0 && threadIdx.x == 0) *ticket = 0u;  // of the next kernel
@@ -100,14 +102,15 @@ __global__ __launch_bounds__(NT) void token_stat_kernel(const TokenRows a, const
     add(r.t());
   }
   regs_each(r, g, add);
+  float before = 0.f;  // sum over earlier pieces
   for (int64_t v0 = NT * KREG; v0 < g.nvec; v0 += NT * KREG) {
     const int left = g.nvec - v0 < NT * KREG ? (int)(g.nvec - v0) : NT * KREG;
     const VecBuffer piece = vec_buffer(srow + g.head + v0 * VEC, left);
 #pragma unroll
     for (int j = 0; j < KREG; ++j) r.v[j] = vec_load<T>(piece, threadIdx.x + j * NT);
     const float shift = regs_raise(r, left, k, c);
-    s_a = __builtin_amdgcn_ldexpf(fmaf(z, shift, s_a), (int)shift);
-    z = __builtin_amdgcn_ldexpf(z, (int)shift);
+    s_a = __builtin_amdgcn_ldexpf(fmaf(before + z, shift, s_a), (int)shift);
+    long_carry(before, z, (int)shift);
 #pragma unroll
     for (int j = 0; j < KREG; ++j) {
       if ((int)threadIdx.x + j * NT < left) {
@@ -118,7 +121,7 @@ __global__ __launch_bounds__(NT) void token_stat_kernel(const TokenRows a, const
       __builtin_amdgcn_sched_barrier(0);
     }
   }
-  double sum = wave_sum_f64((double)z);
+  double sum = wave_sum_f64((double)before + (double)z);
   s_a = wave_sum(s_a);
   if (NW > 1) {  // (as rowsum_put and rowsum_get do it; s_a = sum of terms times their exponents)
     if (threadIdx.x % kWave == 0) {

@@ -347,8 +347,9 @@ __device__ __forceinline__ bool top_expand(TopShared<NT, KREG>& sh, int k) {
 // when the noted vectors are spread over all threads.
 //
 // MULTI: the row has more than one piece.  Eight wavefronts a SIMD, so 64
-// registers, which the forms of one piece fit; that of several leaves four or five
-// in scratch memory (20 to 24 bytes a thread).  With 80 and six wavefronts 4096 x
+// registers, which the forms of one piece fit; that of several leaves three or four
+// in scratch memory (16 to 20 bytes a thread; with its sum over pieces in a register
+// up to 20, 2048 x 30522 fp32 75 us instead of 61).  With 80 and six wavefronts 4096 x
 // 30522 bf16 took 67 us instead of 58 (55 by now), 1024 x 131072 96 instead of 79
 // (75 by now).
 template <typename T, int NT, int KREG, bool MULTI>
@@ -359,6 +360,7 @@ __global__ __launch_bounds__(NT, NT > 256 ? 8 : 1) void top_logits_kernel(const 
   constexpr int VEC = Vec16<T>::N;
   typedef RawMax<T> Raw;
   __shared__ TopShared<NT, KREG> sh;
+  __shared__ float before[MULTI ? NT : 1];  // each thread's sum over earlier pieces, added to without a register
   const int64_t row = blockIdx.x, V = a.V;
   const T* x = vocab_row<T>(a, row);
   const VocabGeom g = vocab_geom(x, V);
@@ -394,6 +396,10 @@ __global__ __launch_bounds__(NT, NT > 256 ? 8 : 1) void top_logits_kernel(const 
       for (int i = 0; i < VEC; ++i) add(to_f32(r.v[j].v[i]));
     }
     __builtin_amdgcn_sched_barrier(0);
+  }
+  if (MULTI) {
+    before[tid] = z;
+    z = 0.f;
   }
   auto publish = [&](auto group_max) {
     uint32_t whole = r.has_h || r.has_t ? top_key(fmaxf(r.h(), r.t())) : 0u;
@@ -512,8 +518,11 @@ __global__ __launch_bounds__(NT, NT > 256 ? 8 : 1) void top_logits_kernel(const 
       __builtin_amdgcn_sched_barrier(0);
     }
     if (!MULTI || after == 0) break;
+    __hip_atomic_fetch_add(&before[tid], z, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+    z = 0.f;
     if ((v0 / (NT * KREG)) % 2 == 1) fits = top_expand<T, false, MULTI>(sh, k);
   }
+  if (MULTI) z += before[tid];
   const RowSum mine = rowsum_put<NT / kWave, false>(c, z, 0.f, sh.sums);
   fits = fits && top_expand<T, true, MULTI>(sh, k);
   const RowSum s = rowsum_get<NT / kWave, false>(mine, sh.sums);
@@ -838,9 +847,11 @@ __global__ __launch_bounds__(NT, (KREG > 8 || LONG ? 4 : NT > 256 ? (NT > 512 ? 
       }
     };
     if (LONG) {
+      float before = 0.f;
       long_each(
           r, x, g, [&](const Vec16<T>& v, int64_t at) { add(v, (uint32_t)at); },
-          [&](int left) { out = __builtin_amdgcn_ldexpf(out, (int)regs_raise(r, left, kk, c)); });
+          [&](int left) { long_carry(before, out, (int)regs_raise(r, left, kk, c)); });
+      out += before;
     } else {
 #pragma unroll
       for (int j = 0; j < KREG; ++j) {
@@ -887,13 +898,14 @@ __global__ __launch_bounds__(NT, (KREG > 8 || LONG ? 4 : NT > 256 ? (NT > 512 ? 
   // Rows whose sums need the true maximum: walked.
   VocabStat out = vstat_init(), all;
   if (TAIL) {
+    VocabStatSum others;
     for (int64_t i = tid; i < V; i += NT) {
       const uint32_t bit = top_mark_bit((int)i, g);
       if ((marks[bit >> 5] >> (bit & 31)) & 1u) continue;
       float x1[1] = {to_f32(x[i])};
-      vstat_fold<1>(out, x1, kk);
+      others.add(x1, kk);
     }
-    out = vstat_block<NW>(out, kk, sh.stats);
+    out = vstat_block<NW>(others.whole(kk), kk, sh.stats);
     VocabStat in = vstat_init();
 #pragma unroll
     for (int i = 0; i < NE; ++i)

@@ -206,29 +206,48 @@ __device__ __forceinline__ VocabGeom vocab_geom(const T* row, int64_t V) {
   return g;
 }
 
+// Statistics of many elements: 64 at a time, and those of these.  (A sum of n terms
+// is off by up to n 2^-25 of itself where logits are coarse and every addition rounds
+// the same way: 1e-5 for 300.)
+struct VocabStatSum {
+  VocabStat s = vstat_init(), before = vstat_init();
+  int n = 0;
+  template <int N>
+  __device__ __forceinline__ void add(const float (&x)[N], float k) {
+    vstat_fold<N>(s, x, k);
+    n += N;
+    if (n >= 64) {
+      before = vstat_merge(before, s, k);
+      s.z = 0.f;
+      n = 0;
+    }
+  }
+  __device__ __forceinline__ VocabStat whole(float k) const { return vstat_merge(before, s, k); }
+};
+
 // This thread's share of the row's statistics when NT threads walk it.
 template <typename T, int NT>
 __device__ __forceinline__ VocabStat vocab_stat_walk(const T* row, int64_t V, float k) {
   constexpr int VEC = Vec16<T>::N;
   const VocabGeom g = vocab_geom(row, V);
-  VocabStat s = vstat_init();
+  VocabStatSum s;
   float x1[1];
   if ((int)threadIdx.x < g.head) {
     x1[0] = to_f32(row[threadIdx.x]);
-    vstat_fold<1>(s, x1, k);
+    s.add(x1, k);
   }
   if (g.tail0 + threadIdx.x < V) {
     x1[0] = to_f32(row[g.tail0 + threadIdx.x]);
-    vstat_fold<1>(s, x1, k);
+    s.add(x1, k);
   }
   for (int64_t v = threadIdx.x; v < g.nvec; v += NT) {
     const Vec16<T> r = load16(row + g.head + v * VEC);
     float x[VEC];
 #pragma unroll
     for (int i = 0; i < VEC; ++i) x[i] = to_f32(r.v[i]);
-    vstat_fold<VEC>(s, x, k);
+    s.add(x, k);
   }
-  return s;
+  return s.whole(k);
 }
 
 // grad[j] = f(x[j], j) over a row; the gradient row may be aligned differently.
@@ -661,11 +680,18 @@ __device__ __forceinline__ void long_each(RowRegs<T, NT, KREG>& r, const T* row,
   }
 }
 
+// A sum over such a row's pieces, of one piece's sum at a time (see VocabStatSum):
+// to = (to + z) 2^shift, and z starts again.
+__device__ __forceinline__ void long_carry(float& to, float& z, int shift) {
+  to = __builtin_amdgcn_ldexpf(to + z, shift);
+  z = 0.f;
+}
+
 // regs_sum of such rows.
 template <typename T, int NT, int KREG>
 __device__ __forceinline__ RowSum long_sum(RowRegs<T, NT, KREG>& r, const T* row, const VocabGeom& g, float k, RowSum* lds) {
   constexpr int VEC = Vec16<T>::N;
-  float c = regs_anchor<true>(r, g, k), z = 0.f;
+  float c = regs_anchor<true>(r, g, k), before = 0.f, z = 0.f;
   auto add = [&](float x) { z += fast_exp2(fmaf(x, k, c)); };
   if (threadIdx.x < kWave) {
     add(r.h());
@@ -677,8 +703,8 @@ __device__ __forceinline__ RowSum long_sum(RowRegs<T, NT, KREG>& r, const T* row
 #pragma unroll
         for (int i = 0; i < VEC; ++i) add(to_f32(v.v[i]));
       },
-      [&](int left) { z = __builtin_amdgcn_ldexpf(z, (int)regs_raise(r, left, k, c)); });
-  return rowsum_block<NT / kWave, false>(c, z, 0.f, lds);
+      [&](int left) { long_carry(before, z, (int)regs_raise(r, left, k, c)); });
+  return rowsum_block<NT / kWave, false>(c, before + z, 0.f, lds);
 }
 
 // This thread's share of sum(v[0..n)) when NT threads walk the array together, in
